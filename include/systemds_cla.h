@@ -268,6 +268,106 @@ int64_t cla_comm_destroy(int64_t comm);
 int64_t cla_group_decode(cla_handle h, int32_t g, int32_t* ids);
 int64_t cla_group_counts(cla_handle h, int32_t g, int64_t* counts);
 
+/* ---- dense operators beside the compressed products ---------------------------------------------
+ * What follows a compressed product in a model's training and scoring: the hidden layer of a gated feed-forward block with its
+ * gradients, dropout, and products in 8-bit integers. They have no counterpart in the reference. Matrices are device memory in rows
+ * of `ld` elements (ld >= the row's length; rows need no alignment), types CLA_T_*; sums are 32 bits or wider. Calls enqueue
+ * on `stream` of `device` and return CLA_OK without waiting or allocating; the current device stays what it was. Calls share nothing:
+ * any number may run at once on any streams, captured or not, as long as their buffers differ. `work` is the caller's, 256-byte aligned,
+ * of the size that the *_workspace function gives for the same arguments (0: none needed, work may be NULL); a call uses it until its
+ * kernels are done. Outputs may not overlap inputs, but for dropout onto its own input. Every result repeats bit for bit. Elements of a row behind its length, and rows behind
+ * the last, are neither read for a result nor written. A kernel's self-check that trips (a wait that ran out) is reported by cla_dense_status. */
+#define CLA_T_F64 0
+#define CLA_T_F32 1
+#define CLA_T_BF16 2
+#define CLA_T_F16 3
+#define CLA_T_I8 4
+
+#define CLA_ACT_SILU 0      /* g / (1 + exp(-g)) */
+#define CLA_ACT_GELU 1      /* g / 2 (1 + erf(g / sqrt 2)) */
+#define CLA_ACT_GELU_TANH 2 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
+#define CLA_ACT_RELU 3      /* max(g, 0) */
+#define CLA_ACT_SIGMOID 4   /* 1 / (1 + exp(-g)) */
+
+/* Dropout: element (row, col) is kept where word >= floor(p 2^32), and multiplied by 1 / (1 - p); else it becomes 0, whatever it was.
+ * word = Philox4x32-10 (Salmon et al. 2011) of key `seed` and counter (col / 4, row0 + row, step), its word col % 4: the mask is never stored,
+ * the same (seed, step) draw it again for the gradient, and a shard that passes its first row as row0 draws its part of the
+ * whole matrix's mask. 0 <= p < 1 (0: everything is kept and nothing is drawn); row0 + rows <= 2^32. */
+typedef struct cla_drop {
+  double p;
+  uint64_t seed, step;
+  int64_t row0;
+} cla_drop;
+/* y = dropout(x), element by element: forward, and backward of the same (seed, step). x and y of one type (F64, F32, BF16, F16). */
+int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t cols, void* y, int64_t ldy, const cla_drop* drop,
+                        int32_t device, void* stream);
+
+/* Quantises rows (byCols 0) or columns (1) of x [rows x cols] (F64, F32, BF16, F16): scale[i] = fl32(largest magnitude / 127), q = x / scale[i]
+ * to the nearest whole number (even on ties, within -127..127; the division in FP64 for F64, else FP32). Where scale[i] is 0 or not finite q
+ * is 0: a row of zeros gives zeros, one with an infinity or a NaN gives NaN in the product. byCols 0: q [rows x cols];
+ * byCols 1: q [cols x rows], a row per column of x, as cla_q8_mm_dev takes weights. ldq: elements between the rows of q. */
+int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t byCols, int8_t* q, int64_t ldq,
+                            float* scale, int32_t device, void* stream);
+
+/* out[m, n] = aScale[m] * bScale[n] * sum over k of a[m, k] * b[n, k], the sum exact in 32-bit integers, K <= 131071. aType CLA_T_I8, or a
+ * floating type: a's rows are then quantised in the call as cla_q8_quantize_dev does (aScale unused). Scaled in FP64 for
+ * outType F64, else in FP32, and rounded once to outType. */
+typedef struct cla_q8 {
+  int64_t M, N, K;
+  const void* a;
+  int64_t lda;
+  const float* aScale;
+  const int8_t* b;
+  int64_t ldb;
+  const float* bScale;
+  void* out;
+  int64_t ldo;
+  void* work;
+  int64_t workBytes;
+  int32_t aType, outType, device;
+} cla_q8;
+int64_t cla_q8_workspace(const cla_q8* args);
+int64_t cla_q8_mm_dev(const cla_q8* args, void* stream);
+
+/* The gated feed-forward block on x [M x D] with weights wg, wu [D x F]; type BF16 or F16 for all matrices, act CLA_ACT_*.
+ * Forward: g = x wg, u = x wu, h = dropout(act(g) * u) [M x F] in one kernel; g and u are written too where the pointers are not NULL (both or
+ * neither), as the backward call takes them.
+ * Backward: from dh [M x F] and the saved g, u: with dh' = dropout(dh) of the same (seed, step), du = dh' act(g), dg = dh' u act'(g),
+ * dx = dg t(wg) + du t(wu), dwg = t(x) dg, dwu = t(x) du. dx or both of dwg, dwu may be NULL (not wanted). dg and du are
+ * rounded to the type before the products, which take operands of that type.
+ * wTrans 1: wg and wu are stored transposed, as [F x D] rows of ldwg, ldwu elements. dwg and dwu are [D x F] in any case. */
+typedef struct cla_gated {
+  int64_t M, D, F;
+  const void *x, *wg, *wu;
+  int64_t ldx, ldwg, ldwu;
+  void *h, *g, *u;
+  int64_t ldh, ldg, ldu;
+  const void* dh;
+  int64_t lddh;
+  void *dx, *dwg, *dwu;
+  int64_t lddx, lddwg, lddwu;
+  void* work;
+  int64_t workBytes;
+  cla_drop drop;
+  int32_t type, act, wTrans, device;
+} cla_gated;
+int64_t cla_gated_workspace(const cla_gated* args, int32_t backward);
+int64_t cla_gated_fwd_dev(const cla_gated* args, void* stream);
+int64_t cla_gated_bwd_dev(const cla_gated* args, void* stream);
+
+/* Rows [row0, row0 + rows) of a block in type F64, F32, BF16 or F16 (rounded once from FP64): what the gated block and the 8-bit product take
+ * of a compressed matrix. cla_q8_rmm_dev: X in 8 bits times b, i.e. cla_q8_mm_dev with the block's rows as a. Both go through the rows in
+ * chunks of what fits `work` (as the workspace functions say, or more; fewer, larger chunks are faster) and follow
+ * the handle's rules for streams. */
+int64_t cla_rows_workspace(cla_handle h, int64_t rows, int32_t type);
+int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_t type, void* out, int64_t ldo, void* work, int64_t workBytes,
+                                void* stream);
+int64_t cla_q8_rmm_workspace(cla_handle h, int64_t N);
+int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* bScale, int64_t N, int32_t outType, void* out, int64_t ldo,
+                       void* work, int64_t workBytes, void* stream);
+/* Waits for the device and reports (CLA_ERR_DEVICE_CHECK) a self-check that tripped in one of the dense calls above since the last look. */
+int64_t cla_dense_status(int32_t device);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,4 +5,11 @@ from .cmb import (CHAIN_XtXv, CHAIN_XtwXv, CLALibDecompress, CLALibLeftMultBy, C
 from .native import CLAError
 
 __all__ = ["CompressedMatrixBlock", "CLALibRightMultBy", "CLALibLeftMultBy", "CLALibTSMM", "CLALibMMChain",
-           "CLALibDecompress", "CLALibMatrixMult", "CLAError", "CHAIN_XtXv", "CHAIN_XtwXv"]
+           "CLALibDecompress", "CLALibMatrixMult", "CLALibQ8", "CLALibGated", "CLALibDropout", "CLAError", "CHAIN_XtXv", "CHAIN_XtwXv"]
+
+
+def __getattr__(name):  # (the dense operators take torch tensors: torch is imported when one of them is asked for)
+    if name in ("CLALibQ8", "CLALibGated", "CLALibDropout"):
+        from . import dense
+        return getattr(dense, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

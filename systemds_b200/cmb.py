@@ -412,3 +412,20 @@ class CLALibDecompress:
         out = np.empty((cmb.rlen, cmb.clen), np.float64)
         nnz = check(native.lib().cla_decompress(cmb.handle(), ptr(out)))
         return _wrap(out, nnz)
+
+    @staticmethod
+    def rows(cmb: CompressedMatrixBlock, row0: int, rows: int, dtype, out=None):
+        """Rows ``[row0, row0 + rows)`` as a torch tensor on the block's device, rounded once to ``dtype`` (float64, float32, bfloat16,
+        float16): what the dense operators take of a compressed block."""
+        import torch
+        from .dense import _result, _rows, _stream, _type, _workspace
+        h, t = cmb.handle(), _type(dtype, "rows of a block")
+        dev = torch.device("cuda", cmb.device)
+        if row0 < 0 or rows < 0 or row0 + rows > cmb.rlen:
+            raise native.CLAError(-4, "rows of a block: outside the matrix")
+        y = _result(out, (rows, cmb.clen), dtype, dev, "rows of a block, out")
+        py, ldo = _rows(y, "rows of a block, out", dtype, dev)
+        n = check(native.lib().cla_rows_workspace(h, rows, t))
+        work = _workspace(n, dev)
+        check(native.lib().cla_decompress_rows_dev(h, row0, rows, t, py, ldo, work.data_ptr() if n else None, n, _stream(cmb.device)))
+        return y

@@ -1,0 +1,657 @@
+// Dense operators beside the compressed products (cla_*_dev of include/systemds_cla.h): dropout, quantisation to 8 bits, products in 8 bits,
+// the gated feed-forward block with its gradients. Their products are in cla_gemm.cu; here are the entry points and the kernels that
+// go once over a matrix, all bound by memory.
+#include "cla_dense.cuh"
+#include <algorithm>
+#include <cmath>
+
+namespace cla {
+
+std::shared_ptr<Matrix> lookup(cla_handle h);
+
+constexpr int DN_T = 256;
+
+// 16 bytes of a row of T: vectors where every row starts on a 16-byte boundary, else element by element
+template <class T> constexpr int DN_V = 16 / (int)sizeof(T);
+template <class T>
+__device__ __forceinline__ void load_vec(const T* p, int n, bool vec, T (&v)[DN_V<T>]) {
+  if (vec && n == DN_V<T>) {
+    *(uint4*)v = *(const uint4*)p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < DN_V<T>; i++) v[i] = i < n ? p[i] : from_f32<T>(0.f);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_vec(T* p, int n, bool vec, const T (&v)[DN_V<T>]) {
+  if (vec && n == DN_V<T>) {
+    *(uint4*)p = *(const uint4*)v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < DN_V<T>; i++)
+      if (i < n) p[i] = v[i];
+  }
+}
+inline bool rows_aligned(const void* p, int64_t ld, int64_t rows, int bytes, int to = 16) {
+  return ((uintptr_t)p % to) == 0 && (rows <= 1 || (ld * bytes) % to == 0);
+}
+
+// ---- dropout --------------------------------------------------------------------------------------------------------
+// A thread per 16 bytes of a row (F64: 32, the four columns of a counter). Bound: memory; the ten rounds are 40 multiplications for 4 columns.
+template <class T>
+__global__ void __launch_bounds__(DN_T) k_dropout(const T* x, int64_t ldx, int64_t rows, int64_t cols, T* y, int64_t ldy,
+                                                  const __grid_constant__ DropDev d, int vec) {
+  constexpr int V = DN_V<T> < 4 ? 4 : DN_V<T>;
+  const int64_t per = (cols + V - 1) / V, n = per * rows;
+  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
+    const int64_t r = i / per, c = (i - r * per) * V;
+#pragma unroll
+    for (int h = 0; h < V; h += DN_V<T>) {
+      const int left = (int)min((int64_t)DN_V<T>, cols - c - h);
+      if (left <= 0) break;
+      alignas(16) T v[DN_V<T>];
+      load_vec(x + r * ldx + c + h, left, vec, v);
+      if (d.on) {
+#pragma unroll
+        for (int q = 0; q < DN_V<T>; q += 4) {
+          const uint4 w = drop_words(d, (uint32_t)r, (uint32_t)((c + h + q) / 4));
+#pragma unroll
+          for (int j = 0; j < (DN_V<T> < 4 ? DN_V<T> : 4); j++) {
+            const bool keep = word_of(w, DN_V<T> < 4 ? h + j : j) >= d.cut;
+            if constexpr (sizeof(T) == 8) v[q + j] = keep ? v[q + j] * d.scale64 : 0.0;
+            else v[q + j] = from_f32<T>(keep ? to_f32(v[q + j]) * d.scale : 0.f);
+          }
+        }
+      }
+      store_vec(y + r * ldy + c + h, left, vec, v);
+    }
+  }
+}
+
+// ---- quantisation -----------------------------------------------------------------------------------------------------
+template <class T> struct WideOf { using type = float; };
+template <> struct WideOf<double> { using type = double; };
+template <class T> __device__ __forceinline__ typename WideOf<T>::type widen(T v) { return to_f32(v); }
+template <> __device__ __forceinline__ double widen(double v) { return v; }
+
+template <class W> __device__ __forceinline__ W larger(W m, W a) { return a > m || a != a ? a : m; }  // (a NaN stays)
+template <class W> __device__ __forceinline__ float q8_scale(W most) { return (float)(most / (W)127); }
+// (divided, not multiplied by a reciprocal: the result is the nearest whole number of the quotient itself)
+template <class W> __device__ __forceinline__ int q8_of(W x, float scale, bool some) {
+  return some ? (int)fmin((W)127, fmax((W)-127, rint(x / (W)scale))) : 0;
+}
+
+// G threads per row: its largest magnitude, then, from the caches, its quotients. Bound: memory, one pass over x.
+template <class T, int G>
+__global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, int8_t* __restrict__ q,
+                                                        int64_t ldq, float* __restrict__ scale, int vec, int vecQ) {
+  using W = typename WideOf<T>::type;
+  constexpr int V = DN_V<T>;
+  __shared__ W part[DN_T / 32];
+  const int lane = threadIdx.x % G, warp = threadIdx.x / 32;
+  const int64_t r = (int64_t)blockIdx.x * (DN_T / G) + threadIdx.x / G;
+  if (G == 32 && r >= rows) return;
+  const T* p = x + r * ldx;
+  W most = 0;
+  for (int64_t c = (int64_t)lane * V; c < cols; c += G * V) {
+    alignas(16) T v[V];
+    load_vec(p + c, (int)min((int64_t)V, cols - c), vec, v);
+#pragma unroll
+    for (int i = 0; i < V; i++) most = larger(most, (W)fabs(widen(v[i])));
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
+  if (G > 32) {
+    if (threadIdx.x % 32 == 0) part[warp] = most;
+    __syncthreads();
+    most = part[0];
+#pragma unroll
+    for (int i = 1; i < DN_T / 32; i++) most = larger(most, part[i]);
+  }
+  const float s = q8_scale(most);
+  const bool some = s > 0.f && s < INFINITY;
+  if (lane == 0) scale[r] = s;
+  for (int64_t c = (int64_t)lane * V; c < cols; c += G * V) {
+    alignas(16) T v[V];
+    const int n = (int)min((int64_t)V, cols - c);
+    load_vec(p + c, n, vec, v);
+    alignas(16) int8_t o[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] = (int8_t)q8_of(widen(v[i]), s, some);
+    int8_t* t = q + r * ldq + c;
+    if (vecQ && n == V) {
+      if constexpr (V == 8) *(uint2*)t = *(const uint2*)o;
+      else if constexpr (V == 4) *(uint32_t*)t = *(const uint32_t*)o;
+      else *(uint16_t*)t = *(const uint16_t*)o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (i < n) t[i] = o[i];
+    }
+  }
+}
+
+// 32 columns per CTA, 32 threads down each: the columns' largest magnitudes, then their quotients, turned in shared memory.
+template <class T>
+__global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, int8_t* __restrict__ q,
+                                                        int64_t ldq, float* __restrict__ scale) {
+  using W = typename WideOf<T>::type;
+  __shared__ W part[32][33];
+  __shared__ float sc[32];
+  __shared__ int8_t tile[32][132];
+  const int tx = threadIdx.x, ty = threadIdx.y;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+  W most = 0;
+  if (c < cols)
+    for (int64_t r = ty; r < rows; r += 32) most = larger(most, (W)fabs(widen(x[r * ldx + c])));
+  part[ty][tx] = most;
+  __syncthreads();
+  if (ty == 0) {
+    for (int i = 1; i < 32; i++) most = larger(most, part[i][tx]);
+    sc[tx] = q8_scale(most);
+    if (c < cols) scale[c] = sc[tx];
+  }
+  __syncthreads();
+  const float s = sc[tx];
+  const bool some = s > 0.f && s < INFINITY;
+  for (int64_t r0 = 0; r0 < rows; r0 += 128) {
+#pragma unroll
+    for (int i = 0; i < 128; i += 32) {
+      const int64_t r = r0 + i + ty;
+      tile[tx][i + ty] = c < cols && r < rows ? (int8_t)q8_of(widen(x[r * ldx + c]), s, some) : 0;
+    }
+    __syncthreads();
+    const int64_t oc = (int64_t)blockIdx.x * 32 + ty;
+    if (oc < cols)
+#pragma unroll
+      for (int i = 0; i < 128; i += 32)
+        if (r0 + i + tx < rows) q[oc * ldq + r0 + i + tx] = tile[ty][i + tx];
+    __syncthreads();
+  }
+}
+
+// ---- the gated block's elementwise gradients ----------------------------------------------------------------------------
+template <class T>
+__global__ void __launch_bounds__(DN_T) k_gate_grad(const T* __restrict__ dh, int64_t lddh, const T* __restrict__ g, int64_t ldg,
+                                                    const T* __restrict__ u, int64_t ldu, int64_t rows, int64_t cols, T* __restrict__ dg,
+                                                    T* __restrict__ du, int64_t ldo, const __grid_constant__ DropDev d, int act, int vec) {
+  constexpr int V = DN_V<T>;
+  const int64_t per = (cols + V - 1) / V, n = per * rows;
+  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
+    const int64_t r = i / per, c = (i - r * per) * V;
+    const int left = (int)min((int64_t)V, cols - c);
+    alignas(16) T vh[V], vg[V], vu[V];
+    load_vec(dh + r * lddh + c, left, vec, vh);
+    load_vec(g + r * ldg + c, left, vec, vg);
+    load_vec(u + r * ldu + c, left, vec, vu);
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+      uint4 w;
+      if (d.on) w = drop_words(d, (uint32_t)r, (uint32_t)((c + q) / 4));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        float h = to_f32(vh[q + j]), a;
+        if (d.on) h = word_of(w, j) >= d.cut ? h * d.scale : 0.f;
+        const float slope = act_slope(act, to_f32(vg[q + j]), a);
+        vg[q + j] = from_f32<T>(h * to_f32(vu[q + j]) * slope);
+        vu[q + j] = from_f32<T>(h * a);
+      }
+    }
+    store_vec(dg + r * ldo + c, left, true, vg);
+    store_vec(du + r * ldo + c, left, true, vu);
+  }
+}
+
+// ---- copies -----------------------------------------------------------------------------------------------------------
+// Rows to rows that start on 16-byte boundaries, as the products read them: a thread per 16 bytes.
+template <class T>
+__global__ void __launch_bounds__(DN_T) k_repitch(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, T* __restrict__ y, int64_t ldy) {
+  constexpr int V = DN_V<T>;
+  const int64_t per = (cols + V - 1) / V, n = per * rows;
+  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
+    const int64_t r = i / per, c = (i - r * per) * V;
+    alignas(16) T v[V];
+    const int left = (int)min((int64_t)V, cols - c);
+    load_vec(x + r * ldx + c, left, false, v);
+    store_vec(y + r * ldy + c, left, true, v);
+  }
+}
+template <class T>
+__global__ void __launch_bounds__(DN_T) k_narrow(const double* __restrict__ x, int64_t rows, int64_t cols, T* __restrict__ y, int64_t ldy) {
+  const int64_t n = rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
+    const int64_t r = i / cols;
+    y[r * ldy + i - r * cols] = from_f64<T>(x[i]);
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+namespace {
+
+// The call's device is current while it lives, then the caller's again
+struct OnDevice {
+  int before = -1;
+  int64_t rc = CLA_OK;
+  explicit OnDevice(int device) {
+    int now = -1;
+    cudaError_t e = cudaGetDevice(&now);
+    if (e == cudaSuccess && now != device) {
+      e = cudaSetDevice(device);
+      if (e == cudaSuccess) before = now;
+    }
+    if (e != cudaSuccess) rc = fail(CLA_ERR_CUDA, std::string("device of a dense call: ") + cudaGetErrorString(e));
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+unsigned blocks_for(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + DN_T - 1) / DN_T, 148 * 16)); }
+
+int64_t check_matrix(const char* what, const void* p, int64_t rows, int64_t cols, int64_t ld, int bytes) {
+  if (rows < 0 || cols < 0) return fail(CLA_ERR_SHAPE, std::string(what) + ": negative size");
+  if (rows > INT32_MAX || cols > INT32_MAX) return fail(CLA_ERR_UNSUPPORTED, std::string(what) + ": more than 2^31 - 1 rows or columns");
+  if (rows == 0 || cols == 0) return CLA_OK;
+  if (!p) return fail(CLA_ERR_BAD_ARG, std::string(what) + ": null buffer");
+  if (ld < cols) return fail(CLA_ERR_SHAPE, std::string(what) + ": rows overlap (ld below the row's length)");
+  if (ld > (int64_t)1 << 38) return fail(CLA_ERR_UNSUPPORTED, std::string(what) + ": rows too far apart");
+  if ((uintptr_t)p % bytes) return fail(CLA_ERR_BAD_ARG, std::string(what) + ": address not a multiple of the element size");
+  return CLA_OK;
+}
+#define DN_CHECK(...)                                     \
+  do {                                                    \
+    if (const int64_t rc_ = (__VA_ARGS__); rc_ < 0) return rc_; \
+  } while (0)
+
+int64_t drop_device(const cla_drop& d, int64_t rows, DropDev& o) {
+  if (!(d.p >= 0.0 && d.p < 1.0)) return fail(CLA_ERR_BAD_ARG, "dropout: p must be at least 0 and below 1");
+  if (d.row0 < 0 || d.row0 + rows > (int64_t)1 << 32) return fail(CLA_ERR_BAD_ARG, "dropout: rows beyond 2^32");
+  o.on = d.p > 0.0;
+  o.cut = (uint32_t)std::floor(d.p * 4294967296.0);
+  o.row0 = (uint32_t)d.row0;
+  o.seed[0] = (uint32_t)d.seed, o.seed[1] = (uint32_t)(d.seed >> 32);
+  o.step[0] = (uint32_t)d.step, o.step[1] = (uint32_t)(d.step >> 32);
+  o.scale64 = 1.0 / (1.0 - d.p);
+  o.scale = (float)o.scale64;
+  return CLA_OK;
+}
+bool is_float_type(int t) { return t == CLA_T_F64 || t == CLA_T_F32 || t == CLA_T_BF16 || t == CLA_T_F16; }
+
+// Calls f with a pointer of the type: f(T())
+template <class F> void with_type(int type, F&& f) {
+  if (type == CLA_T_F64) f(double());
+  else if (type == CLA_T_F32) f(float());
+  else if (type == CLA_T_BF16) f(__nv_bfloat16());
+  else f(__half());
+}
+
+int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t cols, bool byCols, int8_t* q, int64_t ldq, float* scale,
+                 cudaStream_t s) {
+  if ((byCols ? cols : rows) == 0) return CLA_OK;
+  with_type(type, [&](auto t) {
+    using T = decltype(t);
+    if (byCols) {
+      k_quantize_cols<T><<<(unsigned)((cols + 31) / 32), dim3(32, 32), 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale);
+      return;
+    }
+    const int vec = rows_aligned(x, ldx, rows, sizeof(T)), vecQ = rows_aligned(q, ldq, rows, 1, DN_V<T>);
+    // rows of up to 8 vectors a lane: a warp each, no barrier; longer ones a CTA each
+    if (cols <= 32 * 8 * DN_V<T> && rows >= 148)
+      k_quantize_rows<T, 32><<<(unsigned)((rows + DN_T / 32 - 1) / (DN_T / 32)), DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec, vecQ);
+    else
+      k_quantize_rows<T, DN_T><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec, vecQ);
+  });
+  CLA_CUDA(cudaGetLastError());
+  return CLA_OK;
+}
+
+// Hands out parts of the caller's workspace; with a null base it only counts
+struct Work {
+  char* p;
+  int64_t used = 0;
+  void* take(int64_t bytes) {
+    void* r = p ? p + used : nullptr;
+    used += round_up(bytes, 256);
+    return r;
+  }
+};
+// The operand as the products read it: itself, or a copy in the workspace where its rows do not start on 16-byte boundaries.
+int64_t aligned(GemmOperand& o, int64_t i, int64_t k, int type, Work& w, bool run, cudaStream_t s) {
+  const int bytes = type_bytes(type);
+  const int64_t rows = o.mn ? k : i, cols = o.mn ? i : k;
+  if (rows <= 1 && (uintptr_t)o.p % 16 == 0) o.ld = round_up(o.ld, 16 / bytes);  // (no second row)
+  if (rows_aligned(o.p, o.ld, 2, bytes)) return CLA_OK;
+  const int64_t ld = round_up(cols, 16 / bytes);
+  void* to = w.take(rows * ld * bytes);
+  if (run && rows && cols) {
+    const unsigned b = blocks_for(rows * ((cols * bytes + 15) / 16));
+    if (bytes == 1) k_repitch<int8_t><<<b, DN_T, 0, s>>>((const int8_t*)o.p, o.ld, rows, cols, (int8_t*)to, ld);
+    else k_repitch<__half><<<b, DN_T, 0, s>>>((const __half*)o.p, o.ld, rows, cols, (__half*)to, ld);
+    CLA_CUDA(cudaGetLastError());
+  }
+  o.p = to;
+  o.ld = ld;
+  return CLA_OK;
+}
+
+int64_t check_q8(const cla_q8* c) {
+  if (!c) return fail(CLA_ERR_BAD_ARG, "8-bit product: null arguments");
+  if (c->aType != CLA_T_I8 && !is_float_type(c->aType)) return fail(CLA_ERR_UNSUPPORTED, "8-bit product: type of a");
+  if (!is_float_type(c->outType)) return fail(CLA_ERR_UNSUPPORTED, "8-bit product: type of the result");
+  if (c->K > 131071) return fail(CLA_ERR_UNSUPPORTED, "8-bit product: more than 131071 terms may leave 32 bits");
+  DN_CHECK(check_matrix("8-bit product, a", c->a, c->M, c->K, c->lda, type_bytes(c->aType)));
+  DN_CHECK(check_matrix("8-bit product, b", c->b, c->N, c->K, c->ldb, 1));
+  DN_CHECK(check_matrix("8-bit product, result", c->out, c->M, c->N, c->ldo, type_bytes(c->outType)));
+  if (c->M && c->N && ((c->aType == CLA_T_I8 && !c->aScale) || !c->bScale)) return fail(CLA_ERR_BAD_ARG, "8-bit product: null scales");
+  return CLA_OK;
+}
+int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s) {
+  GemmCall g;
+  g.kind = GK_Q8;
+  g.type = CLA_T_I8;
+  g.outType = c.outType;
+  g.M = c.M, g.N = c.N, g.K = c.K;
+  g.a[0] = {c.a, c.lda, false};
+  g.b[0] = {c.b, c.ldb, false};
+  g.out[0] = c.out, g.ldo[0] = c.ldo;
+  g.aScale = c.aScale, g.bScale = c.bScale;
+  g.device = c.device;
+  if (c.M == 0 || c.N == 0) return CLA_OK;
+  if (c.aType != CLA_T_I8) {
+    const int64_t ld = round_up(c.K, 16);
+    int8_t* q = (int8_t*)w.take(c.M * ld);
+    float* sc = (float*)w.take(c.M * 4);
+    if (run) DN_CHECK(quantize(c.aType, c.a, c.lda, c.M, c.K, false, q, ld, sc, s));
+    g.a[0] = {q, ld, false};
+    g.aScale = sc;
+  } else {
+    DN_CHECK(aligned(g.a[0], c.M, c.K, CLA_T_I8, w, run, s));
+  }
+  DN_CHECK(aligned(g.b[0], c.N, c.K, CLA_T_I8, w, run, s));
+  return run ? launch_gemm(g, s) : CLA_OK;
+}
+
+int64_t check_gated(const cla_gated* c, bool backward, DropDev& d) {
+  if (!c) return fail(CLA_ERR_BAD_ARG, "gated block: null arguments");
+  if (c->type != CLA_T_BF16 && c->type != CLA_T_F16) return fail(CLA_ERR_UNSUPPORTED, "gated block: types BF16 and F16");
+  if (c->act < CLA_ACT_SILU || c->act > CLA_ACT_SIGMOID) return fail(CLA_ERR_UNSUPPORTED, "gated block: unknown activation");
+  if (c->wTrans != 0 && c->wTrans != 1) return fail(CLA_ERR_BAD_ARG, "gated block: wTrans is 0 or 1");
+  const int64_t wr = c->wTrans ? c->F : c->D, wc = c->wTrans ? c->D : c->F;
+  DN_CHECK(check_matrix("gated block, x", c->x, c->M, c->D, c->ldx, 2));
+  DN_CHECK(check_matrix("gated block, wg", c->wg, wr, wc, c->ldwg, 2));
+  DN_CHECK(check_matrix("gated block, wu", c->wu, wr, wc, c->ldwu, 2));
+  DN_CHECK(drop_device(c->drop, c->M, d));
+  if (!backward) {
+    DN_CHECK(check_matrix("gated block, h", c->h, c->M, c->F, c->ldh, 2));
+    if (!c->g != !c->u) return fail(CLA_ERR_BAD_ARG, "gated block: g and u go together");
+    if (!c->g) return CLA_OK;
+  } else {
+    DN_CHECK(check_matrix("gated block, dh", c->dh, c->M, c->F, c->lddh, 2));
+    if (!c->dwg != !c->dwu) return fail(CLA_ERR_BAD_ARG, "gated block: dwg and dwu go together");
+    if (c->dx) DN_CHECK(check_matrix("gated block, dx", c->dx, c->M, c->D, c->lddx, 2));
+    if (c->dwg) {
+      DN_CHECK(check_matrix("gated block, dwg", c->dwg, c->D, c->F, c->lddwg, 2));
+      DN_CHECK(check_matrix("gated block, dwu", c->dwu, c->D, c->F, c->lddwu, 2));
+    }
+  }
+  DN_CHECK(check_matrix("gated block, g", c->g, c->M, c->F, c->ldg, 2));
+  return check_matrix("gated block, u", c->u, c->M, c->F, c->ldu, 2);
+}
+GemmCall gated_call(const cla_gated& c, GemmKind kind, int64_t M, int64_t N, int64_t K) {
+  GemmCall g;
+  g.kind = kind;
+  g.type = g.outType = c.type;
+  g.M = M, g.N = N, g.K = K;
+  g.act = c.act;
+  g.device = c.device;
+  return g;
+}
+int64_t gated_fwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaStream_t s) {
+  if (c.M == 0 || c.F == 0) return CLA_OK;
+  GemmCall g = gated_call(c, GK_GATE, c.M, c.F, c.D);
+  g.a[0] = {c.x, c.ldx, false};
+  g.b[0] = {c.wg, c.ldwg, !c.wTrans};
+  g.b[1] = {c.wu, c.ldwu, !c.wTrans};
+  DN_CHECK(aligned(g.a[0], c.M, c.D, c.type, w, run, s));
+  for (int i = 0; i < 2; i++) DN_CHECK(aligned(g.b[i], c.F, c.D, c.type, w, run, s));
+  g.out[0] = c.h, g.out[1] = c.g, g.out[2] = c.u;
+  g.ldo[0] = c.ldh, g.ldo[1] = c.ldg, g.ldo[2] = c.ldu;
+  g.drop = d;
+  return run ? launch_gemm(g, s) : CLA_OK;
+}
+int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaStream_t s) {
+  const int64_t ld = round_up(c.F, 8);
+  void* dg = w.take(c.M * ld * 2);
+  void* du = w.take(c.M * ld * 2);
+  if (run && c.M && c.F) {
+    const int vec = rows_aligned(c.dh, c.lddh, c.M, 2) && rows_aligned(c.g, c.ldg, c.M, 2) && rows_aligned(c.u, c.ldu, c.M, 2);
+    const unsigned b = blocks_for(c.M * (ld / 8));
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      k_gate_grad<T><<<b, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.M, c.F, (T*)dg, (T*)du, ld, d,
+                                        c.act, vec);
+    };
+    if (c.type == CLA_T_BF16) go(__nv_bfloat16());
+    else go(__half());
+    CLA_CUDA(cudaGetLastError());
+  }
+  if (c.dx && c.M && c.D) {
+    GemmCall g = gated_call(c, GK_SUM, c.M, c.D, c.F);
+    g.a[0] = {dg, ld, false};
+    g.a[1] = {du, ld, false};
+    g.b[0] = {c.wg, c.ldwg, (bool)c.wTrans};
+    g.b[1] = {c.wu, c.ldwu, (bool)c.wTrans};
+    for (int i = 0; i < 2; i++) DN_CHECK(aligned(g.b[i], c.D, c.F, c.type, w, run, s));
+    g.out[0] = c.dx, g.ldo[0] = c.lddx;
+    if (run) DN_CHECK(launch_gemm(g, s));
+  }
+  if (c.dwg && c.D && c.F) {
+    GemmCall g = gated_call(c, GK_PAIR, c.D, c.F, c.M);
+    g.a[0] = {c.x, c.ldx, true};
+    g.b[0] = {dg, ld, true};
+    g.b[1] = {du, ld, true};
+    DN_CHECK(aligned(g.a[0], c.D, c.M, c.type, w, run, s));
+    g.out[0] = c.dwg, g.out[1] = c.dwu;
+    g.ldo[0] = c.lddwg, g.ldo[1] = c.lddwu;
+    if (run) DN_CHECK(launch_gemm(g, s));
+  }
+  return CLA_OK;
+}
+int64_t check_work(const Work& need, const void* work, int64_t bytes) {
+  if (need.used == 0) return CLA_OK;
+  if (!work || bytes < need.used) return fail(CLA_ERR_BAD_ARG, "workspace smaller than " + std::to_string(need.used) + " bytes");
+  if ((uintptr_t)work % 256) return fail(CLA_ERR_BAD_ARG, "workspace not 256-byte aligned");
+  return CLA_OK;
+}
+
+// ---- rows of a compressed block ---------------------------------------------------------------------------------------
+constexpr int64_t ROWS_CHUNK = 64ll << 20;  // bytes of FP64 rows at a time that the workspace functions ask for: half the L2
+// Rows [row0, row0 + rows) through an FP64 buffer of `cap` rows: use(first row, rows, their cells). Decompression starts where the skip
+// indexes have entries, so a chunk may begin with rows that were not asked for.
+template <class F>
+int64_t for_rows(Matrix* m, int64_t row0, int64_t rows, double* X, int64_t cap, cudaStream_t s, F&& use) {
+  for (int64_t r = row0; r < row0 + rows;) {
+    const int64_t from = r / SKIP_ROWS * SKIP_ROWS, to = std::min(row0 + rows, from + cap);
+    DN_CHECK(launch_decompress_range(m, (int)from, (int)to, X, s));
+    DN_CHECK(use(r, to - r, X + (r - from) * m->nCols));
+    r = to;
+  }
+  return CLA_OK;
+}
+int64_t chunk_rows(const Matrix* m, int64_t rows) {
+  const int64_t cols = std::max(m->nCols, 1), most = std::max<int64_t>(1, ROWS_CHUNK / 8 / cols / SKIP_ROWS);
+  return std::min(most, rows / SKIP_ROWS + 2) * SKIP_ROWS;
+}
+// what a chunk of so many rows needs beside its cells: q and scales, and b where its rows are not aligned
+int64_t q8_chunk_bytes(const Matrix* m, int64_t rows) {
+  return round_up(rows * round_up(m->nCols, 16), 256) + round_up(rows * 4, 256) + round_up(rows * m->nCols * 8, 256);
+}
+
+}  // namespace
+}  // namespace cla
+
+using namespace cla;
+
+#define DN_MATRIX(h)                                                       \
+  std::shared_ptr<Matrix> mp = lookup(h);                                  \
+  if (!mp) return fail(CLA_ERR_BAD_HANDLE, "unknown or destroyed handle"); \
+  Matrix* m = mp.get();                                                    \
+  std::lock_guard<std::mutex> lk(m->mu);                                   \
+  if (!m->finalized) return fail(CLA_ERR_STATE, "cla_finalize has not been called on this handle")
+
+extern "C" {
+
+int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t cols, void* y, int64_t ldy, const cla_drop* drop,
+                        int32_t device, void* stream) {
+  if (!is_float_type(type)) return fail(CLA_ERR_UNSUPPORTED, "dropout: unknown type");
+  if (!drop) return fail(CLA_ERR_BAD_ARG, "dropout: null arguments");
+  DN_CHECK(check_matrix("dropout, x", x, rows, cols, ldx, type_bytes(type)));
+  DN_CHECK(check_matrix("dropout, y", y, rows, cols, ldy, type_bytes(type)));
+  DropDev d;
+  DN_CHECK(drop_device(*drop, rows, d));
+  OnDevice on(device);
+  if (on.rc < 0) return on.rc;
+  if (rows == 0 || cols == 0) return CLA_OK;
+  with_type(type, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = std::max(4, DN_V<T>);
+    const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(y, ldy, rows, sizeof(T));
+    k_dropout<T><<<blocks_for(rows * ((cols + V - 1) / V)), DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, rows, cols, (T*)y, ldy, d, vec);
+  });
+  CLA_CUDA(cudaGetLastError());
+  return CLA_OK;
+}
+
+int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t byCols, int8_t* q, int64_t ldq,
+                            float* scale, int32_t device, void* stream) {
+  if (!is_float_type(type)) return fail(CLA_ERR_UNSUPPORTED, "quantize: unknown type");
+  if (byCols != 0 && byCols != 1) return fail(CLA_ERR_BAD_ARG, "quantize: byCols is 0 or 1");
+  DN_CHECK(check_matrix("quantize, x", x, rows, cols, ldx, type_bytes(type)));
+  DN_CHECK(check_matrix("quantize, q", q, byCols ? cols : rows, byCols ? rows : cols, ldq, 1));
+  if ((byCols ? cols : rows) && !scale) return fail(CLA_ERR_BAD_ARG, "quantize: null scales");
+  OnDevice on(device);
+  if (on.rc < 0) return on.rc;
+  return quantize(type, x, ldx, rows, cols, byCols, q, ldq, scale, (cudaStream_t)stream);
+}
+
+int64_t cla_q8_workspace(const cla_q8* c) {
+  DN_CHECK(check_q8(c));
+  Work w{nullptr};
+  DN_CHECK(q8_run(*c, false, w, nullptr));
+  return w.used;
+}
+int64_t cla_q8_mm_dev(const cla_q8* c, void* stream) {
+  DN_CHECK(check_q8(c));
+  Work need{nullptr}, w{(char*)c->work};
+  DN_CHECK(q8_run(*c, false, need, nullptr));
+  DN_CHECK(check_work(need, c->work, c->workBytes));
+  OnDevice on(c->device);
+  if (on.rc < 0) return on.rc;
+  return q8_run(*c, true, w, (cudaStream_t)stream);
+}
+
+int64_t cla_gated_workspace(const cla_gated* c, int32_t backward) {
+  DropDev d;
+  DN_CHECK(check_gated(c, backward != 0, d));
+  Work w{nullptr};
+  DN_CHECK(backward ? gated_bwd(*c, d, false, w, nullptr) : gated_fwd(*c, d, false, w, nullptr));
+  return w.used;
+}
+static int64_t gated_dev(const cla_gated* c, bool backward, void* stream) {
+  DropDev d;
+  DN_CHECK(check_gated(c, backward, d));
+  Work need{nullptr}, w{(char*)c->work};
+  DN_CHECK(backward ? gated_bwd(*c, d, false, need, nullptr) : gated_fwd(*c, d, false, need, nullptr));
+  DN_CHECK(check_work(need, c->work, c->workBytes));
+  OnDevice on(c->device);
+  if (on.rc < 0) return on.rc;
+  return backward ? gated_bwd(*c, d, true, w, (cudaStream_t)stream) : gated_fwd(*c, d, true, w, (cudaStream_t)stream);
+}
+int64_t cla_gated_fwd_dev(const cla_gated* c, void* stream) { return gated_dev(c, false, stream); }
+int64_t cla_gated_bwd_dev(const cla_gated* c, void* stream) { return gated_dev(c, true, stream); }
+
+int64_t cla_rows_workspace(cla_handle h, int64_t rows, int32_t type) {
+  DN_MATRIX(h);
+  if (!is_float_type(type)) return fail(CLA_ERR_UNSUPPORTED, "rows of a block: unknown type");
+  if (rows < 0) return fail(CLA_ERR_SHAPE, "rows of a block: negative size");
+  return round_up(chunk_rows(m, rows) * m->nCols * 8, 256);
+}
+int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_t type, void* out, int64_t ldo, void* work, int64_t workBytes,
+                                void* stream) {
+  DN_MATRIX(h);
+  if (!is_float_type(type)) return fail(CLA_ERR_UNSUPPORTED, "rows of a block: unknown type");
+  if (row0 < 0 || rows < 0 || row0 + rows > m->nRows) return fail(CLA_ERR_SHAPE, "rows of a block: outside the matrix");
+  DN_CHECK(check_matrix("rows of a block, result", out, rows, m->nCols, ldo, type_bytes(type)));
+  if (rows == 0 || m->nCols == 0) return CLA_OK;
+  const int64_t cap = workBytes / 8 / m->nCols / SKIP_ROWS * SKIP_ROWS;
+  if (!work || cap < SKIP_ROWS) return fail(CLA_ERR_BAD_ARG, "rows of a block: workspace below 1024 rows of FP64");
+  if ((uintptr_t)work % 256) return fail(CLA_ERR_BAD_ARG, "workspace not 256-byte aligned");
+  OnDevice on(m->device);
+  if (on.rc < 0) return on.rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  m->stats.calls_decompress++;
+  DN_CHECK(order_begin(m, s));
+  const int64_t rc = for_rows(m, row0, rows, (double*)work, cap, s, [&](int64_t r, int64_t n, const double* X) -> int64_t {
+    with_type(type, [&](auto t) {
+      using T = decltype(t);
+      k_narrow<T><<<blocks_for(n * m->nCols), DN_T, 0, s>>>(X, n, m->nCols, (T*)out + (r - row0) * ldo, ldo);
+    });
+    m->stats.kernel_launches++;
+    CLA_CUDA(cudaGetLastError());
+    return CLA_OK;
+  });
+  const int64_t rc2 = order_end(m, s);
+  return rc < 0 ? rc : rc2;
+}
+
+int64_t cla_q8_rmm_workspace(cla_handle h, int64_t N) {
+  DN_MATRIX(h);
+  if (N < 0) return fail(CLA_ERR_SHAPE, "8-bit right product: negative size");
+  return q8_chunk_bytes(m, chunk_rows(m, m->nRows)) + round_up(N * round_up(m->nCols, 16), 256);
+}
+int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* bScale, int64_t N, int32_t outType, void* out, int64_t ldo,
+                       void* work, int64_t workBytes, void* stream) {
+  DN_MATRIX(h);
+  cla_q8 c = {};
+  c.M = m->nRows, c.N = N, c.K = m->nCols;
+  c.a = work, c.lda = m->nCols, c.aType = CLA_T_F64;  // (each chunk's cells)
+  c.b = b, c.ldb = ldb, c.bScale = bScale;
+  c.out = out, c.ldo = ldo, c.outType = outType;
+  c.device = m->device;
+  DN_CHECK(check_q8(&c));
+  if (c.M == 0 || c.N == 0) return CLA_OK;
+  Work w{(char*)work};
+  GemmOperand bo{b, ldb, false};
+  if ((uintptr_t)work % 256) return fail(CLA_ERR_BAD_ARG, "workspace not 256-byte aligned");
+  const int64_t room = workBytes - round_up(N * round_up(m->nCols, 16), 256);
+  int64_t cap = room / std::max<int64_t>(1, q8_chunk_bytes(m, SKIP_ROWS)) * SKIP_ROWS;
+  if (!work || cap < SKIP_ROWS) return fail(CLA_ERR_BAD_ARG, "8-bit right product: workspace below 1024 rows");
+  cap = std::min(cap, round_up(c.M, SKIP_ROWS));
+  OnDevice on(m->device);
+  if (on.rc < 0) return on.rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  m->stats.calls_rmm++;
+  DN_CHECK(order_begin(m, s));
+  int64_t rc = aligned(bo, N, c.K, CLA_T_I8, w, true, s);
+  c.b = (const int8_t*)bo.p, c.ldb = bo.ld;
+  double* X = (double*)w.take(cap * m->nCols * 8);
+  if (rc >= 0)
+    rc = for_rows(m, 0, c.M, X, cap, s, [&](int64_t r, int64_t n, const double* cells) -> int64_t {
+      cla_q8 part = c;
+      part.M = n;
+      part.a = cells;
+      part.out = (char*)out + r * ldo * type_bytes(outType);
+      Work q = w;
+      return q8_run(part, true, q, s);
+    });
+  const int64_t rc2 = order_end(m, s);
+  return rc < 0 ? rc : rc2;
+}
+
+int64_t cla_dense_status(int32_t device) {
+  OnDevice on(device);
+  if (on.rc < 0) return on.rc;
+  return dense_status(device);
+}
+
+}  // extern "C"

@@ -1,0 +1,114 @@
+// What the dense operators share: element types, the activation and its slope, the dropout words, and the product behind them.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "cla_common.cuh"
+
+namespace cla {
+
+inline int type_bytes(int type) {
+  return type == CLA_T_F64 ? 8 : type == CLA_T_F32 ? 4 : type == CLA_T_I8 ? 1 : 2;
+}
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+template <class T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+// (one rounding to the nearest, of a value held in 32 or 64 bits)
+template <class T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <class T> __device__ __forceinline__ T from_f64(double v) { return (T)v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f64(double v) { return __double2bfloat16(v); }
+template <> __device__ __forceinline__ __half from_f64(double v) { return __double2half(v); }
+
+// ---- dropout --------------------------------------------------------------------------------------------------------
+struct DropDev {
+  uint32_t cut = 0;  // kept where word >= cut
+  uint32_t row0 = 0;
+  uint32_t seed[2] = {}, step[2] = {};
+  float scale = 1.f;
+  double scale64 = 1.0;
+  int on = 0;
+};
+// The four words of columns 4 c .. 4 c + 3 of a row: Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011)
+__device__ __forceinline__ uint4 drop_words(const DropDev& d, uint32_t row, uint32_t c) {
+  uint32_t x0 = c, x1 = d.row0 + row, x2 = d.step[0], x3 = d.step[1], k0 = d.seed[0], k1 = d.seed[1];
+#pragma unroll
+  for (int i = 0; i < 10; i++) {
+    const uint64_t a = (uint64_t)0xD2511F53u * x0, b = (uint64_t)0xCD9E8D57u * x2;
+    x0 = (uint32_t)(b >> 32) ^ x1 ^ k0;
+    x1 = (uint32_t)b;
+    x2 = (uint32_t)(a >> 32) ^ x3 ^ k1;
+    x3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(x0, x1, x2, x3);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+// ---- the activation, in FP32 ------------------------------------------------------------------------------------------
+__device__ __forceinline__ float act_value(int act, float g) {
+  switch (act) {
+    case CLA_ACT_SILU: return g / (1.f + expf(-g));
+    case CLA_ACT_SIGMOID: return 1.f / (1.f + expf(-g));
+    case CLA_ACT_RELU: return g < 0.f ? 0.f : g;
+    case CLA_ACT_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+    default: return 0.5f * g * (1.f + tanhf(0.79788456080286536f * (g + 0.044715f * g * g * g)));
+  }
+}
+__device__ __forceinline__ float act_slope(int act, float g, float& value) {
+  switch (act) {
+    case CLA_ACT_SILU: {
+      const float s = 1.f / (1.f + expf(-g));
+      value = g * s;
+      return s * (1.f + g * (1.f - s));
+    }
+    case CLA_ACT_SIGMOID: {
+      const float s = 1.f / (1.f + expf(-g));
+      value = s;
+      return s * (1.f - s);
+    }
+    case CLA_ACT_RELU: value = g < 0.f ? 0.f : g; return g > 0.f ? 1.f : 0.f;
+    case CLA_ACT_GELU: {
+      const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+      value = g * c;
+      return c + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+    }
+    default: {
+      const float t = tanhf(0.79788456080286536f * (g + 0.044715f * g * g * g));
+      value = 0.5f * g * (1.f + t);
+      return 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * g * g);
+    }
+  }
+}
+
+// ---- products (cla_gemm.cu) -------------------------------------------------------------------------------------------
+struct GemmOperand {
+  const void* p = nullptr;
+  int64_t ld = 0;   // elements
+  bool mn = false;  // element (i, k) at p[k * ld + i]; else at p[i * ld + k]
+};
+enum GemmKind {
+  GK_Q8,    // out0 = aScale bScale a0 b0, 8-bit integers
+  GK_GATE,  // out0 = dropout(act(a0 b0) * (a0 b1)); out1, out2 = the two products, where not null
+  GK_SUM,   // out0 = a0 b0 + a1 b1
+  GK_PAIR   // out0 = a0 b0, out1 = a0 b1
+};
+struct GemmCall {
+  GemmKind kind;
+  int type, outType;    // of the operands (I8, BF16 or F16), of the results
+  int64_t M, N, K;      // results [M x N], sums over K
+  GemmOperand a[2], b[2];  // a: the rows' side; addresses 16-byte aligned, ld * element size a multiple of 16
+  void* out[3] = {};
+  int64_t ldo[3] = {};
+  const float *aScale = nullptr, *bScale = nullptr;
+  int act = 0;
+  DropDev drop;
+  int device = 0;
+};
+int64_t launch_gemm(const GemmCall& c, cudaStream_t s);
+int64_t dense_status(int device);  // the self-check word of the product kernels, cleared
+
+}  // namespace cla

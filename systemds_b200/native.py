@@ -31,6 +31,24 @@ class cla_stats(C.Structure):
 
 
 _P, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
+
+
+class cla_drop(C.Structure):
+    _fields_ = [("p", C.c_double), ("seed", C.c_uint64), ("step", C.c_uint64), ("row0", _I64)]
+
+
+class cla_q8(C.Structure):
+    _fields_ = [("M", _I64), ("N", _I64), ("K", _I64), ("a", _P), ("lda", _I64), ("aScale", _P), ("b", _P), ("ldb", _I64), ("bScale", _P),
+                ("out", _P), ("ldo", _I64), ("work", _P), ("workBytes", _I64), ("aType", _I32), ("outType", _I32), ("device", _I32)]
+
+
+class cla_gated(C.Structure):
+    _fields_ = [("M", _I64), ("D", _I64), ("F", _I64), ("x", _P), ("wg", _P), ("wu", _P), ("ldx", _I64), ("ldwg", _I64), ("ldwu", _I64),
+                ("h", _P), ("g", _P), ("u", _P), ("ldh", _I64), ("ldg", _I64), ("ldu", _I64), ("dh", _P), ("lddh", _I64), ("dx", _P),
+                ("dwg", _P), ("dwu", _P), ("lddx", _I64), ("lddwg", _I64), ("lddwu", _I64), ("work", _P), ("workBytes", _I64),
+                ("drop", cla_drop), ("type", _I32), ("act", _I32), ("wTrans", _I32), ("device", _I32)]
+
+
 # name -> argument types; every function returns int64
 SIGNATURES = {
     "cla_create": [_I32, _I32, _I32],
@@ -73,6 +91,18 @@ SIGNATURES = {
     "cla_allreduce_dev": [_I64, _P, _I64, _P],
     "cla_comm_status": [_I64],
     "cla_comm_destroy": [_I64],
+    "cla_dropout_dev": [_I32, _P, _I64, _I64, _I64, _P, _I64, C.POINTER(cla_drop), _I32, _P],
+    "cla_q8_quantize_dev": [_I32, _P, _I64, _I64, _I64, _I32, _P, _I64, _P, _I32, _P],
+    "cla_q8_workspace": [C.POINTER(cla_q8)],
+    "cla_q8_mm_dev": [C.POINTER(cla_q8), _P],
+    "cla_gated_workspace": [C.POINTER(cla_gated), _I32],
+    "cla_gated_fwd_dev": [C.POINTER(cla_gated), _P],
+    "cla_gated_bwd_dev": [C.POINTER(cla_gated), _P],
+    "cla_rows_workspace": [_I64, _I64, _I32],
+    "cla_decompress_rows_dev": [_I64, _I64, _I64, _I32, _P, _I64, _P, _I64, _P],
+    "cla_q8_rmm_workspace": [_I64, _I64],
+    "cla_q8_rmm_dev": [_I64, _P, _I64, _P, _I64, _I32, _P, _I64, _P, _I64, _P],
+    "cla_dense_status": [_I32],
     "cla_group_decode": [_I64, _I32, _P],
     "cla_group_counts": [_I64, _I32, _P],
 }
