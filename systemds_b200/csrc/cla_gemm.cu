@@ -1,87 +1,559 @@
-// Products of dense operands in 8 and 16 bits with their epilogues: see cla_dense.cuh.
+// Products of dense operands in 8 and 16 bits with their epilogues (GemmCall of cla_dense.cuh), on the 5th-generation tensor cores: operands by
+// TMA into 128-byte-swizzled shared memory, sums in tensor memory (FP32, or 32-bit integers for 8-bit operands), epilogues from there.
+//  * k_gemm_pair: two CTAs share a 256 x 256 tile. For large results.
+//  * k_gemm_few: one CTA per 128 columns of the result and 16 to 128 of its rows, the depth split over a cluster. For few rows.
+#include <cuda.h>
+#include <algorithm>
 #include "cla_dense.cuh"
 
 namespace cla {
 
-// The plain kernel: a CTA per 64 x 64 results, operands through shared memory 16 deep, a thread per 4 x 4 results, sums in FP32 (8-bit
-// operands: 32-bit integers). Bound: the FMA pipe.
-constexpr int GS_T = 64, GS_K = 16;
-template <class T> struct SumOf { using type = float; };
-template <> struct SumOf<int8_t> { using type = int32_t; };
+static __device__ int32_t denseErr;
 
-template <class T>
-__global__ void __launch_bounds__(256) k_gemm_simple(const __grid_constant__ GemmCall c) {
-  using S = typename SumOf<T>::type;
-  __shared__ S sa[GS_K][GS_T + 4], sb[2][GS_K][GS_T + 4];
-  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-  const int64_t m0 = (int64_t)blockIdx.y * GS_T, n0 = (int64_t)blockIdx.x * GS_T;
-  const int which = blockIdx.z;  // PAIR: the product
-  const bool two = c.kind == GK_GATE;
-  S acc[2][4][4] = {};
-  for (int seg = 0; seg < (c.kind == GK_SUM ? 2 : 1); seg++)
-    for (int64_t k0 = 0; k0 < c.K; k0 += GS_K) {
-      for (int e = tid; e < GS_T * GS_K; e += 256) {
-        auto load = [&](const GemmOperand& o, int64_t i0, int64_t rows, S (*dst)[GS_T + 4]) {
-          const int i = o.mn ? e % GS_T : e / GS_K, k = o.mn ? e / GS_T : e % GS_K;
-          S v = 0;
-          if (i0 + i < rows && k0 + k < c.K) {
-            const T* p = (const T*)o.p;
-            v = (S)to_f32(p[o.mn ? (k0 + k) * o.ld + i0 + i : (i0 + i) * o.ld + k0 + k]);
-          }
-          dst[k][i] = v;
-        };
-        load(c.a[seg], m0, c.M, sa);
-        load(c.b[c.kind == GK_PAIR ? which : seg], n0, c.N, sb[0]);
-        if (two) load(c.b[1], n0, c.N, sb[1]);
-      }
-      __syncthreads();
+// ---- PTX ------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t gm_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t gm_now() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool gm_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+// Gives up after GM_LIMIT ns: far longer than any launch, so that a mistake ends as an error and not as a hung GPU
+constexpr uint64_t GM_LIMIT = 8000000000ull;
+__device__ __noinline__ bool gm_wait_long(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = gm_now();
+  do {
+    for (int i = 0; i < 64; i++)
+      if (gm_try(bar, parity)) return true;
+  } while (gm_now() - t0 < GM_LIMIT);
+  return false;
+}
+__device__ __forceinline__ bool gm_wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < 32; i++)
+    if (gm_try(bar, parity)) return true;
+  return gm_wait_long(bar, parity);
+}
+__device__ __forceinline__ uint32_t gm_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t gm_peer(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void gm_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ bool gm_elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void gm_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void gm_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A box at element (x, y); PAIR: the barrier may be the other CTA's
+template <bool PAIR>
+__device__ __forceinline__ void gm_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+template <bool PAIR, bool I8>
+__device__ __forceinline__ void gm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+#define GM_MMA(GROUP, KIND)                                                                                                             \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
+               "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)                                                                            \
+               : "memory")
+  if (PAIR) {
+    if (I8) GM_MMA("2", "i8");
+    else GM_MMA("2", "f16");
+  } else {
+    if (I8) GM_MMA("1", "i8");
+    else GM_MMA("1", "f16");
+  }
+#undef GM_MMA
+}
+// The barrier gets an arrival when the products issued so far are done; PAIR: both CTAs' barriers
+template <bool PAIR>
+__device__ __forceinline__ void gm_commit(uint32_t bar) {
+  if (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// 16 columns of a warp's 32 lanes; gm_loaded() before the registers are read
+__device__ __forceinline__ void gm_tmem16(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void gm_loaded(uint32_t (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-      for (int k = 0; k < GS_K; k++)
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
+
+// ---- operands in shared memory ----------------------------------------------------------------------------------------
+// A stage is 128 bytes deep: 64 values of 16 bits, 128 of 8. Rows of 128 bytes, swizzled over 1024-byte groups of eight.
+// Depth contiguous (K-major): a row per index, groups of eight indexes 1024 bytes apart; the next 32 bytes of depth lie 32 bytes on.
+// Index contiguous (16-bit types): a row per depth step, 64 indexes wide, 64 rows to a box of 8 KB; the next 16 steps lie 2 KB on.
+constexpr uint32_t GM_OPERAND = 128 * 128;  // bytes of 128 indexes
+__device__ __forceinline__ uint64_t gm_desc(uint32_t addr, bool mn) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(mn ? 8192 >> 4 : 1) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+__host__ __device__ constexpr uint32_t gm_step(bool mn) { return mn ? 2048 >> 4 : 32 >> 4; }
+
+struct alignas(64) GemmArgs {
+  CUtensorMap a[2], b[2];
+  GemmCall c;
+  int depth;             // values of a stage
+  int kBlocks;           // stages of a segment
+  int tilesM, tilesN;    // PAIR: tilesN of both products
+  int nc, stages;        // k_gemm_few: rows of a tile, stages of the ring
+  uint32_t idesc;
+};
+
+// ---- epilogues ----------------------------------------------------------------------------------------------------------
+template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f32<O>(v); }
+
+// N values of a row, the first `valid` of them; vec: the row's pieces start on 16-byte boundaries
+template <class O, int N>
+__device__ __forceinline__ void gm_store(O* p, int valid, bool vec, const O (&v)[N]) {
+  constexpr int V = 16 / (int)sizeof(O);
+  if (vec && valid >= N) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+    for (int i = 0; i < N; i += V) *(uint4*)(p + i) = *(const uint4*)(v + i);
+  } else {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            acc[0][i][j] += sa[k][ty * 4 + i] * sb[0][k][tx * 4 + j];
-            if (two) acc[1][i][j] += sa[k][ty * 4 + i] * sb[1][k][tx * 4 + j];
-          }
-      __syncthreads();
+    for (int i = 0; i < N; i++)
+      if (i < valid) p[i] = v[i];
+  }
+}
+template <class F> __device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {
+    case CLA_ACT_SILU: f(std::integral_constant<int, CLA_ACT_SILU>()); break;
+    case CLA_ACT_GELU: f(std::integral_constant<int, CLA_ACT_GELU>()); break;
+    case CLA_ACT_GELU_TANH: f(std::integral_constant<int, CLA_ACT_GELU_TANH>()); break;
+    case CLA_ACT_RELU: f(std::integral_constant<int, CLA_ACT_RELU>()); break;
+    default: f(std::integral_constant<int, CLA_ACT_SIGMOID>()); break;
+  }
+}
+template <int KIND, class O>
+__device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa, float sb) {
+  if constexpr (sizeof(O) == 8) return (double)sum * sa * sb;
+  else return gm_cast<O>((float)sum * sa * sb);
+}
+
+// ---- large results --------------------------------------------------------------------------------------------------------
+// Tile 256 x 256 per pair of CTAs (GATE: 256 x 128 of both products): each CTA holds the sums of its 128 rows and brings 128 rows and 128
+// columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight take the sums out of one half of
+// tensor memory while the other fills. A launch's pairs take tiles in turn, along the rows within groups of GP_GROUP row tiles, so that what
+// runs at once shares operands in L2.
+constexpr int GP_T = 384, GP_STAGES = 6, GP_STAGE = 2 * GM_OPERAND, GP_GROUP = 8;
+
+__device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& tn) {
+  const int per = GP_GROUP * A.tilesN, g = t / per, first = g * GP_GROUP, n = min(GP_GROUP, A.tilesM - first), r = t - g * per;
+  tm = first + r % n;
+  tn = r / n;
+}
+
+template <int KIND, class O>
+__global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
+  constexpr bool I8 = KIND == GK_Q8;
+  extern __shared__ __align__(1024) unsigned char gmsm[];
+  __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumEmpty[2];
+  __shared__ uint32_t tmemAt;
+  const GemmCall& c = A.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = gm_rank(), smem = (gm_smem(gmsm) + 1023u) & ~1023u;
+  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2, tiles = A.tilesM * A.tilesN;
+  const int segments = KIND == GK_SUM ? 2 : 1, nk = A.kBlocks * segments;
+  const bool aMn = !I8 && c.a[0].mn, bMn = !I8 && c.b[0].mn;
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < GP_STAGES; i++) {
+      gm_init(gm_smem(full + i), 1);
+      gm_init(gm_smem(empty + i), 1);
     }
-  for (int i = 0; i < 4; i++) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= c.M) break;
-    uint4 w;
-    if (c.drop.on) w = drop_words(c.drop, (uint32_t)m, (uint32_t)((n0 + tx * 4) / 4));
-    for (int j = 0; j < 4; j++) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (n >= c.N) break;
-      auto put = [&](int o, int outType, double d, float f) {
-        const int64_t at = m * c.ldo[o] + n;
-        if (outType == CLA_T_F64) ((double*)c.out[o])[at] = d;
-        else if (outType == CLA_T_F32) ((float*)c.out[o])[at] = f;
-        else if (outType == CLA_T_BF16) ((__nv_bfloat16*)c.out[o])[at] = from_f32<__nv_bfloat16>(f);
-        else ((__half*)c.out[o])[at] = from_f32<__half>(f);
-      };
-      if (c.kind == GK_Q8) {
-        if (c.outType == CLA_T_F64) put(0, c.outType, (double)acc[0][i][j] * c.aScale[m] * c.bScale[n], 0.f);
-        else put(0, c.outType, 0.0, (float)acc[0][i][j] * c.aScale[m] * c.bScale[n]);
-      } else if (c.kind == GK_GATE) {
-        const float g = (float)acc[0][i][j], u = (float)acc[1][i][j];
-        float h = act_value(c.act, g) * u;
-        if (c.drop.on) h = word_of(w, j) >= c.drop.cut ? h * c.drop.scale : 0.f;
-        put(0, c.outType, 0.0, h);
-        if (c.out[1]) {
-          put(1, c.outType, 0.0, g);
-          put(2, c.outType, 0.0, u);
+    for (int i = 0; i < 2; i++) {
+      gm_init(gm_smem(sumFull + i), 1);
+      gm_init(gm_smem(sumEmpty + i), 16);  // the eight warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  gm_cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmemAt;
+  bool ok = true;
+  if (warp == 0) {
+    if (gm_elect()) {
+      int s = 0;
+      uint32_t ph = 1;
+      int64_t issued = 0;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int tm, tn;
+        gp_tile(A, t, tm, tn);
+        const int m0 = tm * 256 + rank * 128;
+        const int halfN = A.tilesN / 2, which = KIND == GK_GATE ? (int)rank : KIND == GK_PAIR && tn >= halfN;
+        const int n0 = KIND == GK_GATE ? tn * 128 : (KIND == GK_PAIR && tn >= halfN ? tn - halfN : tn) * 256 + rank * 128;
+        for (int kb = 0; kb < nk; kb++) {
+          ok = gm_wait(gm_smem(empty + s), ph);
+          if (!ok) break;
+          const int seg = KIND == GK_SUM && kb >= A.kBlocks, k0 = (kb - seg * A.kBlocks) * A.depth;
+          const uint32_t bar = gm_peer(gm_smem(full + s), 0), da = smem + s * GP_STAGE, db = da + GM_OPERAND;
+          if (rank == 0) gm_expect(gm_smem(full + s), 2 * GP_STAGE);
+          const CUtensorMap *ma = A.a + seg, *mb = A.b + (KIND == GK_SUM ? seg : which);
+          if (aMn) {
+            gm_load<true>(da, ma, m0, k0, bar);
+            gm_load<true>(da + 8192, ma, m0 + 64, k0, bar);
+          } else {
+            gm_load<true>(da, ma, k0, m0, bar);
+          }
+          if (bMn) {
+            gm_load<true>(db, mb, n0, k0, bar);
+            gm_load<true>(db + 8192, mb, n0 + 64, k0, bar);
+          } else {
+            gm_load<true>(db, mb, k0, n0, bar);
+          }
+          issued++;
+          if (++s == GP_STAGES) s = 0, ph ^= 1;
+        }
+      }
+      // what is still on its way, here and to the other CTA's barriers
+      for (int i = 0; i < GP_STAGES; i++) {
+        const int64_t n = (issued - i + GP_STAGES - 1) / GP_STAGES;  // times stage i was filled
+        if (n <= 0) break;
+        if (!ok && rank == 0) gm_wait(gm_smem(full + i), (uint32_t)(n - 1) & 1u);
+        if (ok && !gm_wait(gm_smem(empty + i), (uint32_t)(n - 1) & 1u)) ok = false;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && gm_elect()) {
+      int s = 0;
+      uint32_t ph = 0;
+      int n = 0;
+      for (int t = pair; t < tiles && ok; t += pairs, n++) {
+        const int buf = n & 1;
+        ok = gm_wait(gm_smem(sumEmpty + buf), ((n >> 1) & 1) ^ 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int kb = 0; kb < nk; kb++) {
+          ok = gm_wait(gm_smem(full + s), ph);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          uint64_t a = gm_desc(smem + s * GP_STAGE, aMn), b = gm_desc(smem + s * GP_STAGE + GM_OPERAND, bMn);
+#pragma unroll
+          for (int i = 0; i < 4; i++, a += gm_step(aMn), b += gm_step(bMn)) gm_mma<true, I8>(tmem + buf * 256, a, b, A.idesc, kb > 0 || i > 0);
+          gm_commit<true>(gm_smem(empty + s));
+          if (++s == GP_STAGES) s = 0, ph ^= 1;
+        }
+        if (ok) gm_commit<true>(gm_smem(sumFull + buf));
+      }
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    int n = 0;
+    for (int t = pair; t < tiles; t += pairs, n++) {
+      const int buf = n & 1;
+      ok = gm_wait(gm_smem(sumFull + buf), (n >> 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      int tm, tn;
+      gp_tile(A, t, tm, tn);
+      const int64_t m = (int64_t)tm * 256 + rank * 128 + quarter * 32 + lane;
+      const uint32_t at = tmem + buf * 256 + ((uint32_t)quarter << 21);
+      if constexpr (KIND == GK_GATE) {
+        const int64_t n0 = (int64_t)tn * 128 + half * 64;
+        const bool vec = ((uintptr_t)c.out[0] | (uintptr_t)(c.ldo[0] * 2) | (uintptr_t)c.out[1] | (uintptr_t)(c.ldo[1] * 2) | (uintptr_t)c.out[2] |
+                          (uintptr_t)(c.ldo[2] * 2)) % 16 == 0;
+#pragma unroll 1
+        for (int j = 0; j < 64; j += 16) {
+          uint32_t v[32];
+          gm_tmem16(at + half * 64 + j, v);
+          gm_tmem16(at + 128 + half * 64 + j, v + 16);
+          gm_loaded(v);
+          const int valid = m < c.M ? (int)min((int64_t)16, c.N - n0 - j) : 0;
+          alignas(16) O o[16];
+          if (c.out[1]) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(__uint_as_float(v[i]));
+            gm_store((O*)c.out[1] + m * c.ldo[1] + n0 + j, valid, vec, o);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(__uint_as_float(v[16 + i]));
+            gm_store((O*)c.out[2] + m * c.ldo[2] + n0 + j, valid, vec, o);
+          }
+          float h[16];
+          with_act(c.act, [&](auto act) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) h[i] = act_value(decltype(act)::value, __uint_as_float(v[i])) * __uint_as_float(v[16 + i]);
+          });
+          if (c.drop.on) {
+#pragma unroll
+            for (int q = 0; q < 16; q += 4) {
+              const uint4 w = drop_words(c.drop, (uint32_t)m, (uint32_t)((n0 + j + q) / 4));
+#pragma unroll
+              for (int i = 0; i < 4; i++) h[q + i] = word_of(w, i) >= c.drop.cut ? h[q + i] * c.drop.scale : 0.f;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(h[i]);
+          gm_store((O*)c.out[0] + m * c.ldo[0] + n0 + j, valid, vec, o);
+          __syncwarp();
         }
       } else {
-        put(c.kind == GK_PAIR ? which : 0, c.outType, 0.0, (float)acc[0][i][j]);
+        const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
+        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * 256 + half * 128;
+        O* out = (O*)c.out[which] + m * c.ldo[which] + n0;
+        const bool vec = ((uintptr_t)c.out[which] | (uintptr_t)(c.ldo[which] * sizeof(O))) % 16 == 0;
+        const float sa = I8 && m < c.M ? c.aScale[m] : 0.f;
+#pragma unroll 1
+        for (int j = 0; j < 128; j += 16) {
+          uint32_t v[16];
+          gm_tmem16(at + half * 128 + j, v);
+          gm_loaded(v);
+          const int valid = m < c.M ? (int)min((int64_t)16, c.N - n0 - j) : 0;
+          alignas(16) O o[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, i < valid ? __ldg(c.bScale + n0 + j + i) : 0.f);
+            else o[i] = gm_cast<O>(__uint_as_float(v[i]));
+          }
+          gm_store(out + j, valid, vec, o);
+          __syncwarp();
+        }
       }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gm_peer(gm_smem(sumEmpty + buf), 0)) : "memory");
     }
+  }
+  if (!ok) atomicExch(&denseErr, 201);
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  gm_cluster_sync();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
-static __device__ int32_t denseErr;
+// ---- few rows -------------------------------------------------------------------------------------------------------------
+// A CTA per 128 columns of the result (the lanes of tensor memory) and nc rows, so that little of the tensor cores' width is spent on
+// rows that are not there; the depth is split over the CTAs of a cluster, whose partial sums meet in shared memory, each CTA adding up its
+// share of the rows in the order of the ranks. GATE: both weights' tiles in a stage, two sums.
+constexpr int GF_T = 192;
 
+template <int KIND, class O>
+__global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ GemmArgs A) {
+  constexpr bool I8 = KIND == GK_Q8;
+  constexpr int NP = KIND == GK_GATE ? 2 : 1;
+  constexpr int MOST = 16;
+  extern __shared__ __align__(1024) unsigned char gmsm[];
+  __shared__ __align__(8) uint64_t full[MOST], empty[MOST], sumFull;
+  __shared__ uint32_t tmemAt;
+  const GemmCall& c = A.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = gm_rank(), smem = (gm_smem(gmsm) + 1023u) & ~1023u;
+  uint32_t split;
+  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(split));
+  const int tile = blockIdx.x / split, tn = tile % A.tilesN, tm = tile / A.tilesN;
+  const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
+  const int n0 = (which ? tn - halfN : tn) * 128, m0 = tm * A.nc;
+  const int nk = A.kBlocks * (KIND == GK_SUM ? 2 : 1);
+  const int kb0 = (int)((int64_t)nk * rank / split), kb1 = (int)((int64_t)nk * (rank + 1) / split);
+  const bool cMn = !I8 && c.a[0].mn, lMn = !I8 && c.b[0].mn;  // the result's rows and columns
+  const uint32_t stage = NP * GM_OPERAND + A.nc * 128, cols = max(32, NP * A.nc);
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gm_smem(&tmemAt)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < A.stages; i++) {
+      gm_init(gm_smem(full + i), 1);
+      gm_init(gm_smem(empty + i), 1);
+    }
+    gm_init(gm_smem(&sumFull), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmemAt;
+  bool ok = true;
+  if (warp == 4) {
+    if (gm_elect()) {
+      int s = 0, issued = 0;
+      uint32_t ph = 1;
+      for (int kb = kb0; kb < kb1; kb++) {
+        ok = gm_wait(gm_smem(empty + s), ph);
+        if (!ok) break;
+        const int seg = KIND == GK_SUM && kb >= A.kBlocks, k0 = (kb - seg * A.kBlocks) * A.depth;
+        const uint32_t bar = gm_smem(full + s), dl = smem + s * stage, dc = dl + NP * GM_OPERAND;
+        gm_expect(bar, stage);
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const CUtensorMap* ml = A.b + (KIND == GK_GATE ? p : KIND == GK_SUM ? seg : which);
+          if (lMn) {
+            gm_load<false>(dl + p * GM_OPERAND, ml, n0, k0, bar);
+            gm_load<false>(dl + p * GM_OPERAND + 8192, ml, n0 + 64, k0, bar);
+          } else {
+            gm_load<false>(dl + p * GM_OPERAND, ml, k0, n0, bar);
+          }
+        }
+        if (cMn) {
+          for (int i = 0; i < A.nc; i += 64) gm_load<false>(dc + i * 128, A.a + seg, m0 + i, k0, bar);
+        } else {
+          gm_load<false>(dc, A.a + seg, k0, m0, bar);
+        }
+        issued++;
+        if (++s == A.stages) s = 0, ph ^= 1;
+      }
+      for (int i = 0; i < min(issued, A.stages); i++) {
+        const int n = (issued - i + A.stages - 1) / A.stages;
+        if (!ok) gm_wait(gm_smem(full + i), (uint32_t)(n - 1) & 1u);
+        else if (!gm_wait(gm_smem(empty + i), (uint32_t)(n - 1) & 1u)) ok = false;
+      }
+    }
+  } else if (warp == 5) {
+    if (gm_elect()) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = kb0; kb < kb1; kb++) {
+        ok = gm_wait(gm_smem(full + s), ph);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t dl = smem + s * stage;
+        uint64_t b = gm_desc(dl + NP * GM_OPERAND, cMn);
+        uint64_t l[NP];
+#pragma unroll
+        for (int p = 0; p < NP; p++) l[p] = gm_desc(dl + p * GM_OPERAND, lMn);
+#pragma unroll
+        for (int i = 0; i < 4; i++, b += gm_step(cMn))
+#pragma unroll
+          for (int p = 0; p < NP; p++) {
+            gm_mma<false, I8>(tmem + p * A.nc, l[p], b, A.idesc, kb > kb0 || i > 0);
+            l[p] += gm_step(lMn);
+          }
+        gm_commit<false>(gm_smem(empty + s));
+        if (++s == A.stages) s = 0, ph ^= 1;
+      }
+      if (ok) gm_commit<false>(gm_smem(&sumFull));
+    }
+  } else {
+    ok = gm_wait(gm_smem(&sumFull), 0);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  }
+  __syncwarp();
+  // The sums of lane n0 + 32 warp + lane (a column of the result), rows m0 .. m0 + nc
+  const int rows = (int)min((int64_t)A.nc, c.M - m0);
+  const int64_t n = n0 + warp * 32 + lane;
+  const float sb = I8 && warp < 4 && n < c.N ? c.bScale[n] : 0.f;
+  auto put = [&](int r, const uint32_t (&v)[NP]) {
+    const int64_t m = m0 + r;
+    if (n >= c.N) return;
+    if constexpr (I8) {
+      ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<KIND, O>(c, (int32_t)v[0], c.aScale[m], sb);
+    } else if constexpr (KIND == GK_GATE) {
+      const float g = __uint_as_float(v[0]), u = __uint_as_float(v[1]);
+      float h = act_value(c.act, g) * u;
+      if (c.drop.on) h = word_of(drop_words(c.drop, (uint32_t)m, (uint32_t)(n / 4)), (int)(n & 3)) >= c.drop.cut ? h * c.drop.scale : 0.f;
+      ((O*)c.out[0])[m * c.ldo[0] + n] = gm_cast<O>(h);
+      if (c.out[1]) {
+        ((O*)c.out[1])[m * c.ldo[1] + n] = gm_cast<O>(g);
+        ((O*)c.out[2])[m * c.ldo[2] + n] = gm_cast<O>(u);
+      }
+    } else {
+      ((O*)c.out[which])[m * c.ldo[which] + n] = gm_cast<O>(__uint_as_float(v[0]));
+    }
+  };
+  const uint32_t at = tmem + ((uint32_t)(warp & 3) << 21);
+  if (warp < 4) {
+    for (int r = 0; r < rows; r += 16) {
+      uint32_t v[NP * 16];
+#pragma unroll
+      for (int p = 0; p < NP; p++) gm_tmem16(at + p * A.nc + r, v + 16 * p);
+      gm_loaded(v);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        if (r + i >= rows) break;
+        uint32_t w[NP];
+#pragma unroll
+        for (int p = 0; p < NP; p++) w[p] = kb1 > kb0 ? v[16 * p + i] : 0u;
+        if (split == 1) put(r + i, w);
+        else
+#pragma unroll
+          for (int p = 0; p < NP; p++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem + ((p * A.nc + r + i) * 128 + threadIdx.x) * 4), "r"(w[p]) : "memory");
+      }
+      __syncwarp();
+    }
+  }
+  if (split > 1) {
+    gm_cluster_sync();
+    if (warp < 4) {
+      for (int r = rank; r < rows; r += split) {
+        uint32_t w[NP];
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const uint32_t mine = smem + ((p * A.nc + r) * 128 + threadIdx.x) * 4;
+          float f = 0.f;
+          uint32_t sum = 0;
+          for (uint32_t q = 0; q < split; q++) {
+            uint32_t x;
+            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(x) : "r"(gm_peer(mine, q)) : "memory");
+            if (I8) sum += x;
+            else f += __uint_as_float(x);
+          }
+          w[p] = I8 ? sum : __float_as_uint(f);
+        }
+        put(r, w);
+      }
+    }
+  }
+  if (!ok) atomicExch(&denseErr, 202);
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (split > 1) gm_cluster_sync();  // (the others may still read this one's sums)
+  if (warp == 5) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
 int64_t dense_status(int device) {
   (void)device;
   int32_t e = 0, zero = 0;
@@ -91,14 +563,134 @@ int64_t dense_status(int device) {
   return fail(CLA_ERR_DEVICE_CHECK, "a dense product's self-check tripped (code " + std::to_string(e) + ")");
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+  static EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? (EncodeTiled)p
+               : nullptr;
+  }();
+  return f;
+}
+// An operand of `count` indexes and depth k, in boxes of `box` indexes (index contiguous: always 64) and a stage's depth
+static int64_t operand_map(CUtensorMap& map, const GemmOperand& o, int type, int64_t count, int64_t k, int box) {
+  EncodeTiled enc = encode_tiled();
+  if (!enc) return fail(CLA_ERR_CUDA, "dense product: the driver has no tensor maps");
+  const int bytes = type_bytes(type);
+  const cuuint64_t dims[2] = {(cuuint64_t)(o.mn ? count : k), (cuuint64_t)(o.mn ? k : count)}, stride[1] = {(cuuint64_t)(o.ld * bytes)};
+  const cuuint32_t boxes[2] = {o.mn ? 64u : 128u / bytes, o.mn ? 64u : (cuuint32_t)box}, ones[2] = {1, 1};
+  const CUtensorMapDataType t =
+      type == CLA_T_I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == CLA_T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = enc(&map, t, 2, (void*)o.p, dims, stride, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CLA_OK : fail(CLA_ERR_CUDA, "dense product: tensor map refused (" + std::to_string((int)r) + ")");
+}
+
+// Shared memory of a CTA in proportion to its columns of tensor memory, so that an SM never holds CTAs of more columns than it has: CTAs that
+// wait for columns while their cluster waits for them could otherwise hold up one another, of any launches.
+constexpr int GM_SM_SMEM = 228 * 1024, GM_CTA_SMEM = 1024;  // an SM's, and what it keeps for each CTA
+template <class K>
+static int64_t smem_for(OncePerDevice& once, int* room, int device, int cols, K kernel, int& least) {
+  const int64_t rc = once(device, [&]() -> int64_t {
+    cudaFuncAttributes a;
+    CLA_CUDA(cudaFuncGetAttributes(&a, kernel));
+    const int most = GM_SM_SMEM - GM_CTA_SMEM - (int)a.sharedSizeBytes;
+    CLA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    *room = most;
+    return CLA_OK;
+  });
+  least = GM_SM_SMEM / 512 * cols - (GM_SM_SMEM - *room);
+  return rc;
+}
+
+template <int KIND, class O>
+static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
+  const GemmCall& c = A.c;
+  const int bytes = type_bytes(c.type), segs = KIND == GK_SUM ? 2 : 1;
+  int sms = 148;
+  CLA_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device));
+  A.depth = 128 / bytes;
+  A.kBlocks = (int)((c.K + A.depth - 1) / A.depth);
+  const int nk = A.kBlocks * segs;
+  // both operands' types, where their index is contiguous, sums in 32 bits
+  const uint32_t type = c.type == CLA_T_BF16 || c.type == CLA_T_I8 ? 1u : 0u;
+  const uint32_t base = (KIND == GK_Q8 ? 2u : 1u) << 4 | type << 7 | type << 10;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = s;
+  const bool large = c.M > 128 && nk > 0;
+  for (int i = 0; i < 2; i++) {
+    const bool hasA = i == 0 || KIND == GK_SUM, hasB = i == 0 || KIND != GK_Q8;
+    int nc = 128;
+    if (!large)
+      while (nc > 16 && nc / 2 >= c.M && !(c.a[0].mn && nc == 64)) nc /= 2;
+    A.nc = nc;
+    if (nk == 0) continue;
+    if (hasA)
+      if (const int64_t rc = operand_map(A.a[i], c.a[i], c.type, c.M, c.K, nc); rc < 0) return rc;
+    if (hasB)
+      if (const int64_t rc = operand_map(A.b[i], c.b[i], c.type, c.N, c.K, 128); rc < 0) return rc;
+  }
+  if (large) {
+    const int wide = KIND == GK_GATE ? 128 : 256;
+    A.tilesM = (int)((c.M + 255) / 256);
+    A.tilesN = (int)((c.N + wide - 1) / wide) * (KIND == GK_PAIR ? 2 : 1);
+    A.idesc = base | (uint32_t)c.a[0].mn << 15 | (uint32_t)c.b[0].mn << 16 | (256u >> 3) << 17 | (256u >> 4) << 24;
+    static OncePerDevice once;
+    static int room;
+    int smem;
+    if (const int64_t e = smem_for(once, &room, c.device, 512, k_gemm_pair<KIND, O>, smem); e < 0) return e;
+    static_assert(GP_STAGES * GP_STAGE + 1024 <= GM_SM_SMEM - 8192, "the ring fits");
+    cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, sms / 2);
+    cfg.blockDim = GP_T;
+    cfg.dynamicSmemBytes = smem;
+    CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_pair<KIND, O>, A));
+    return CLA_OK;
+  }
+  const int np = KIND == GK_GATE ? 2 : 1;
+  A.tilesM = (int)((c.M + A.nc - 1) / A.nc);
+  A.tilesN = (int)((c.N + 127) / 128) * (KIND == GK_PAIR ? 2 : 1);
+  A.idesc = base | (uint32_t)c.b[0].mn << 15 | (uint32_t)c.a[0].mn << 16 | (uint32_t)(A.nc >> 3) << 17 | (128u >> 4) << 24;
+  const int64_t tiles = (int64_t)A.tilesM * A.tilesN;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * sms && nk >= split * 4) split *= 2;
+  const int stage = np * (int)GM_OPERAND + A.nc * 128;
+  A.stages = std::min(16, (int)(104 * 1024 / stage));
+  if (A.stages < 4) A.stages = std::min(16, (int)(220 * 1024 / stage));
+  A.stages = std::max(1, std::min(A.stages, (nk + split - 1) / split));
+  static OncePerDevice once;
+  static int room;
+  int least;
+  if (const int64_t e = smem_for(once, &room, c.device, std::max(32, np * A.nc), k_gemm_few<KIND, O>, least); e < 0) return e;
+  const int smem = std::max(std::max(A.stages * stage, split > 1 ? np * A.nc * 512 : 0) + 1024, least);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)split, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cfg.gridDim = (unsigned)(tiles * split);
+  cfg.blockDim = GF_T;
+  cfg.dynamicSmemBytes = smem;
+  CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_few<KIND, O>, A));
+  return CLA_OK;
+}
+
 int64_t launch_gemm(const GemmCall& c, cudaStream_t s) {
   if (c.M == 0 || c.N == 0) return CLA_OK;
-  const dim3 grid((unsigned)((c.N + GS_T - 1) / GS_T), (unsigned)((c.M + GS_T - 1) / GS_T), c.kind == GK_PAIR ? 2 : 1);
-  if (c.type == CLA_T_I8) k_gemm_simple<int8_t><<<grid, 256, 0, s>>>(c);
-  else if (c.type == CLA_T_BF16) k_gemm_simple<__nv_bfloat16><<<grid, 256, 0, s>>>(c);
-  else k_gemm_simple<__half><<<grid, 256, 0, s>>>(c);
-  CLA_CUDA(cudaGetLastError());
-  return CLA_OK;
+  GemmArgs A = {};
+  A.c = c;
+  if (c.kind == GK_Q8) {
+    if (c.outType == CLA_T_F64) return launch_kind<GK_Q8, double>(A, s);
+    if (c.outType == CLA_T_F32) return launch_kind<GK_Q8, float>(A, s);
+    if (c.outType == CLA_T_BF16) return launch_kind<GK_Q8, __nv_bfloat16>(A, s);
+    return launch_kind<GK_Q8, __half>(A, s);
+  }
+  const bool bf = c.type == CLA_T_BF16;
+  if (c.kind == GK_GATE) return bf ? launch_kind<GK_GATE, __nv_bfloat16>(A, s) : launch_kind<GK_GATE, __half>(A, s);
+  if (c.kind == GK_SUM) return bf ? launch_kind<GK_SUM, __nv_bfloat16>(A, s) : launch_kind<GK_SUM, __half>(A, s);
+  return bf ? launch_kind<GK_PAIR, __nv_bfloat16>(A, s) : launch_kind<GK_PAIR, __half>(A, s);
 }
 
 }  // namespace cla
