@@ -15,7 +15,7 @@ constexpr int DN_T = 256;
 template <class T> constexpr int DN_V = 16 / (int)sizeof(T);
 template <class T>
 __device__ __forceinline__ void load_vec(const T* p, int n, bool vec, T (&v)[DN_V<T>]) {
-  if (vec && n == DN_V<T>) {
+  if (vec && n >= DN_V<T>) {
     *(uint4*)v = *(const uint4*)p;
   } else {
 #pragma unroll
@@ -24,7 +24,7 @@ __device__ __forceinline__ void load_vec(const T* p, int n, bool vec, T (&v)[DN_
 }
 template <class T>
 __device__ __forceinline__ void store_vec(T* p, int n, bool vec, const T (&v)[DN_V<T>]) {
-  if (vec && n == DN_V<T>) {
+  if (vec && n >= DN_V<T>) {
     *(uint4*)p = *(const uint4*)v;
   } else {
 #pragma unroll
@@ -36,36 +36,57 @@ inline bool rows_aligned(const void* p, int64_t ld, int64_t rows, int bytes, int
   return ((uintptr_t)p % to) == 0 && (rows <= 1 || (ld * bytes) % to == 0);
 }
 
+// Which pieces of a matrix a thread takes: 2^log adjacent threads along a row, the others of the block down the rows, U rows at a time so
+// that U loads are on their way before the first is used. f(r, c, n): rows r, r + step, .. (n of them), piece c of each.
+struct Walk {
+  int log;         // threads along a row
+  int64_t rows;
+  int per;         // pieces of a row
+};
+template <int U, class F>
+__device__ __forceinline__ void walk(const Walk& w, F&& f) {
+  const int tx = threadIdx.x & ((1 << w.log) - 1), down = DN_T >> w.log;
+  const int64_t step = (int64_t)gridDim.y * down;
+  for (int c = blockIdx.x * (1 << w.log) + tx; c < w.per; c += gridDim.x << w.log)
+    for (int64_t r = (int64_t)blockIdx.y * down + (threadIdx.x >> w.log); r < w.rows; r += U * step)
+      f(r, c, step, (int)min((int64_t)U, (w.rows - r + step - 1) / step));
+}
+
 // ---- dropout --------------------------------------------------------------------------------------------------------
-// A thread per 16 bytes of a row (F64: 32, the four columns of a counter). Bound: memory; the ten rounds are 40 multiplications for 4 columns.
-template <class T>
-__global__ void __launch_bounds__(DN_T) k_dropout(const T* x, int64_t ldx, int64_t rows, int64_t cols, T* y, int64_t ldy,
-                                                  const __grid_constant__ DropDev d, int vec) {
-  constexpr int V = DN_V<T> < 4 ? 4 : DN_V<T>;
-  const int64_t per = (cols + V - 1) / V, n = per * rows;
-  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
-    const int64_t r = i / per, c = (i - r * per) * V;
+// Pieces of 16 bytes (F64: 32, the four columns of a counter). Bound: the words (twenty 64-bit products and as many three-way logic
+// operations for four columns) next to memory.
+template <class T, int U>
+__global__ void __launch_bounds__(DN_T) k_dropout(const T* x, int64_t ldx, int64_t cols, T* y, int64_t ldy, const __grid_constant__ DropDev d,
+                                                  const __grid_constant__ Walk w, int vec) {
+  constexpr int P = DN_V<T>, V = P < 4 ? 4 : P;
+  walk<U>(w, [&](int64_t r, int piece, int64_t step, int n) {
+    const int64_t c = (int64_t)piece * V;
+    alignas(16) T v[U][V];
+    const int left = (int)min((int64_t)V, cols - c);
 #pragma unroll
-    for (int h = 0; h < V; h += DN_V<T>) {
-      const int left = (int)min((int64_t)DN_V<T>, cols - c - h);
-      if (left <= 0) break;
-      alignas(16) T v[DN_V<T>];
-      load_vec(x + r * ldx + c + h, left, vec, v);
+    for (int u = 0; u < U; u++)
+      if (u < n)
+#pragma unroll
+        for (int h = 0; h < V; h += P) load_vec(x + (r + u * step) * ldx + c + h, left - h, vec && left - h >= P, (T(&)[P])v[u][h]);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (u >= n) break;
       if (d.on) {
 #pragma unroll
-        for (int q = 0; q < DN_V<T>; q += 4) {
-          const uint4 w = drop_words(d, (uint32_t)r, (uint32_t)((c + h + q) / 4));
+        for (int q = 0; q < V; q += 4) {
+          const uint4 words = drop_words(d, (uint32_t)(r + u * step), (uint32_t)((c + q) / 4));
 #pragma unroll
-          for (int j = 0; j < (DN_V<T> < 4 ? DN_V<T> : 4); j++) {
-            const bool keep = word_of(w, DN_V<T> < 4 ? h + j : j) >= d.cut;
-            if constexpr (sizeof(T) == 8) v[q + j] = keep ? v[q + j] * d.scale64 : 0.0;
-            else v[q + j] = from_f32<T>(keep ? to_f32(v[q + j]) * d.scale : 0.f);
+          for (int j = 0; j < 4; j++) {
+            const bool keep = word_of(words, j) >= d.cut;
+            if constexpr (sizeof(T) == 8) v[u][q + j] = keep ? v[u][q + j] * d.scale64 : 0.0;
+            else v[u][q + j] = from_f32<T>(keep ? to_f32(v[u][q + j]) * d.scale : 0.f);
           }
         }
       }
-      store_vec(y + r * ldy + c + h, left, vec, v);
+#pragma unroll
+      for (int h = 0; h < V; h += P) store_vec(y + (r + u * step) * ldy + c + h, left - h, vec && left - h >= P, (const T(&)[P])v[u][h]);
     }
-  }
+  });
 }
 
 // ---- quantisation -----------------------------------------------------------------------------------------------------
@@ -76,15 +97,26 @@ template <> __device__ __forceinline__ double widen(double v) { return v; }
 
 template <class W> __device__ __forceinline__ W larger(W m, W a) { return a > m || a != a ? a : m; }  // (a NaN stays)
 template <class W> __device__ __forceinline__ float q8_scale(W most) { return (float)(most / (W)127); }
-// (divided, not multiplied by a reciprocal: the result is the nearest whole number of the quotient itself)
-template <class W> __device__ __forceinline__ int q8_of(W x, float scale, bool some) {
-  return some ? (int)fmin((W)127, fmax((W)-127, rint(x / (W)scale))) : 0;
-}
+// The nearest whole number of x / scale. The product with the reciprocal is off by three roundings of a value below 128: unless it comes that
+// near to a half, where the quotient itself decides, both have the same nearest whole number.
+template <class W> struct Q8Row {
+  W scale, inv;
+  bool some;
+  __device__ __forceinline__ explicit Q8Row(float s) : scale((W)s), inv((W)1 / (W)s), some(s > 0.f && s < INFINITY) {}
+  __device__ __forceinline__ int operator()(W x) const {
+    constexpr W NEAR = sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-14;  // 2^7 times 2^-50, 2^-21
+    const W t = x * inv;
+    W q = rint(t);
+    if (!(fabs(fabs(t - q) - (W)0.5) > NEAR)) q = rint(x / scale);  // (also where the reciprocal is not finite)
+    return some ? (int)fmin((W)127, fmax((W)-127, q)) : 0;
+  }
+};
 
-// G threads per row: its largest magnitude, then, from the caches, its quotients. Bound: memory, one pass over x.
-template <class T, int G>
+// G threads per row, which they keep in registers: its largest magnitude, then its quotients. One pass over x; rows longer than G * C pieces are
+// read a second time. Where rows do not start on 16-byte boundaries the threads take single values in turn. Bound: memory.
+template <class T, int G, int C>
 __global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, int8_t* __restrict__ q,
-                                                        int64_t ldq, float* __restrict__ scale, int vec, int vecQ) {
+                                                        int64_t ldq, float* __restrict__ scale, int vec) {
   using W = typename WideOf<T>::type;
   constexpr int V = DN_V<T>;
   __shared__ W part[DN_T / 32];
@@ -92,12 +124,32 @@ __global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x,
   const int64_t r = (int64_t)blockIdx.x * (DN_T / G) + threadIdx.x / G;
   if (G == 32 && r >= rows) return;
   const T* p = x + r * ldx;
-  W most = 0;
-  for (int64_t c = (int64_t)lane * V; c < cols; c += G * V) {
-    alignas(16) T v[V];
-    load_vec(p + c, (int)min((int64_t)V, cols - c), vec, v);
+  const int64_t n = cols;
+  alignas(16) T v[C][V];
+  auto load = [&](int64_t k0) {
 #pragma unroll
-    for (int i = 0; i < V; i++) most = larger(most, (W)fabs(widen(v[i])));
+    for (int k = 0; k < C; k++) {
+      const int64_t at = (k0 + k) * G * V;
+      if (vec) {
+        const int64_t c = at + lane * V;
+        load_vec(p + c, (int)max((int64_t)0, min((int64_t)V, n - c)), true, v[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const int64_t c = at + i * G + lane;
+          v[k][i] = c < n ? p[c] : from_f32<T>(0.f);
+        }
+      }
+    }
+  };
+  const int64_t rounds = (n + G * V * C - 1) / (G * V * C);
+  W most = 0;
+  for (int64_t k = 0; k < rounds; k++) {
+    load(k * C);
+#pragma unroll
+    for (int j = 0; j < C; j++)
+#pragma unroll
+      for (int i = 0; i < V; i++) most = larger(most, (W)fabs(widen(v[j][i])));
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
@@ -109,24 +161,30 @@ __global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x,
     for (int i = 1; i < DN_T / 32; i++) most = larger(most, part[i]);
   }
   const float s = q8_scale(most);
-  const bool some = s > 0.f && s < INFINITY;
+  const Q8Row<W> q8(s);
   if (lane == 0) scale[r] = s;
-  for (int64_t c = (int64_t)lane * V; c < cols; c += G * V) {
-    alignas(16) T v[V];
-    const int n = (int)min((int64_t)V, cols - c);
-    load_vec(p + c, n, vec, v);
-    alignas(16) int8_t o[V];
+  int8_t* to = q + r * ldq;
+  for (int64_t k = 0; k < rounds; k++) {
+    if (rounds > 1) load(k * C);
 #pragma unroll
-    for (int i = 0; i < V; i++) o[i] = (int8_t)q8_of(widen(v[i]), s, some);
-    int8_t* t = q + r * ldq + c;
-    if (vecQ && n == V) {
-      if constexpr (V == 8) *(uint2*)t = *(const uint2*)o;
-      else if constexpr (V == 4) *(uint32_t*)t = *(const uint32_t*)o;
-      else *(uint16_t*)t = *(const uint16_t*)o;
-    } else {
+    for (int j = 0; j < C; j++) {
+      const int64_t at = (k * C + j) * G * V;
+      if (at >= n) break;
+      alignas(16) int8_t o[V];
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (i < n) t[i] = o[i];
+      for (int i = 0; i < V; i++) o[i] = (int8_t)q8(widen(v[j][i]));
+      const int64_t c = at + lane * V;
+      if (vec && c + V <= n) {
+        if constexpr (V == 8) *(uint2*)(to + c) = *(const uint2*)o;
+        else if constexpr (V == 4) *(uint32_t*)(to + c) = *(const uint32_t*)o;
+        else *(uint16_t*)(to + c) = *(const uint16_t*)o;
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const int64_t e = vec ? c + i : at + i * G + lane;
+          if (e < n) to[e] = o[i];
+        }
+      }
     }
   }
 }
@@ -152,13 +210,12 @@ __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x,
     if (c < cols) scale[c] = sc[tx];
   }
   __syncthreads();
-  const float s = sc[tx];
-  const bool some = s > 0.f && s < INFINITY;
+  const Q8Row<W> q8(sc[tx]);
   for (int64_t r0 = 0; r0 < rows; r0 += 128) {
 #pragma unroll
     for (int i = 0; i < 128; i += 32) {
       const int64_t r = r0 + i + ty;
-      tile[tx][i + ty] = c < cols && r < rows ? (int8_t)q8_of(widen(x[r * ldx + c]), s, some) : 0;
+      tile[tx][i + ty] = c < cols && r < rows ? (int8_t)q8(widen(x[r * ldx + c])) : 0;
     }
     __syncthreads();
     const int64_t oc = (int64_t)blockIdx.x * 32 + ty;
@@ -171,58 +228,81 @@ __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x,
 }
 
 // ---- the gated block's elementwise gradients ----------------------------------------------------------------------------
-template <class T>
+template <class T, int U>
 __global__ void __launch_bounds__(DN_T) k_gate_grad(const T* __restrict__ dh, int64_t lddh, const T* __restrict__ g, int64_t ldg,
-                                                    const T* __restrict__ u, int64_t ldu, int64_t rows, int64_t cols, T* __restrict__ dg,
-                                                    T* __restrict__ du, int64_t ldo, const __grid_constant__ DropDev d, int act, int vec) {
+                                                    const T* __restrict__ u, int64_t ldu, int64_t cols, T* __restrict__ dg, T* __restrict__ du,
+                                                    int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w, int vec) {
   constexpr int V = DN_V<T>;
-  const int64_t per = (cols + V - 1) / V, n = per * rows;
-  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
-    const int64_t r = i / per, c = (i - r * per) * V;
+  walk<U>(w, [&](int64_t r, int piece, int64_t step, int n) {
+    const int64_t c = (int64_t)piece * V;
     const int left = (int)min((int64_t)V, cols - c);
-    alignas(16) T vh[V], vg[V], vu[V];
-    load_vec(dh + r * lddh + c, left, vec, vh);
-    load_vec(g + r * ldg + c, left, vec, vg);
-    load_vec(u + r * ldu + c, left, vec, vu);
+    alignas(16) T vh[U][V], vg[U][V], vu[U][V];
 #pragma unroll
-    for (int q = 0; q < V; q += 4) {
-      uint4 w;
-      if (d.on) w = drop_words(d, (uint32_t)r, (uint32_t)((c + q) / 4));
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        float h = to_f32(vh[q + j]), a;
-        if (d.on) h = word_of(w, j) >= d.cut ? h * d.scale : 0.f;
-        const float slope = act_slope(act, to_f32(vg[q + j]), a);
-        vg[q + j] = from_f32<T>(h * to_f32(vu[q + j]) * slope);
-        vu[q + j] = from_f32<T>(h * a);
+    for (int k = 0; k < U; k++)
+      if (k < n) {
+        const int64_t at = r + k * step;
+        load_vec(dh + at * lddh + c, left, vec, vh[k]);
+        load_vec(g + at * ldg + c, left, vec, vg[k]);
+        load_vec(u + at * ldu + c, left, vec, vu[k]);
       }
-    }
-    store_vec(dg + r * ldo + c, left, true, vg);
-    store_vec(du + r * ldo + c, left, true, vu);
-  }
+    with_act(act, [&](auto name) {
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        if (k >= n) break;
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+          uint4 words;
+          if (d.on) words = drop_words(d, (uint32_t)(r + k * step), (uint32_t)((c + q) / 4));
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float h = to_f32(vh[k][q + j]), a;
+            if (d.on) h = word_of(words, j) >= d.cut ? h * d.scale : 0.f;
+            const float slope = act_slope(decltype(name)::value, to_f32(vg[k][q + j]), a);
+            vg[k][q + j] = from_f32<T>(h * to_f32(vu[k][q + j]) * slope);
+            vu[k][q + j] = from_f32<T>(h * a);
+          }
+        }
+      }
+    });
+#pragma unroll
+    for (int k = 0; k < U; k++)
+      if (k < n) {
+        store_vec(dg + (r + k * step) * ldo + c, left, true, vg[k]);
+        store_vec(du + (r + k * step) * ldo + c, left, true, vu[k]);
+      }
+  });
 }
 
 // ---- copies -----------------------------------------------------------------------------------------------------------
-// Rows to rows that start on 16-byte boundaries, as the products read them: a thread per 16 bytes.
-template <class T>
-__global__ void __launch_bounds__(DN_T) k_repitch(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, T* __restrict__ y, int64_t ldy) {
+// Rows to rows that start on 16-byte boundaries, as the products read them.
+template <class T, int U>
+__global__ void __launch_bounds__(DN_T) k_repitch(const T* __restrict__ x, int64_t ldx, int64_t cols, T* __restrict__ y, int64_t ldy,
+                                                  const __grid_constant__ Walk w) {
   constexpr int V = DN_V<T>;
-  const int64_t per = (cols + V - 1) / V, n = per * rows;
-  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
-    const int64_t r = i / per, c = (i - r * per) * V;
-    alignas(16) T v[V];
+  walk<U>(w, [&](int64_t r, int piece, int64_t step, int n) {
+    const int64_t c = (int64_t)piece * V;
     const int left = (int)min((int64_t)V, cols - c);
-    load_vec(x + r * ldx + c, left, false, v);
-    store_vec(y + r * ldy + c, left, true, v);
-  }
+    alignas(16) T v[U][V];
+#pragma unroll
+    for (int k = 0; k < U; k++)
+      if (k < n) load_vec(x + (r + k * step) * ldx + c, left, false, v[k]);
+#pragma unroll
+    for (int k = 0; k < U; k++)
+      if (k < n) store_vec(y + (r + k * step) * ldy + c, left, true, v[k]);
+  });
 }
-template <class T>
-__global__ void __launch_bounds__(DN_T) k_narrow(const double* __restrict__ x, int64_t rows, int64_t cols, T* __restrict__ y, int64_t ldy) {
-  const int64_t n = rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * DN_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DN_T) {
-    const int64_t r = i / cols;
-    y[r * ldy + i - r * cols] = from_f64<T>(x[i]);
-  }
+template <class T, int U>
+__global__ void __launch_bounds__(DN_T) k_narrow(const double* __restrict__ x, int64_t cols, T* __restrict__ y, int64_t ldy,
+                                                 const __grid_constant__ Walk w) {
+  walk<U>(w, [&](int64_t r, int c, int64_t step, int n) {
+    double v[U];
+#pragma unroll
+    for (int k = 0; k < U; k++)
+      if (k < n) v[k] = x[(r + k * step) * cols + c];
+#pragma unroll
+    for (int k = 0; k < U; k++)
+      if (k < n) y[(r + k * step) * ldy + c] = from_f64<T>(v[k]);
+  });
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -246,7 +326,16 @@ struct OnDevice {
   }
 };
 
-unsigned blocks_for(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + DN_T - 1) / DN_T, 148 * 16)); }
+// The grid of a walk over rows of `per` pieces, `at` rows at a time: eight CTAs an SM, or fewer
+dim3 walk_grid(Walk& w, int64_t rows, int64_t per, int at) {
+  w.rows = rows;
+  w.per = (int)per;
+  w.log = 0;
+  while (w.log < 8 && (1 << w.log) < per) w.log++;
+  const int64_t x = (per + (1 << w.log) - 1) >> w.log, down = DN_T >> w.log;
+  const int64_t most = std::max<int64_t>(1, 148 * 8 / x), need = (rows + down * at - 1) / (down * at);
+  return dim3((unsigned)std::min<int64_t>(x, 148 * 8), (unsigned)std::max<int64_t>(1, std::min(most, need)));
+}
 
 int64_t check_matrix(const char* what, const void* p, int64_t rows, int64_t cols, int64_t ld, int bytes) {
   if (rows < 0 || cols < 0) return fail(CLA_ERR_SHAPE, std::string(what) + ": negative size");
@@ -269,7 +358,10 @@ int64_t drop_device(const cla_drop& d, int64_t rows, DropDev& o) {
   o.on = d.p > 0.0;
   o.cut = (uint32_t)std::floor(d.p * 4294967296.0);
   o.row0 = (uint32_t)d.row0;
-  o.seed[0] = (uint32_t)d.seed, o.seed[1] = (uint32_t)(d.seed >> 32);
+  for (uint32_t i = 0; i < 10; i++) {
+    o.key[2 * i] = (uint32_t)d.seed + i * 0x9E3779B9u;
+    o.key[2 * i + 1] = (uint32_t)(d.seed >> 32) + i * 0xBB67AE85u;
+  }
   o.step[0] = (uint32_t)d.step, o.step[1] = (uint32_t)(d.step >> 32);
   o.scale64 = 1.0 / (1.0 - d.p);
   o.scale = (float)o.scale64;
@@ -294,12 +386,13 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
       k_quantize_cols<T><<<(unsigned)((cols + 31) / 32), dim3(32, 32), 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale);
       return;
     }
-    const int vec = rows_aligned(x, ldx, rows, sizeof(T)), vecQ = rows_aligned(q, ldq, rows, 1, DN_V<T>);
-    // rows of up to 8 vectors a lane: a warp each, no barrier; longer ones a CTA each
-    if (cols <= 32 * 8 * DN_V<T> && rows >= 148)
-      k_quantize_rows<T, 32><<<(unsigned)((rows + DN_T / 32 - 1) / (DN_T / 32)), DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec, vecQ);
+    constexpr int V = DN_V<T>, C = 8;
+    const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
+    // a warp per row, without a barrier, where it holds the row and there are rows enough
+    if (cols <= 32 * C * V && rows >= 148)
+      k_quantize_rows<T, 32, C><<<(unsigned)((rows + DN_T / 32 - 1) / (DN_T / 32)), DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec);
     else
-      k_quantize_rows<T, DN_T><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec, vecQ);
+      k_quantize_rows<T, DN_T, C><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec);
   });
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;
@@ -324,9 +417,10 @@ int64_t aligned(GemmOperand& o, int64_t i, int64_t k, int type, Work& w, bool ru
   const int64_t ld = round_up(cols, 16 / bytes);
   void* to = w.take(rows * ld * bytes);
   if (run && rows && cols) {
-    const unsigned b = blocks_for(rows * ((cols * bytes + 15) / 16));
-    if (bytes == 1) k_repitch<int8_t><<<b, DN_T, 0, s>>>((const int8_t*)o.p, o.ld, rows, cols, (int8_t*)to, ld);
-    else k_repitch<__half><<<b, DN_T, 0, s>>>((const __half*)o.p, o.ld, rows, cols, (__half*)to, ld);
+    Walk k;
+    const dim3 grid = walk_grid(k, rows, (cols * bytes + 15) / 16, 2);
+    if (bytes == 1) k_repitch<int8_t, 2><<<grid, DN_T, 0, s>>>((const int8_t*)o.p, o.ld, cols, (int8_t*)to, ld, k);
+    else k_repitch<__half, 2><<<grid, DN_T, 0, s>>>((const __half*)o.p, o.ld, cols, (__half*)to, ld, k);
     CLA_CUDA(cudaGetLastError());
   }
   o.p = to;
@@ -425,11 +519,12 @@ int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
   void* du = w.take(c.M * ld * 2);
   if (run && c.M && c.F) {
     const int vec = rows_aligned(c.dh, c.lddh, c.M, 2) && rows_aligned(c.g, c.ldg, c.M, 2) && rows_aligned(c.u, c.ldu, c.M, 2);
-    const unsigned b = blocks_for(c.M * (ld / 8));
+    Walk k;
+    const dim3 grid = walk_grid(k, c.M, ld / 8, 2);
     auto go = [&](auto t) {
       using T = decltype(t);
-      k_gate_grad<T><<<b, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.M, c.F, (T*)dg, (T*)du, ld, d,
-                                        c.act, vec);
+      k_gate_grad<T, 2><<<grid, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld, d, c.act, k,
+                                              vec);
     };
     if (c.type == CLA_T_BF16) go(__nv_bfloat16());
     else go(__half());
@@ -516,7 +611,9 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
     using T = decltype(t);
     constexpr int V = std::max(4, DN_V<T>);
     const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(y, ldy, rows, sizeof(T));
-    k_dropout<T><<<blocks_for(rows * ((cols + V - 1) / V)), DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, rows, cols, (T*)y, ldy, d, vec);
+    Walk w;
+    const dim3 grid = walk_grid(w, rows, (cols + V - 1) / V, 4);
+    k_dropout<T, 4><<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w, vec);
   });
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;
@@ -594,7 +691,9 @@ int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_
   const int64_t rc = for_rows(m, row0, rows, (double*)work, cap, s, [&](int64_t r, int64_t n, const double* X) -> int64_t {
     with_type(type, [&](auto t) {
       using T = decltype(t);
-      k_narrow<T><<<blocks_for(n * m->nCols), DN_T, 0, s>>>(X, n, m->nCols, (T*)out + (r - row0) * ldo, ldo);
+      Walk w;
+      const dim3 grid = walk_grid(w, n, m->nCols, 4);
+      k_narrow<T, 4><<<grid, DN_T, 0, s>>>(X, m->nCols, (T*)out + (r - row0) * ldo, ldo, w);
     });
     m->stats.kernel_launches++;
     CLA_CUDA(cudaGetLastError());

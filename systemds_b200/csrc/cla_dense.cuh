@@ -26,47 +26,50 @@ template <> __device__ __forceinline__ __half from_f64(double v) { return __doub
 struct DropDev {
   uint32_t cut = 0;  // kept where word >= cut
   uint32_t row0 = 0;
-  uint32_t seed[2] = {}, step[2] = {};
+  uint32_t key[20] = {}, step[2] = {};  // the rounds' keys, the same for every counter
   float scale = 1.f;
   double scale64 = 1.0;
   int on = 0;
 };
 // The four words of columns 4 c .. 4 c + 3 of a row: Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011)
 __device__ __forceinline__ uint4 drop_words(const DropDev& d, uint32_t row, uint32_t c) {
-  uint32_t x0 = c, x1 = d.row0 + row, x2 = d.step[0], x3 = d.step[1], k0 = d.seed[0], k1 = d.seed[1];
+  uint32_t x0 = c, x1 = d.row0 + row, x2 = d.step[0], x3 = d.step[1];
 #pragma unroll
   for (int i = 0; i < 10; i++) {
     const uint64_t a = (uint64_t)0xD2511F53u * x0, b = (uint64_t)0xCD9E8D57u * x2;
-    x0 = (uint32_t)(b >> 32) ^ x1 ^ k0;
+    x0 = (uint32_t)(b >> 32) ^ x1 ^ d.key[2 * i];
     x1 = (uint32_t)b;
-    x2 = (uint32_t)(a >> 32) ^ x3 ^ k1;
+    x2 = (uint32_t)(a >> 32) ^ x3 ^ d.key[2 * i + 1];
     x3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(x0, x1, x2, x3);
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 
 // ---- the activation, in FP32 ------------------------------------------------------------------------------------------
+// With the fast exponential and quotient: off by some units of 2^-23, under 2^-20 of the value where |g| < 10 (beyond, a unit more for each
+// of g's), next to the 2^-11 or 2^-8 of the rounding that follows.
+__device__ __forceinline__ float sigmoid_of(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+// (1 + tanh(y)) / 2 is sigmoid(2 y)
+__device__ __forceinline__ float gelu_arg(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
 __device__ __forceinline__ float act_value(int act, float g) {
   switch (act) {
-    case CLA_ACT_SILU: return g / (1.f + expf(-g));
-    case CLA_ACT_SIGMOID: return 1.f / (1.f + expf(-g));
+    case CLA_ACT_SILU: return g * sigmoid_of(g);
+    case CLA_ACT_SIGMOID: return sigmoid_of(g);
     case CLA_ACT_RELU: return g < 0.f ? 0.f : g;
     case CLA_ACT_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-    default: return 0.5f * g * (1.f + tanhf(0.79788456080286536f * (g + 0.044715f * g * g * g)));
+    default: return g * sigmoid_of(gelu_arg(g));
   }
 }
 __device__ __forceinline__ float act_slope(int act, float g, float& value) {
   switch (act) {
     case CLA_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-g));
+      const float s = sigmoid_of(g);
       value = g * s;
       return s * (1.f + g * (1.f - s));
     }
     case CLA_ACT_SIGMOID: {
-      const float s = 1.f / (1.f + expf(-g));
+      const float s = sigmoid_of(g);
       value = s;
       return s * (1.f - s);
     }
@@ -74,13 +77,22 @@ __device__ __forceinline__ float act_slope(int act, float g, float& value) {
     case CLA_ACT_GELU: {
       const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
       value = g * c;
-      return c + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+      return c + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
     }
     default: {
-      const float t = tanhf(0.79788456080286536f * (g + 0.044715f * g * g * g));
-      value = 0.5f * g * (1.f + t);
-      return 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * g * g);
+      const float s = sigmoid_of(gelu_arg(g));
+      value = g * s;
+      return s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
     }
+  }
+}
+template <class F> __device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {
+    case CLA_ACT_SILU: f(std::integral_constant<int, CLA_ACT_SILU>()); break;
+    case CLA_ACT_GELU: f(std::integral_constant<int, CLA_ACT_GELU>()); break;
+    case CLA_ACT_GELU_TANH: f(std::integral_constant<int, CLA_ACT_GELU_TANH>()); break;
+    case CLA_ACT_RELU: f(std::integral_constant<int, CLA_ACT_RELU>()); break;
+    default: f(std::integral_constant<int, CLA_ACT_SIGMOID>()); break;
   }
 }
 

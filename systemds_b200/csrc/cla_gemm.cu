@@ -133,6 +133,7 @@ struct alignas(64) GemmArgs {
   int depth;             // values of a stage
   int kBlocks;           // stages of a segment
   int tilesM, tilesN;    // PAIR: tilesN of both products
+  int wide;              // k_gemm_pair: columns of a tile (GATE: of each product)
   int nc, stages;        // k_gemm_few: rows of a tile, stages of the ring
   uint32_t idesc;
 };
@@ -140,26 +141,59 @@ struct alignas(64) GemmArgs {
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f32<O>(v); }
 
-// N values of a row, the first `valid` of them; vec: the row's pieces start on 16-byte boundaries
-template <class O, int N>
-__device__ __forceinline__ void gm_store(O* p, int valid, bool vec, const O (&v)[N]) {
-  constexpr int V = 16 / (int)sizeof(O);
-  if (vec && valid >= N) {
+// 32 rows (a lane each) of `width` columns to memory. f(j, o): columns j .. j + 15 of the lane's row, all lanes together. vec: the rows' pieces
+// start on 16-byte boundaries, and a lane writes its own; else they go through the warp's 4 KB of shared memory, 128 bytes of every row at
+// a time, and are written row by row, a word or its two halves a lane.
+template <class O, class F>
+__device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t cols, int width, bool vec, uint32_t buf, F&& f) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    O* p = out + lane * ld;
+#pragma unroll 1
+    for (int j = 0; j < width; j += 16) {
+      alignas(16) O o[16];
+      f(j, o);
+      const int valid = lane < rows ? (int)min((int64_t)16, cols - j) : 0;
+      if (valid == 16) {
 #pragma unroll
-    for (int i = 0; i < N; i += V) *(uint4*)(p + i) = *(const uint4*)(v + i);
-  } else {
+        for (int i = 0; i < 16; i += 16 / (int)sizeof(O)) *(uint4*)(p + j + i) = *(const uint4*)(o + i);
+      } else {
 #pragma unroll
-    for (int i = 0; i < N; i++)
-      if (i < valid) p[i] = v[i];
+        for (int i = 0; i < 16; i++)
+          if (i < valid) p[j + i] = o[i];
+      }
+      __syncwarp();
+    }
+    return;
   }
-}
-template <class F> __device__ __forceinline__ void with_act(int act, F&& f) {
-  switch (act) {
-    case CLA_ACT_SILU: f(std::integral_constant<int, CLA_ACT_SILU>()); break;
-    case CLA_ACT_GELU: f(std::integral_constant<int, CLA_ACT_GELU>()); break;
-    case CLA_ACT_GELU_TANH: f(std::integral_constant<int, CLA_ACT_GELU_TANH>()); break;
-    case CLA_ACT_RELU: f(std::integral_constant<int, CLA_ACT_RELU>()); break;
-    default: f(std::integral_constant<int, CLA_ACT_SIGMOID>()); break;
+  constexpr int PIECE = 128 / (int)sizeof(O), WORDS = 16 * (int)sizeof(O) / 4;
+#pragma unroll 1
+  for (int c0 = 0; c0 < width; c0 += PIECE) {
+#pragma unroll 1
+    for (int j = 0; j < min(PIECE, width - c0); j += 16) {
+      alignas(16) O o[16];
+      f(c0 + j, o);
+      const int w0 = j * (int)sizeof(O) / 4;
+#pragma unroll
+      for (int i = 0; i < WORDS; i++)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + (lane * 32 + ((w0 + i) ^ lane)) * 4), "r"(((const uint32_t*)o)[i]) : "memory");
+    }
+    __syncwarp();
+    // the elements of word `lane`
+    const int64_t left = min((int64_t)min(PIECE, width - c0), cols - c0) * (int)sizeof(O) - 4 * lane;
+    for (int r = 0; r < rows; r++) {
+      uint32_t v;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buf + (r * 32 + (lane ^ r)) * 4) : "memory");
+      char* p = (char*)(out + r * ld + c0) + 4 * lane;
+      if (sizeof(O) >= 4 || ((uintptr_t)p & 3) == 0) {
+        if (left >= 4) *(uint32_t*)p = v;
+        else if (left > 0) *(uint16_t*)p = (uint16_t)v;
+      } else {
+        if (left > 0) *(uint16_t*)p = (uint16_t)v;
+        if (left > 2) *(uint16_t*)(p + 2) = (uint16_t)(v >> 16);
+      }
+    }
+    __syncwarp();
   }
 }
 template <int KIND, class O>
@@ -169,8 +203,8 @@ __device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa,
 }
 
 // ---- large results --------------------------------------------------------------------------------------------------------
-// Tile 256 x 256 per pair of CTAs (GATE: 256 x 128 of both products): each CTA holds the sums of its 128 rows and brings 128 rows and 128
-// columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight take the sums out of one half of
+// Tile 256 x 256 per pair of CTAs (GATE: 256 x 128 of both products; narrower for few columns): each CTA holds the sums of its 128 rows and
+// brings 128 rows and 128 columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight take the sums out of one half of
 // tensor memory while the other fills. A launch's pairs take tiles in turn, along the rows within groups of GP_GROUP row tiles, so that what
 // runs at once shares operands in L2.
 constexpr int GP_T = 384, GP_STAGES = 6, GP_STAGE = 2 * GM_OPERAND, GP_GROUP = 8;
@@ -193,6 +227,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
   const int pairs = gridDim.x / 2, pair = blockIdx.x / 2, tiles = A.tilesM * A.tilesN;
   const int segments = KIND == GK_SUM ? 2 : 1, nk = A.kBlocks * segments;
   const bool aMn = !I8 && c.a[0].mn, bMn = !I8 && c.b[0].mn;
+  const int mine = KIND == GK_GATE ? A.wide : A.wide / 2;  // columns that a CTA brings
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -225,13 +260,13 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
         gp_tile(A, t, tm, tn);
         const int m0 = tm * 256 + rank * 128;
         const int halfN = A.tilesN / 2, which = KIND == GK_GATE ? (int)rank : KIND == GK_PAIR && tn >= halfN;
-        const int n0 = KIND == GK_GATE ? tn * 128 : (KIND == GK_PAIR && tn >= halfN ? tn - halfN : tn) * 256 + rank * 128;
+        const int n0 = KIND == GK_GATE ? tn * A.wide : (KIND == GK_PAIR && tn >= halfN ? tn - halfN : tn) * A.wide + rank * mine;
         for (int kb = 0; kb < nk; kb++) {
           ok = gm_wait(gm_smem(empty + s), ph);
           if (!ok) break;
           const int seg = KIND == GK_SUM && kb >= A.kBlocks, k0 = (kb - seg * A.kBlocks) * A.depth;
           const uint32_t bar = gm_peer(gm_smem(full + s), 0), da = smem + s * GP_STAGE, db = da + GM_OPERAND;
-          if (rank == 0) gm_expect(gm_smem(full + s), 2 * GP_STAGE);
+          if (rank == 0) gm_expect(gm_smem(full + s), 2 * (GM_OPERAND + mine * 128));
           const CUtensorMap *ma = A.a + seg, *mb = A.b + (KIND == GK_SUM ? seg : which);
           if (aMn) {
             gm_load<true>(da, ma, m0, k0, bar);
@@ -240,8 +275,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
             gm_load<true>(da, ma, k0, m0, bar);
           }
           if (bMn) {
-            gm_load<true>(db, mb, n0, k0, bar);
-            gm_load<true>(db + 8192, mb, n0 + 64, k0, bar);
+            for (int i = 0; i < mine; i += 64) gm_load<true>(db + i * 128, mb, n0 + i, k0, bar);
           } else {
             gm_load<true>(db, mb, k0, n0, bar);
           }
@@ -290,28 +324,17 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       int tm, tn;
       gp_tile(A, t, tm, tn);
-      const int64_t m = (int64_t)tm * 256 + rank * 128 + quarter * 32 + lane;
-      const uint32_t at = tmem + buf * 256 + ((uint32_t)quarter << 21);
+      const int64_t m0 = (int64_t)tm * 256 + rank * 128 + quarter * 32, m = m0 + lane;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, c.M - m0)), width = A.wide / 2;
+      const uint32_t at = tmem + buf * 256 + half * width + ((uint32_t)quarter << 21), room = smem + GP_STAGES * GP_STAGE + (warp - 4) * 4096;
+      auto aligned = [&](int o) { return ((uintptr_t)c.out[o] | (uintptr_t)(c.ldo[o] * sizeof(O))) % 16 == 0; };
       if constexpr (KIND == GK_GATE) {
-        const int64_t n0 = (int64_t)tn * 128 + half * 64;
-        const bool vec = ((uintptr_t)c.out[0] | (uintptr_t)(c.ldo[0] * 2) | (uintptr_t)c.out[1] | (uintptr_t)(c.ldo[1] * 2) | (uintptr_t)c.out[2] |
-                          (uintptr_t)(c.ldo[2] * 2)) % 16 == 0;
-#pragma unroll 1
-        for (int j = 0; j < 64; j += 16) {
+        const int64_t n0 = (int64_t)tn * A.wide + half * width;
+        gm_rows((O*)c.out[0] + m0 * c.ldo[0] + n0, c.ldo[0], rows, c.N - n0, width, aligned(0), room, [&](int j, O(&o)[16]) {
           uint32_t v[32];
-          gm_tmem16(at + half * 64 + j, v);
-          gm_tmem16(at + 128 + half * 64 + j, v + 16);
+          gm_tmem16(at + j, v);
+          gm_tmem16(at + A.wide + j, v + 16);
           gm_loaded(v);
-          const int valid = m < c.M ? (int)min((int64_t)16, c.N - n0 - j) : 0;
-          alignas(16) O o[16];
-          if (c.out[1]) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(__uint_as_float(v[i]));
-            gm_store((O*)c.out[1] + m * c.ldo[1] + n0 + j, valid, vec, o);
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(__uint_as_float(v[16 + i]));
-            gm_store((O*)c.out[2] + m * c.ldo[2] + n0 + j, valid, vec, o);
-          }
           float h[16];
           with_act(c.act, [&](auto act) {
 #pragma unroll
@@ -327,30 +350,30 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
           }
 #pragma unroll
           for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(h[i]);
-          gm_store((O*)c.out[0] + m * c.ldo[0] + n0 + j, valid, vec, o);
-          __syncwarp();
-        }
+        });
+        if (c.out[1])
+          for (int p = 0; p < 2; p++)
+            gm_rows((O*)c.out[1 + p] + m0 * c.ldo[1 + p] + n0, c.ldo[1 + p], rows, c.N - n0, width, aligned(1 + p), room, [&](int j, O(&o)[16]) {
+              uint32_t v[16];
+              gm_tmem16(at + p * A.wide + j, v);
+              gm_loaded(v);
+#pragma unroll
+              for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(__uint_as_float(v[i]));
+            });
       } else {
         const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
-        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * 256 + half * 128;
-        O* out = (O*)c.out[which] + m * c.ldo[which] + n0;
-        const bool vec = ((uintptr_t)c.out[which] | (uintptr_t)(c.ldo[which] * sizeof(O))) % 16 == 0;
+        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * A.wide + half * width;
         const float sa = I8 && m < c.M ? c.aScale[m] : 0.f;
-#pragma unroll 1
-        for (int j = 0; j < 128; j += 16) {
+        gm_rows((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, width, aligned(which), room, [&](int j, O(&o)[16]) {
           uint32_t v[16];
-          gm_tmem16(at + half * 128 + j, v);
+          gm_tmem16(at + j, v);
           gm_loaded(v);
-          const int valid = m < c.M ? (int)min((int64_t)16, c.N - n0 - j) : 0;
-          alignas(16) O o[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, i < valid ? __ldg(c.bScale + n0 + j + i) : 0.f);
+            if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
             else o[i] = gm_cast<O>(__uint_as_float(v[i]));
           }
-          gm_store(out + j, valid, vec, o);
-          __syncwarp();
-        }
+        });
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -606,6 +629,45 @@ static int64_t smem_for(OncePerDevice& once, int* room, int device, int cols, K 
   return rc;
 }
 
+// Which kernel and tile: the one that a count of clocks makes the fastest.
+struct GemmPlan {
+  bool large = false;
+  int wide = 0;                      // k_gemm_pair
+  int nc = 0, split = 1, stages = 1; // k_gemm_few
+  double clocks = 1e30;
+};
+static GemmPlan gemm_plan(const GemmCall& c, int nk, int sms) {
+  GemmPlan best;
+  const int np = c.kind == GK_GATE ? 2 : 1, products = c.kind == GK_PAIR ? 2 : 1;
+  const auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const double L2 = 40;  // bytes a clock that an SM gets
+  for (int wide = 256 / np; wide >= 64 && nk > 0; wide /= 2) {
+    const int mine = np == 2 ? wide : wide / 2;
+    if (c.b[0].mn && mine < 64) break;
+    const int64_t tiles = ceil_div(c.M, 256) * ceil_div(c.N, wide) * products, turns = ceil_div(tiles, sms / 2);
+    const double step = std::max(2.0 * mine * 2, (GM_OPERAND + mine * 128) / L2 / 1.5), t = 5000 + turns * (nk * step + 600);
+    if (t < best.clocks) best.large = true, best.wide = wide, best.clocks = t;
+  }
+  for (int nc = 16; nc <= 128; nc *= 2) {
+    const int least = c.a[0].mn ? 64 : 16;
+    if (nc < least) continue;
+    if (nc > least && nc / 2 >= c.M) break;
+    const int stage = np * (int)GM_OPERAND + nc * 128;
+    const int64_t tiles = ceil_div(c.M, nc) * ceil_div(c.N, 128) * products;
+    for (int split = 1; split <= 8 && split <= std::max(1, nk); split++) {
+      const int perSm = 2 * stage <= 111 * 1024 && (split == 1 || np * nc * 512 <= 111 * 1024) ? 2 : 1;
+      const int64_t ctas = tiles * split, slots = (int64_t)sms * perSm, turns = ceil_div(ctas, slots);
+      const double together = std::min<double>(perSm, (double)ceil_div(ctas, sms));
+      const double step = together * std::max(2.0 * nc * np, stage / L2), t = 4000 + (split > 1 ? 1500 + nc * np * 4 : 0) + turns * (ceil_div(nk, split) * step + 2000 + nc * 20);
+      if (t < best.clocks) {
+        best.large = false, best.nc = nc, best.split = split, best.clocks = t;
+        best.stages = (int)std::max<int64_t>(1, std::min<int64_t>({16, (ctas > sms && perSm == 2 ? 111 : 220) * 1024 / stage, ceil_div(nk, split)}));
+      }
+    }
+  }
+  return best;
+}
+
 template <int KIND, class O>
 static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   const GemmCall& c = A.c;
@@ -615,62 +677,50 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   A.depth = 128 / bytes;
   A.kBlocks = (int)((c.K + A.depth - 1) / A.depth);
   const int nk = A.kBlocks * segs;
+  const GemmPlan p = gemm_plan(c, nk, sms);
   // both operands' types, where their index is contiguous, sums in 32 bits
   const uint32_t type = c.type == CLA_T_BF16 || c.type == CLA_T_I8 ? 1u : 0u;
   const uint32_t base = (KIND == GK_Q8 ? 2u : 1u) << 4 | type << 7 | type << 10;
   cudaLaunchConfig_t cfg = {};
   cfg.stream = s;
-  const bool large = c.M > 128 && nk > 0;
-  for (int i = 0; i < 2; i++) {
-    const bool hasA = i == 0 || KIND == GK_SUM, hasB = i == 0 || KIND != GK_Q8;
-    int nc = 128;
-    if (!large)
-      while (nc > 16 && nc / 2 >= c.M && !(c.a[0].mn && nc == 64)) nc /= 2;
-    A.nc = nc;
-    if (nk == 0) continue;
-    if (hasA)
-      if (const int64_t rc = operand_map(A.a[i], c.a[i], c.type, c.M, c.K, nc); rc < 0) return rc;
-    if (hasB)
-      if (const int64_t rc = operand_map(A.b[i], c.b[i], c.type, c.N, c.K, 128); rc < 0) return rc;
-  }
-  if (large) {
-    const int wide = KIND == GK_GATE ? 128 : 256;
+  if (nk > 0)
+    for (int i = 0; i < 2; i++) {
+      const int boxB = !p.large ? 128 : KIND == GK_GATE ? p.wide : p.wide / 2;
+      if (i == 0 || KIND == GK_SUM)
+        if (const int64_t rc = operand_map(A.a[i], c.a[i], c.type, c.M, c.K, p.large ? 128 : p.nc); rc < 0) return rc;
+      if (i == 0 || KIND != GK_Q8)
+        if (const int64_t rc = operand_map(A.b[i], c.b[i], c.type, c.N, c.K, boxB); rc < 0) return rc;
+    }
+  const int np = KIND == GK_GATE ? 2 : 1, products = KIND == GK_PAIR ? 2 : 1;
+  static OncePerDevice oncePair, onceFew;
+  static int roomPair, roomFew;
+  int smem;
+  if (p.large) {
+    A.wide = p.wide;
     A.tilesM = (int)((c.M + 255) / 256);
-    A.tilesN = (int)((c.N + wide - 1) / wide) * (KIND == GK_PAIR ? 2 : 1);
-    A.idesc = base | (uint32_t)c.a[0].mn << 15 | (uint32_t)c.b[0].mn << 16 | (256u >> 3) << 17 | (256u >> 4) << 24;
-    static OncePerDevice once;
-    static int room;
-    int smem;
-    if (const int64_t e = smem_for(once, &room, c.device, 512, k_gemm_pair<KIND, O>, smem); e < 0) return e;
-    static_assert(GP_STAGES * GP_STAGE + 1024 <= GM_SM_SMEM - 8192, "the ring fits");
+    A.tilesN = (int)((c.N + p.wide - 1) / p.wide) * products;
+    A.idesc = base | (uint32_t)c.a[0].mn << 15 | (uint32_t)c.b[0].mn << 16 | (uint32_t)(p.wide * np >> 3) << 17 | (256u >> 4) << 24;
+    if (const int64_t e = smem_for(oncePair, &roomPair, c.device, 512, k_gemm_pair<KIND, O>, smem); e < 0) return e;
+    static_assert(GP_STAGES * GP_STAGE + 1024 + 8 * 4096 <= GM_SM_SMEM - GM_CTA_SMEM - 1024, "the ring and the warps' rooms fit");
     cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, sms / 2);
     cfg.blockDim = GP_T;
     cfg.dynamicSmemBytes = smem;
     CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
   }
-  const int np = KIND == GK_GATE ? 2 : 1;
+  A.nc = p.nc;
+  A.stages = p.stages;
   A.tilesM = (int)((c.M + A.nc - 1) / A.nc);
-  A.tilesN = (int)((c.N + 127) / 128) * (KIND == GK_PAIR ? 2 : 1);
+  A.tilesN = (int)((c.N + 127) / 128) * products;
   A.idesc = base | (uint32_t)c.b[0].mn << 15 | (uint32_t)c.a[0].mn << 16 | (uint32_t)(A.nc >> 3) << 17 | (128u >> 4) << 24;
-  const int64_t tiles = (int64_t)A.tilesM * A.tilesN;
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * sms && nk >= split * 4) split *= 2;
-  const int stage = np * (int)GM_OPERAND + A.nc * 128;
-  A.stages = std::min(16, (int)(104 * 1024 / stage));
-  if (A.stages < 4) A.stages = std::min(16, (int)(220 * 1024 / stage));
-  A.stages = std::max(1, std::min(A.stages, (nk + split - 1) / split));
-  static OncePerDevice once;
-  static int room;
-  int least;
-  if (const int64_t e = smem_for(once, &room, c.device, std::max(32, np * A.nc), k_gemm_few<KIND, O>, least); e < 0) return e;
-  const int smem = std::max(std::max(A.stages * stage, split > 1 ? np * A.nc * 512 : 0) + 1024, least);
+  if (const int64_t e = smem_for(onceFew, &roomFew, c.device, std::max(32, np * A.nc), k_gemm_few<KIND, O>, smem); e < 0) return e;
+  smem = std::max(smem, std::max(A.stages * (np * (int)GM_OPERAND + A.nc * 128), p.split > 1 ? np * A.nc * 512 : 0) + 1024);
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)split, 1, 1};
+  at[0].val.clusterDim = {(unsigned)p.split, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cfg.gridDim = (unsigned)(tiles * split);
+  cfg.gridDim = (unsigned)((int64_t)A.tilesM * A.tilesN * p.split);
   cfg.blockDim = GF_T;
   cfg.dynamicSmemBytes = smem;
   CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_few<KIND, O>, A));
