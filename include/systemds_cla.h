@@ -305,7 +305,8 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
 /* Quantises rows (byCols 0) or columns (1) of x [rows x cols] (F64, F32, BF16, F16): scale[i] = fl32(largest magnitude / 127), q = x / scale[i]
  * to the nearest whole number (even on ties, within -127..127; the division in FP64 for F64, else FP32). Where scale[i] is 0 or not finite q
  * is 0: a row of zeros gives zeros, one with an infinity or a NaN gives NaN in the product. byCols 0: q [rows x cols];
- * byCols 1: q [cols x rows], a row per column of x, as cla_q8_mm_dev takes weights. ldq: elements between the rows of q. */
+ * byCols 1: q [cols x rows], a row per column of x, as cla_q8_mm_dev takes weights. ldq: elements between the rows of q. At most 2^30 rows
+ * and columns. */
 int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t byCols, int8_t* q, int64_t ldq,
                             float* scale, int32_t device, void* stream);
 

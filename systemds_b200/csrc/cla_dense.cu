@@ -95,8 +95,13 @@ template <> struct WideOf<double> { using type = double; };
 template <class T> __device__ __forceinline__ typename WideOf<T>::type widen(T v) { return to_f32(v); }
 template <> __device__ __forceinline__ double widen(double v) { return v; }
 
-template <class W> __device__ __forceinline__ W larger(W m, W a) { return a > m || a != a ? a : m; }  // (a NaN stays)
-template <class W> __device__ __forceinline__ float q8_scale(W most) { return (float)(most / (W)127); }
+// Magnitudes as whole numbers, which have the values' order with infinity and then NaN as the largest
+__device__ __forceinline__ unsigned long long magnitude(double v) { return (unsigned long long)__double_as_longlong(v) & 0x7fffffffffffffffull; }
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float q8_scale(unsigned long long most) { return (float)(__longlong_as_double((long long)most) / 127.0); }
+__device__ __forceinline__ float q8_scale(uint32_t most) { return __uint_as_float(most) / 127.f; }
+__device__ __forceinline__ int whole(double v) { return __double2int_rn(v); }
+__device__ __forceinline__ int whole(float v) { return __float2int_rn(v); }
 // The nearest whole number of x / scale. The product with the reciprocal is off by three roundings of a value below 128: unless it comes that
 // near to a half, where the quotient itself decides, both have the same nearest whole number.
 template <class W> struct Q8Row {
@@ -104,85 +109,84 @@ template <class W> struct Q8Row {
   bool some;
   __device__ __forceinline__ explicit Q8Row(float s) : scale((W)s), inv((W)1 / (W)s), some(s > 0.f && s < INFINITY) {}
   __device__ __forceinline__ int operator()(W x) const {
-    constexpr W NEAR = sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-14;  // 2^7 times 2^-50, 2^-21
+    constexpr W FAR = (W)0.5 - (sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-14);  // 2^7 times 2^-50, 2^-21
     const W t = x * inv;
-    W q = rint(t);
-    if (!(fabs(fabs(t - q) - (W)0.5) > NEAR)) q = rint(x / scale);  // (also where the reciprocal is not finite)
-    return some ? (int)fmin((W)127, fmax((W)-127, q)) : 0;
+    int q = whole(t);
+    if (!(fabs(t - (W)q) <= FAR)) q = whole(x / scale);  // (also where the reciprocal is not finite)
+    return some ? min(127, max(-127, q)) : 0;
   }
 };
 
 // G threads per row, which they keep in registers: its largest magnitude, then its quotients. One pass over x; rows longer than G * C pieces are
 // read a second time. Where rows do not start on 16-byte boundaries the threads take single values in turn. Bound: memory.
 template <class T, int G, int C>
-__global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, int8_t* __restrict__ q,
+__global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int8_t* __restrict__ q,
                                                         int64_t ldq, float* __restrict__ scale, int vec) {
   using W = typename WideOf<T>::type;
+  using Bits = decltype(magnitude(W()));
   constexpr int V = DN_V<T>;
-  __shared__ W part[DN_T / 32];
+  __shared__ Bits part[DN_T / 32];
   const int lane = threadIdx.x % G, warp = threadIdx.x / 32;
   const int64_t r = (int64_t)blockIdx.x * (DN_T / G) + threadIdx.x / G;
   if (G == 32 && r >= rows) return;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the product's weights may come meanwhile)
   const T* p = x + r * ldx;
-  const int64_t n = cols;
   alignas(16) T v[C][V];
-  auto load = [&](int64_t k0) {
+  auto load = [&](int first) {
 #pragma unroll
     for (int k = 0; k < C; k++) {
-      const int64_t at = (k0 + k) * G * V;
-      if (vec) {
-        const int64_t c = at + lane * V;
-        load_vec(p + c, (int)max((int64_t)0, min((int64_t)V, n - c)), true, v[k]);
+      const int at = first + k * G * V, c = at + lane * V;
+      if (vec && c + V <= cols) {
+        *(uint4*)v[k] = *(const uint4*)(p + c);
       } else {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          const int64_t c = at + i * G + lane;
-          v[k][i] = c < n ? p[c] : from_f32<T>(0.f);
+          const int e = vec ? c + i : at + i * G + lane;
+          v[k][i] = e < cols ? p[e] : from_f32<T>(0.f);
         }
       }
     }
   };
-  const int64_t rounds = (n + G * V * C - 1) / (G * V * C);
-  W most = 0;
-  for (int64_t k = 0; k < rounds; k++) {
-    load(k * C);
+  constexpr int ROUND = G * V * C;
+  Bits most = 0;
+  for (int first = 0; first < cols; first += ROUND) {
+    load(first);
 #pragma unroll
     for (int j = 0; j < C; j++)
 #pragma unroll
-      for (int i = 0; i < V; i++) most = larger(most, (W)fabs(widen(v[j][i])));
+      for (int i = 0; i < V; i++) most = max(most, magnitude(widen(v[j][i])));
   }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
+  for (int d = 16; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
   if (G > 32) {
     if (threadIdx.x % 32 == 0) part[warp] = most;
     __syncthreads();
     most = part[0];
 #pragma unroll
-    for (int i = 1; i < DN_T / 32; i++) most = larger(most, part[i]);
+    for (int i = 1; i < DN_T / 32; i++) most = max(most, part[i]);
   }
   const float s = q8_scale(most);
   const Q8Row<W> q8(s);
   if (lane == 0) scale[r] = s;
   int8_t* to = q + r * ldq;
-  for (int64_t k = 0; k < rounds; k++) {
-    if (rounds > 1) load(k * C);
+  for (int first = 0; first < cols; first += ROUND) {
+    if (cols > ROUND) load(first);
 #pragma unroll
     for (int j = 0; j < C; j++) {
-      const int64_t at = (k * C + j) * G * V;
-      if (at >= n) break;
+      const int at = first + j * G * V, c = at + lane * V;
+      if (at >= cols) break;
       alignas(16) int8_t o[V];
 #pragma unroll
       for (int i = 0; i < V; i++) o[i] = (int8_t)q8(widen(v[j][i]));
-      const int64_t c = at + lane * V;
-      if (vec && c + V <= n) {
+      if (vec && c + V <= cols) {
         if constexpr (V == 8) *(uint2*)(to + c) = *(const uint2*)o;
         else if constexpr (V == 4) *(uint32_t*)(to + c) = *(const uint32_t*)o;
         else *(uint16_t*)(to + c) = *(const uint16_t*)o;
       } else {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          const int64_t e = vec ? c + i : at + i * G + lane;
-          if (e < n) to[e] = o[i];
+          const int e = vec ? c + i : at + i * G + lane;
+          if (e < cols) to[e] = o[i];
         }
       }
     }
@@ -194,18 +198,19 @@ template <class T>
 __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, int8_t* __restrict__ q,
                                                         int64_t ldq, float* __restrict__ scale) {
   using W = typename WideOf<T>::type;
-  __shared__ W part[32][33];
+  using Bits = decltype(magnitude(W()));
+  __shared__ Bits part[32][33];
   __shared__ float sc[32];
   __shared__ int8_t tile[32][132];
   const int tx = threadIdx.x, ty = threadIdx.y;
   const int64_t c = (int64_t)blockIdx.x * 32 + tx;
-  W most = 0;
+  Bits most = 0;
   if (c < cols)
-    for (int64_t r = ty; r < rows; r += 32) most = larger(most, (W)fabs(widen(x[r * ldx + c])));
+    for (int64_t r = ty; r < rows; r += 32) most = max(most, magnitude(widen(x[r * ldx + c])));
   part[ty][tx] = most;
   __syncthreads();
   if (ty == 0) {
-    for (int i = 1; i < 32; i++) most = larger(most, part[i][tx]);
+    for (int i = 1; i < 32; i++) most = max(most, part[i][tx]);
     sc[tx] = q8_scale(most);
     if (c < cols) scale[c] = sc[tx];
   }
@@ -386,13 +391,13 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
       k_quantize_cols<T><<<(unsigned)((cols + 31) / 32), dim3(32, 32), 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale);
       return;
     }
-    constexpr int V = DN_V<T>, C = 8;
+    constexpr int V = DN_V<T>, C = sizeof(T) == 8 ? 8 : 4;
     const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
     // a warp per row, without a barrier, where it holds the row and there are rows enough
     if (cols <= 32 * C * V && rows >= 148)
-      k_quantize_rows<T, 32, C><<<(unsigned)((rows + DN_T / 32 - 1) / (DN_T / 32)), DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec);
+      k_quantize_rows<T, 32, C><<<(unsigned)((rows + DN_T / 32 - 1) / (DN_T / 32)), DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale, vec);
     else
-      k_quantize_rows<T, DN_T, C><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, cols, q, ldq, scale, vec);
+      k_quantize_rows<T, DN_T, C><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale, vec);
   });
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;
@@ -428,6 +433,11 @@ int64_t aligned(GemmOperand& o, int64_t i, int64_t k, int type, Work& w, bool ru
   return CLA_OK;
 }
 
+int64_t product(GemmCall& g, Work& w, bool run, cudaStream_t s) {
+  if (const int64_t n = gemm_workspace(g)) g.parts = w.take(n);
+  return run ? launch_gemm(g, s) : CLA_OK;
+}
+
 int64_t check_q8(const cla_q8* c) {
   if (!c) return fail(CLA_ERR_BAD_ARG, "8-bit product: null arguments");
   if (c->aType != CLA_T_I8 && !is_float_type(c->aType)) return fail(CLA_ERR_UNSUPPORTED, "8-bit product: type of a");
@@ -439,7 +449,7 @@ int64_t check_q8(const cla_q8* c) {
   if (c->M && c->N && ((c->aType == CLA_T_I8 && !c->aScale) || !c->bScale)) return fail(CLA_ERR_BAD_ARG, "8-bit product: null scales");
   return CLA_OK;
 }
-int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s) {
+int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s, bool split = true) {
   GemmCall g;
   g.kind = GK_Q8;
   g.type = CLA_T_I8;
@@ -450,7 +460,9 @@ int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s) {
   g.out[0] = c.out, g.ldo[0] = c.ldo;
   g.aScale = c.aScale, g.bScale = c.bScale;
   g.device = c.device;
+  g.split = split;
   if (c.M == 0 || c.N == 0) return CLA_OK;
+  DN_CHECK(aligned(g.b[0], c.N, c.K, CLA_T_I8, w, run, s));
   if (c.aType != CLA_T_I8) {
     const int64_t ld = round_up(c.K, 16);
     int8_t* q = (int8_t*)w.take(c.M * ld);
@@ -458,11 +470,11 @@ int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s) {
     if (run) DN_CHECK(quantize(c.aType, c.a, c.lda, c.M, c.K, false, q, ld, sc, s));
     g.a[0] = {q, ld, false};
     g.aScale = sc;
+    g.aLate = c.K > 0;  // (the last kernel before the product)
   } else {
     DN_CHECK(aligned(g.a[0], c.M, c.K, CLA_T_I8, w, run, s));
   }
-  DN_CHECK(aligned(g.b[0], c.N, c.K, CLA_T_I8, w, run, s));
-  return run ? launch_gemm(g, s) : CLA_OK;
+  return product(g, w, run, s);
 }
 
 int64_t check_gated(const cla_gated* c, bool backward, DropDev& d) {
@@ -511,7 +523,7 @@ int64_t gated_fwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
   g.out[0] = c.h, g.out[1] = c.g, g.out[2] = c.u;
   g.ldo[0] = c.ldh, g.ldo[1] = c.ldg, g.ldo[2] = c.ldu;
   g.drop = d;
-  return run ? launch_gemm(g, s) : CLA_OK;
+  return product(g, w, run, s);
 }
 int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaStream_t s) {
   const int64_t ld = round_up(c.F, 8);
@@ -520,10 +532,10 @@ int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
   if (run && c.M && c.F) {
     const int vec = rows_aligned(c.dh, c.lddh, c.M, 2) && rows_aligned(c.g, c.ldg, c.M, 2) && rows_aligned(c.u, c.ldu, c.M, 2);
     Walk k;
-    const dim3 grid = walk_grid(k, c.M, ld / 8, 2);
+    const dim3 grid = walk_grid(k, c.M, ld / 8, 1);
     auto go = [&](auto t) {
       using T = decltype(t);
-      k_gate_grad<T, 2><<<grid, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld, d, c.act, k,
+      k_gate_grad<T, 1><<<grid, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld, d, c.act, k,
                                               vec);
     };
     if (c.type == CLA_T_BF16) go(__nv_bfloat16());
@@ -538,7 +550,7 @@ int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
     g.b[1] = {c.wu, c.ldwu, (bool)c.wTrans};
     for (int i = 0; i < 2; i++) DN_CHECK(aligned(g.b[i], c.D, c.F, c.type, w, run, s));
     g.out[0] = c.dx, g.ldo[0] = c.lddx;
-    if (run) DN_CHECK(launch_gemm(g, s));
+    DN_CHECK(product(g, w, run, s));
   }
   if (c.dwg && c.D && c.F) {
     GemmCall g = gated_call(c, GK_PAIR, c.D, c.F, c.M);
@@ -548,7 +560,7 @@ int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
     DN_CHECK(aligned(g.a[0], c.D, c.M, c.type, w, run, s));
     g.out[0] = c.dwg, g.out[1] = c.dwu;
     g.ldo[0] = c.lddwg, g.ldo[1] = c.lddwu;
-    if (run) DN_CHECK(launch_gemm(g, s));
+    DN_CHECK(product(g, w, run, s));
   }
   return CLA_OK;
 }
@@ -577,7 +589,7 @@ int64_t chunk_rows(const Matrix* m, int64_t rows) {
   const int64_t cols = std::max(m->nCols, 1), most = std::max<int64_t>(1, ROWS_CHUNK / 8 / cols / SKIP_ROWS);
   return std::min(most, rows / SKIP_ROWS + 2) * SKIP_ROWS;
 }
-// what a chunk of so many rows needs beside its cells: q and scales, and b where its rows are not aligned
+// What the 8-bit product of a chunk of so many rows needs: their cells, q and scales
 int64_t q8_chunk_bytes(const Matrix* m, int64_t rows) {
   return round_up(rows * round_up(m->nCols, 16), 256) + round_up(rows * 4, 256) + round_up(rows * m->nCols * 8, 256);
 }
@@ -612,8 +624,8 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
     constexpr int V = std::max(4, DN_V<T>);
     const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(y, ldy, rows, sizeof(T));
     Walk w;
-    const dim3 grid = walk_grid(w, rows, (cols + V - 1) / V, 4);
-    k_dropout<T, 4><<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w, vec);
+    const dim3 grid = walk_grid(w, rows, (cols + V - 1) / V, 1);
+    k_dropout<T, 1><<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w, vec);
   });
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;
@@ -626,6 +638,7 @@ int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t ro
   DN_CHECK(check_matrix("quantize, x", x, rows, cols, ldx, type_bytes(type)));
   DN_CHECK(check_matrix("quantize, q", q, byCols ? cols : rows, byCols ? rows : cols, ldq, 1));
   if ((byCols ? cols : rows) && !scale) return fail(CLA_ERR_BAD_ARG, "quantize: null scales");
+  if (rows > 1 << 30 || cols > 1 << 30) return fail(CLA_ERR_UNSUPPORTED, "quantize: more than 2^30 rows or columns");
   OnDevice on(device);
   if (on.rc < 0) return on.rc;
   return quantize(type, x, ldx, rows, cols, byCols, q, ldq, scale, (cudaStream_t)stream);
@@ -741,7 +754,7 @@ int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* 
       part.a = cells;
       part.out = (char*)out + r * ldo * type_bytes(outType);
       Work q = w;
-      return q8_run(part, true, q, s);
+      return q8_run(part, true, q, s, false);  // (rows enough without: its workspace goes by the rows alone)
     });
   const int64_t rc2 = order_end(m, s);
   return rc < 0 ? rc : rc2;

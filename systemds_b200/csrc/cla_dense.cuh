@@ -119,7 +119,12 @@ struct GemmCall {
   int act = 0;
   DropDev drop;
   int device = 0;
+  bool split = true;      // whether the depth may be split (gemm_workspace() is 0 if not)
+  void* parts = nullptr;  // gemm_workspace() bytes, 256-byte aligned
+  bool aLate = false;     // the kernel before this one in the stream writes a (and aScale) and nothing else that is read here, and
+                          // itself started after everything before it was done
 };
+int64_t gemm_workspace(const GemmCall& c);  // goes by the sizes, the types and which index is contiguous
 int64_t launch_gemm(const GemmCall& c, cudaStream_t s);
 int64_t dense_status(int device);  // the self-check word of the product kernels, cleared
 

@@ -1,7 +1,9 @@
 // Products of dense operands in 8 and 16 bits with their epilogues (GemmCall of cla_dense.cuh), on the 5th-generation tensor cores: operands by
 // TMA into 128-byte-swizzled shared memory, sums in tensor memory (FP32, or 32-bit integers for 8-bit operands), epilogues from there.
 //  * k_gemm_pair: two CTAs share a 256 x 256 tile. For large results.
-//  * k_gemm_few: one CTA per 128 columns of the result and 16 to 128 of its rows, the depth split over a cluster. For few rows.
+//  * k_gemm_few: tiles of 128 columns of the result and 16 to 128 of its rows, whose depth the CTAs share evenly; k_gemm_join adds up the
+//    parts of tiles that several CTAs share. For few rows.
+// Both are launched with at most one CTA an SM, which takes all of the SM's shared and tensor memory and loops: no CTA waits for tensor memory.
 #include <cuda.h>
 #include <algorithm>
 #include "cla_dense.cuh"
@@ -12,11 +14,6 @@ static __device__ int32_t denseErr;
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t gm_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ uint64_t gm_now() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ bool gm_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -25,20 +22,11 @@ __device__ __forceinline__ bool gm_try(uint32_t bar, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-// Gives up after GM_LIMIT ns: far longer than any launch, so that a mistake ends as an error and not as a hung GPU
-constexpr uint64_t GM_LIMIT = 8000000000ull;
-__device__ __noinline__ bool gm_wait_long(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = gm_now();
-  do {
-    for (int i = 0; i < 64; i++)
-      if (gm_try(bar, parity)) return true;
-  } while (gm_now() - t0 < GM_LIMIT);
-  return false;
-}
+// Gives up after some seconds, far longer than any launch: a mistake ends as an error and not as a hung GPU
 __device__ __forceinline__ bool gm_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < 32; i++)
+  for (int i = 0; i < (1 << 22); i++)
     if (gm_try(bar, parity)) return true;
-  return gm_wait_long(bar, parity);
+  return false;
 }
 __device__ __forceinline__ uint32_t gm_rank() {
   uint32_t r;
@@ -50,8 +38,11 @@ __device__ __forceinline__ uint32_t gm_peer(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// (the warps whole before and after: what follows may need all lanes together)
 __device__ __forceinline__ void gm_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncwarp();
 }
 __device__ __forceinline__ bool gm_elect() {
   uint32_t r;
@@ -134,7 +125,9 @@ struct alignas(64) GemmArgs {
   int kBlocks;           // stages of a segment
   int tilesM, tilesN;    // PAIR: tilesN of both products
   int wide;              // k_gemm_pair: columns of a tile (GATE: of each product)
-  int nc, stages;        // k_gemm_few: rows of a tile, stages of the ring
+  int nc, stages;        // k_gemm_few: rows of a tile, stages of the ring,
+  int ctas, whole;       // CTAs, and whether each has whole tiles
+  int early;             // whether the weights need not wait for the kernel before
   uint32_t idesc;
 };
 
@@ -377,7 +370,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0)
+      if (lane == 0 && t + 2 * pairs < tiles)  // (somebody waits for it: no arrival on its way when the CTAs end)
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gm_peer(gm_smem(sumEmpty + buf), 0)) : "memory");
     }
   }
@@ -393,33 +386,69 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
-// A CTA per 128 columns of the result (the lanes of tensor memory) and nc rows, so that little of the tensor cores' width is spent on
-// rows that are not there; the depth is split over the CTAs of a cluster, whose partial sums meet in shared memory, each CTA adding up its
-// share of the rows in the order of the ranks. GATE: both weights' tiles in a stage, two sums.
-constexpr int GF_T = 192;
+// Tiles of 128 columns of the result (the lanes of tensor memory) by nc rows, so that little of the tensor cores' width is spent on rows that are
+// not there; GATE: both weights' tiles in a stage, two sums. The stages of all tiles, one tile after the other, are dealt to the CTAs in even
+// ranges (or in whole tiles, where that takes no longer). A CTA writes the results of the tiles that are its own alone; of a tile that it shares its
+// sums go to the workspace, in its first room where its range starts in the tile, in its second where it ends there, and k_gemm_join
+// adds them up in the order of the depth.
+// The operand of the rows may come from the kernel before (quantised activations), whose end is waited for only where they are
+// needed: the weights are on their way by then.
+constexpr int GF_T = 256, GF_STAGES = 16, GF_RING = 220 * 1024;
+
+__device__ __forceinline__ void gm_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void gm_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// The first stage of CTA i's range; `whole`: of tiles. (of n stages in tiles of nk)
+__host__ __device__ inline int64_t gf_start(int64_t i, int ctas, int64_t n, int nk, bool whole) {
+  return whole ? n / nk * i / ctas * nk : n * i / ctas;
+}
+
+template <int KIND, class O>
+__device__ __forceinline__ void gm_finish(const GemmCall& c, int which, int64_t m, int64_t n, uint32_t v0, uint32_t v1, float sb) {
+  if constexpr (KIND == GK_Q8) {
+    ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<KIND, O>(c, (int32_t)v0, c.aScale[m], sb);
+  } else if constexpr (KIND == GK_GATE) {
+    const float g = __uint_as_float(v0), u = __uint_as_float(v1);
+    float h = act_value(c.act, g) * u;
+    if (c.drop.on) h = word_of(drop_words(c.drop, (uint32_t)m, (uint32_t)(n / 4)), (int)(n & 3)) >= c.drop.cut ? h * c.drop.scale : 0.f;
+    ((O*)c.out[0])[m * c.ldo[0] + n] = gm_cast<O>(h);
+    if (c.out[1]) {
+      ((O*)c.out[1])[m * c.ldo[1] + n] = gm_cast<O>(g);
+      ((O*)c.out[2])[m * c.ldo[2] + n] = gm_cast<O>(u);
+    }
+  } else {
+    ((O*)c.out[which])[m * c.ldo[which] + n] = gm_cast<O>(__uint_as_float(v0));
+  }
+}
+
+// Tile t: its product (PAIR), first column and first row. Tiles of the same columns lie next to each other: their CTAs share the weights in L2.
+template <int KIND>
+__device__ __forceinline__ void gf_tile(const GemmArgs& A, int64_t t, int& which, int& n0, int64_t& m0) {
+  int tn = (int)(t / A.tilesM);
+  m0 = (t - (int64_t)tn * A.tilesM) * A.nc;
+  which = KIND == GK_PAIR && tn >= A.tilesN / 2;
+  n0 = (which ? tn - A.tilesN / 2 : tn) * 128;
+}
 
 template <int KIND, class O>
 __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ GemmArgs A) {
   constexpr bool I8 = KIND == GK_Q8;
   constexpr int NP = KIND == GK_GATE ? 2 : 1;
-  constexpr int MOST = 16;
   extern __shared__ __align__(1024) unsigned char gmsm[];
-  __shared__ __align__(8) uint64_t full[MOST], empty[MOST], sumFull;
+  __shared__ __align__(8) uint64_t full[GF_STAGES], empty[GF_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
   const GemmCall& c = A.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = gm_rank(), smem = (gm_smem(gmsm) + 1023u) & ~1023u;
-  uint32_t split;
-  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(split));
-  const int tile = blockIdx.x / split, tn = tile % A.tilesN, tm = tile / A.tilesN;
-  const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
-  const int n0 = (which ? tn - halfN : tn) * 128, m0 = tm * A.nc;
-  const int nk = A.kBlocks * (KIND == GK_SUM ? 2 : 1);
-  const int kb0 = (int)((int64_t)nk * rank / split), kb1 = (int)((int64_t)nk * (rank + 1) / split);
+  const uint32_t smem = (gm_smem(gmsm) + 1023u) & ~1023u;
+  const int nk = max(1, A.kBlocks * (KIND == GK_SUM ? 2 : 1));  // (a depth of zero: one stage that nothing is added from)
+  const bool none = A.kBlocks == 0;
+  const int64_t n = (int64_t)A.tilesM * A.tilesN * nk;
+  const int64_t b0 = gf_start(blockIdx.x, gridDim.x, n, nk, A.whole), b1 = gf_start(blockIdx.x + 1, gridDim.x, n, nk, A.whole);
   const bool cMn = !I8 && c.a[0].mn, lMn = !I8 && c.b[0].mn;  // the result's rows and columns
-  const uint32_t stage = NP * GM_OPERAND + A.nc * 128, cols = max(32, NP * A.nc);
-  if (warp == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gm_smem(&tmemAt)), "r"(cols) : "memory");
+  const uint32_t stage = NP * GM_OPERAND + A.nc * 128;
+  if (!A.whole) gm_let_next();
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (threadIdx.x == 0) {
@@ -427,7 +456,10 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       gm_init(gm_smem(full + i), 1);
       gm_init(gm_smem(empty + i), 1);
     }
-    gm_init(gm_smem(&sumFull), 1);
+    for (int i = 0; i < 2; i++) {
+      gm_init(gm_smem(sumFull + i), 1);
+      gm_init(gm_smem(sumEmpty + i), 4);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -436,15 +468,20 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmemAt;
   bool ok = true;
-  if (warp == 4) {
-    if (gm_elect()) {
-      int s = 0, issued = 0;
-      uint32_t ph = 1;
-      for (int kb = kb0; kb < kb1; kb++) {
-        ok = gm_wait(gm_smem(empty + s), ph);
-        if (!ok) break;
-        const int seg = KIND == GK_SUM && kb >= A.kBlocks, k0 = (kb - seg * A.kBlocks) * A.depth;
-        const uint32_t bar = gm_smem(full + s), dl = smem + s * stage, dc = dl + NP * GM_OPERAND;
+  if (warp == 0) {
+    if (!none && gm_elect()) {
+      auto at = [&](int64_t b, int& which, int& n0, int64_t& m0, int& seg, int& k0) {
+        const int64_t t = b / nk;
+        const int kb = (int)(b - t * nk);
+        gf_tile<KIND>(A, t, which, n0, m0);
+        seg = KIND == GK_SUM && kb >= A.kBlocks;
+        k0 = (kb - seg * A.kBlocks) * A.depth;
+      };
+      auto columns = [&](int64_t b, int s) {
+        int which, n0, seg, k0;
+        int64_t m0;
+        at(b, which, n0, m0, seg, k0);
+        const uint32_t bar = gm_smem(full + s), dl = smem + s * stage;
         gm_expect(bar, stage);
 #pragma unroll
         for (int p = 0; p < NP; p++) {
@@ -456,123 +493,169 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
             gm_load<false>(dl + p * GM_OPERAND, ml, k0, n0, bar);
           }
         }
+      };
+      auto rows = [&](int64_t b, int s) {
+        int which, n0, seg, k0;
+        int64_t m0;
+        at(b, which, n0, m0, seg, k0);
+        const uint32_t bar = gm_smem(full + s), dc = smem + s * stage + NP * GM_OPERAND;
         if (cMn) {
-          for (int i = 0; i < A.nc; i += 64) gm_load<false>(dc + i * 128, A.a + seg, m0 + i, k0, bar);
+          for (int i = 0; i < A.nc; i += 64) gm_load<false>(dc + i * 128, A.a + seg, (int)m0 + i, k0, bar);
         } else {
-          gm_load<false>(dc, A.a + seg, k0, m0, bar);
+          gm_load<false>(dc, A.a + seg, k0, (int)m0, bar);
         }
+      };
+      const int64_t ahead = A.early ? min((int64_t)A.stages, b1 - b0) : 0;  // stages whose weights do not wait for the kernel before
+      for (int64_t i = 0; i < ahead; i++) columns(b0 + i, (int)i);
+      gm_after_previous();
+      int s = 0;
+      int64_t issued = 0;
+      uint32_t ph = 1;
+      for (int64_t b = b0; b < b1; b++) {
+        if (issued >= ahead) {
+          ok = gm_wait(gm_smem(empty + s), ph);
+          if (!ok) break;
+          columns(b, s);
+        }
+        rows(b, s);
         issued++;
         if (++s == A.stages) s = 0, ph ^= 1;
       }
-      for (int i = 0; i < min(issued, A.stages); i++) {
-        const int n = (issued - i + A.stages - 1) / A.stages;
-        if (!ok) gm_wait(gm_smem(full + i), (uint32_t)(n - 1) & 1u);
-        else if (!gm_wait(gm_smem(empty + i), (uint32_t)(n - 1) & 1u)) ok = false;
+      for (int i = 0; i < A.stages; i++) {
+        const int64_t times = (issued - i + A.stages - 1) / A.stages;  // that stage i was filled
+        if (times <= 0) break;
+        if (!ok) gm_wait(gm_smem(full + i), (uint32_t)(times - 1) & 1u);
+        else if (!gm_wait(gm_smem(empty + i), (uint32_t)(times - 1) & 1u)) ok = false;
       }
     }
-  } else if (warp == 5) {
-    if (gm_elect()) {
-      int s = 0;
-      uint32_t ph = 0;
-      for (int kb = kb0; kb < kb1; kb++) {
-        ok = gm_wait(gm_smem(full + s), ph);
+  } else if (warp == 1) {
+    if (!none && gm_elect()) {
+      int s = 0, buf = 0;
+      uint32_t ph = 0, phSum = 1;
+      for (int64_t b = b0; b < b1 && ok;) {
+        const int64_t end = min(b1, (b / nk + 1) * nk);  // of this tile's part of the range
+        ok = gm_wait(gm_smem(sumEmpty + buf), phSum);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t dl = smem + s * stage;
-        uint64_t b = gm_desc(dl + NP * GM_OPERAND, cMn);
-        uint64_t l[NP];
+        bool add = false;
+        for (; b < end; b++) {
+          ok = gm_wait(gm_smem(full + s), ph);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t dl = smem + s * stage;
+          uint64_t d = gm_desc(dl + NP * GM_OPERAND, cMn);
+          uint64_t l[NP];
 #pragma unroll
-        for (int p = 0; p < NP; p++) l[p] = gm_desc(dl + p * GM_OPERAND, lMn);
+          for (int p = 0; p < NP; p++) l[p] = gm_desc(dl + p * GM_OPERAND, lMn);
 #pragma unroll
-        for (int i = 0; i < 4; i++, b += gm_step(cMn))
+          for (int i = 0; i < 4; i++, d += gm_step(cMn), add = true)
 #pragma unroll
-          for (int p = 0; p < NP; p++) {
-            gm_mma<false, I8>(tmem + p * A.nc, l[p], b, A.idesc, kb > kb0 || i > 0);
-            l[p] += gm_step(lMn);
-          }
-        gm_commit<false>(gm_smem(empty + s));
-        if (++s == A.stages) s = 0, ph ^= 1;
-      }
-      if (ok) gm_commit<false>(gm_smem(&sumFull));
-    }
-  } else {
-    ok = gm_wait(gm_smem(&sumFull), 0);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  }
-  __syncwarp();
-  // The sums of lane n0 + 32 warp + lane (a column of the result), rows m0 .. m0 + nc
-  const int rows = (int)min((int64_t)A.nc, c.M - m0);
-  const int64_t n = n0 + warp * 32 + lane;
-  const float sb = I8 && warp < 4 && n < c.N ? c.bScale[n] : 0.f;
-  auto put = [&](int r, const uint32_t (&v)[NP]) {
-    const int64_t m = m0 + r;
-    if (n >= c.N) return;
-    if constexpr (I8) {
-      ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<KIND, O>(c, (int32_t)v[0], c.aScale[m], sb);
-    } else if constexpr (KIND == GK_GATE) {
-      const float g = __uint_as_float(v[0]), u = __uint_as_float(v[1]);
-      float h = act_value(c.act, g) * u;
-      if (c.drop.on) h = word_of(drop_words(c.drop, (uint32_t)m, (uint32_t)(n / 4)), (int)(n & 3)) >= c.drop.cut ? h * c.drop.scale : 0.f;
-      ((O*)c.out[0])[m * c.ldo[0] + n] = gm_cast<O>(h);
-      if (c.out[1]) {
-        ((O*)c.out[1])[m * c.ldo[1] + n] = gm_cast<O>(g);
-        ((O*)c.out[2])[m * c.ldo[2] + n] = gm_cast<O>(u);
-      }
-    } else {
-      ((O*)c.out[which])[m * c.ldo[which] + n] = gm_cast<O>(__uint_as_float(v[0]));
-    }
-  };
-  const uint32_t at = tmem + ((uint32_t)(warp & 3) << 21);
-  if (warp < 4) {
-    for (int r = 0; r < rows; r += 16) {
-      uint32_t v[NP * 16];
-#pragma unroll
-      for (int p = 0; p < NP; p++) gm_tmem16(at + p * A.nc + r, v + 16 * p);
-      gm_loaded(v);
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        if (r + i >= rows) break;
-        uint32_t w[NP];
-#pragma unroll
-        for (int p = 0; p < NP; p++) w[p] = kb1 > kb0 ? v[16 * p + i] : 0u;
-        if (split == 1) put(r + i, w);
-        else
-#pragma unroll
-          for (int p = 0; p < NP; p++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem + ((p * A.nc + r + i) * 128 + threadIdx.x) * 4), "r"(w[p]) : "memory");
-      }
-      __syncwarp();
-    }
-  }
-  if (split > 1) {
-    gm_cluster_sync();
-    if (warp < 4) {
-      for (int r = rank; r < rows; r += split) {
-        uint32_t w[NP];
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-          const uint32_t mine = smem + ((p * A.nc + r) * 128 + threadIdx.x) * 4;
-          float f = 0.f;
-          uint32_t sum = 0;
-          for (uint32_t q = 0; q < split; q++) {
-            uint32_t x;
-            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(x) : "r"(gm_peer(mine, q)) : "memory");
-            if (I8) sum += x;
-            else f += __uint_as_float(x);
-          }
-          w[p] = I8 ? sum : __float_as_uint(f);
+            for (int p = 0; p < NP; p++) {
+              gm_mma<false, I8>(tmem + buf * 256 + p * A.nc, l[p], d, A.idesc, add);
+              l[p] += gm_step(lMn);
+            }
+          gm_commit<false>(gm_smem(empty + s));
+          if (++s == A.stages) s = 0, ph ^= 1;
         }
-        put(r, w);
+        if (ok) gm_commit<false>(gm_smem(sumFull + buf));
+        buf ^= 1;
+        if (buf == 0) phSum ^= 1;
       }
+    }
+  } else if (warp >= 4) {
+    gm_after_previous();
+    const int quarter = warp - 4;
+    int buf = 0;
+    uint32_t ph = 0;
+    for (int64_t b = b0; b < b1;) {
+      const int64_t t = b / nk, end = min(b1, (t + 1) * nk);
+      const bool mine = b == t * nk && end == (t + 1) * nk;
+      int which, n0;
+      int64_t m0;
+      gf_tile<KIND>(A, t, which, n0, m0);
+      if (!none) {
+        ok = gm_wait(gm_smem(sumFull + buf), ph);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      const int rows = (int)min((int64_t)A.nc, c.M - m0);
+      const int64_t col = n0 + quarter * 32 + lane;  // the lane's column of the result
+      const float sb = I8 && col < c.N ? c.bScale[col] : 0.f;
+      const uint32_t at = tmem + buf * 256 + ((uint32_t)quarter << 21);
+      uint32_t* room = (uint32_t*)c.parts + ((int64_t)blockIdx.x * 2 + (b == b0 ? 0 : 1)) * NP * A.nc * 128 + quarter * 32 + lane;
+#pragma unroll 1
+      for (int r = 0; r < rows; r += 16) {
+        uint32_t v[NP * 16];
+#pragma unroll
+        for (int p = 0; p < NP; p++) gm_tmem16(at + p * A.nc + r, v + 16 * p);
+        gm_loaded(v);
+        if (none) {
+#pragma unroll
+          for (int i = 0; i < NP * 16; i++) v[i] = 0;
+        }
+        if (col < c.N) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            if (r + i >= rows) break;
+            if (mine) {
+              gm_finish<KIND, O>(c, which, m0 + r + i, col, v[i], v[16 * (NP - 1) + i], sb);
+            } else {
+#pragma unroll
+              for (int p = 0; p < NP; p++) room[(p * A.nc + r + i) * 128] = v[16 * p + i];
+            }
+          }
+        }
+        __syncwarp();
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && !none) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(gm_smem(sumEmpty + buf)) : "memory");
+      buf ^= 1;
+      if (buf == 0) ph ^= 1;
+      b = end;
     }
   }
   if (!ok) atomicExch(&denseErr, 202);
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (split > 1) gm_cluster_sync();  // (the others may still read this one's sums)
-  if (warp == 5) {
+  if (warp == 2) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Tiles that several CTAs share: their sums, added up in the order of the depth, and the epilogue. A CTA per tile and row, a thread per column.
+template <int KIND, class O>
+__global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmArgs A) {
+  constexpr bool I8 = KIND == GK_Q8;
+  constexpr int NP = KIND == GK_GATE ? 2 : 1;
+  const GemmCall& c = A.c;
+  const int nk = A.kBlocks * (KIND == GK_SUM ? 2 : 1);
+  const int64_t t = blockIdx.x, n = (int64_t)A.tilesM * A.tilesN * nk;
+  int which, n0;
+  int64_t m0;
+  gf_tile<KIND>(A, t, which, n0, m0);
+  // the CTAs that hold the tile's first and last stage: start(i) <= stage < start(i + 1)
+  auto holder = [&](int64_t b) { return (int)(((b + 1) * A.ctas - 1) / n); };
+  const int first = holder(t * nk), last = holder(t * nk + nk - 1);
+  gm_after_previous();
+  if (first == last) return;
+  const int64_t col = n0 + threadIdx.x;
+  if (col >= c.N) return;
+  const float sb = I8 ? c.bScale[col] : 0.f;
+  for (int r = blockIdx.y; r < A.nc && m0 + r < c.M; r += gridDim.y) {
+    float f[2] = {};
+    uint32_t u = 0;
+    for (int q = first; q <= last; q++) {
+      const int second = gf_start(q, A.ctas, n, nk, false) < t * nk;
+      const uint32_t* room = (const uint32_t*)c.parts + ((int64_t)q * 2 + second) * NP * A.nc * 128 + threadIdx.x;
+      if (I8) u += room[r * 128];
+      else
+#pragma unroll
+        for (int p = 0; p < NP; p++) f[p] += __uint_as_float(room[(p * A.nc + r) * 128]);
+    }
+    gm_finish<KIND, O>(c, which, m0 + r, col, I8 ? u : __float_as_uint(f[0]), __float_as_uint(f[NP - 1]), sb);
   }
 }
 
@@ -612,40 +695,43 @@ static int64_t operand_map(CUtensorMap& map, const GemmOperand& o, int type, int
   return r == CUDA_SUCCESS ? CLA_OK : fail(CLA_ERR_CUDA, "dense product: tensor map refused (" + std::to_string((int)r) + ")");
 }
 
-// Shared memory of a CTA in proportion to its columns of tensor memory, so that an SM never holds CTAs of more columns than it has: CTAs that
-// wait for columns while their cluster waits for them could otherwise hold up one another, of any launches.
-constexpr int GM_SM_SMEM = 228 * 1024, GM_CTA_SMEM = 1024;  // an SM's, and what it keeps for each CTA
+// All of an SM's shared memory for a CTA, as it takes all of its tensor memory: CTAs that wait for tensor memory while others wait for
+// them could hold up one another
 template <class K>
-static int64_t smem_for(OncePerDevice& once, int* room, int device, int cols, K kernel, int& least) {
-  const int64_t rc = once(device, [&]() -> int64_t {
+static int64_t all_smem(OncePerDevice& once, int* room, int device, K kernel) {
+  return once(device, [&]() -> int64_t {
     cudaFuncAttributes a;
     CLA_CUDA(cudaFuncGetAttributes(&a, kernel));
-    const int most = GM_SM_SMEM - GM_CTA_SMEM - (int)a.sharedSizeBytes;
+    const int most = 227 * 1024 - (int)a.sharedSizeBytes;  // of a CTA; 1 KB more is kept for it
     CLA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     *room = most;
     return CLA_OK;
   });
-  least = GM_SM_SMEM / 512 * cols - (GM_SM_SMEM - *room);
-  return rc;
 }
 
-// Which kernel and tile: the one that a count of clocks makes the fastest.
+// Which kernel and tile: the one that a count of clocks makes the fastest. For 148 SMs: the workspace does not depend on the device.
 struct GemmPlan {
   bool large = false;
   int wide = 0;                      // k_gemm_pair
-  int nc = 0, split = 1, stages = 1; // k_gemm_few
+  int nc = 0, ctas = 0, stages = 1;  // k_gemm_few
+  bool whole = true;
   double clocks = 1e30;
 };
-static GemmPlan gemm_plan(const GemmCall& c, int nk, int sms) {
+constexpr int GM_SMS = 148;
+static int gemm_blocks(const GemmCall& c) {  // stages of a segment
+  const int depth = 128 / type_bytes(c.type);
+  return (int)((c.K + depth - 1) / depth);
+}
+static GemmPlan gemm_plan(const GemmCall& c) {
   GemmPlan best;
+  const int nk = gemm_blocks(c) * (c.kind == GK_SUM ? 2 : 1);
   const int np = c.kind == GK_GATE ? 2 : 1, products = c.kind == GK_PAIR ? 2 : 1;
   const auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  const double L2 = 40;  // bytes a clock that an SM gets
   for (int wide = 256 / np; wide >= 64 && nk > 0; wide /= 2) {
     const int mine = np == 2 ? wide : wide / 2;
     if (c.b[0].mn && mine < 64) break;
-    const int64_t tiles = ceil_div(c.M, 256) * ceil_div(c.N, wide) * products, turns = ceil_div(tiles, sms / 2);
-    const double step = std::max(2.0 * mine * 2, (GM_OPERAND + mine * 128) / L2 / 1.5), t = 5000 + turns * (nk * step + 600);
+    const int64_t tiles = ceil_div(c.M, 256) * ceil_div(c.N, wide) * products, turns = ceil_div(tiles, GM_SMS / 2);
+    const double step = std::max(4.0 * mine, (GM_OPERAND + mine * 128) / 60.0), t = 5000 + turns * (nk * step + 600);
     if (t < best.clocks) best.large = true, best.wide = wide, best.clocks = t;
   }
   for (int nc = 16; nc <= 128; nc *= 2) {
@@ -654,36 +740,33 @@ static GemmPlan gemm_plan(const GemmCall& c, int nk, int sms) {
     if (nc > least && nc / 2 >= c.M) break;
     const int stage = np * (int)GM_OPERAND + nc * 128;
     const int64_t tiles = ceil_div(c.M, nc) * ceil_div(c.N, 128) * products;
-    for (int split = 1; split <= 8 && split <= std::max(1, nk); split++) {
-      const int perSm = 2 * stage <= 111 * 1024 && (split == 1 || np * nc * 512 <= 111 * 1024) ? 2 : 1;
-      const int64_t ctas = tiles * split, slots = (int64_t)sms * perSm, turns = ceil_div(ctas, slots);
-      const double together = std::min<double>(perSm, (double)ceil_div(ctas, sms));
-      const double step = together * std::max(2.0 * nc * np, stage / L2), t = 4000 + (split > 1 ? 1500 + nc * np * 4 : 0) + turns * (ceil_div(nk, split) * step + 2000 + nc * 20);
-      if (t < best.clocks) {
-        best.large = false, best.nc = nc, best.split = split, best.clocks = t;
-        best.stages = (int)std::max<int64_t>(1, std::min<int64_t>({16, (ctas > sms && perSm == 2 ? 111 : 220) * 1024 / stage, ceil_div(nk, split)}));
-      }
+    const double step = std::max(2.0 * nc * np, stage / 40.0), out = 1000 + nc * np * 20;
+    for (int whole = 1; whole >= (c.split && nk > 0 ? 0 : 1); whole--) {
+      const int64_t ctas = whole ? std::min<int64_t>(tiles, GM_SMS) : std::min<int64_t>(GM_SMS, tiles * ceil_div(nk, 4));
+      const double t = whole ? 4000 + ceil_div(tiles, ctas) * std::max(nk * step, out) + out : 9000 + (double)ceil_div(tiles * nk, ctas) * step + out;
+      if (t >= best.clocks) continue;
+      best.large = false, best.nc = nc, best.ctas = (int)ctas, best.whole = whole, best.clocks = t;
+      best.stages = (int)std::min<int64_t>(GF_STAGES, GF_RING / stage);
     }
   }
   return best;
+}
+int64_t gemm_workspace(const GemmCall& c) {
+  if (c.M == 0 || c.N == 0) return 0;
+  const GemmPlan p = gemm_plan(c);
+  return p.large || p.whole ? 0 : (int64_t)p.ctas * 2 * (c.kind == GK_GATE ? 2 : 1) * p.nc * 128 * 4;
 }
 
 template <int KIND, class O>
 static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   const GemmCall& c = A.c;
-  const int bytes = type_bytes(c.type), segs = KIND == GK_SUM ? 2 : 1;
-  int sms = 148;
-  CLA_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device));
-  A.depth = 128 / bytes;
-  A.kBlocks = (int)((c.K + A.depth - 1) / A.depth);
-  const int nk = A.kBlocks * segs;
-  const GemmPlan p = gemm_plan(c, nk, sms);
+  A.depth = 128 / type_bytes(c.type);
+  A.kBlocks = gemm_blocks(c);
+  const GemmPlan p = gemm_plan(c);
   // both operands' types, where their index is contiguous, sums in 32 bits
   const uint32_t type = c.type == CLA_T_BF16 || c.type == CLA_T_I8 ? 1u : 0u;
   const uint32_t base = (KIND == GK_Q8 ? 2u : 1u) << 4 | type << 7 | type << 10;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = s;
-  if (nk > 0)
+  if (A.kBlocks > 0)
     for (int i = 0; i < 2; i++) {
       const int boxB = !p.large ? 128 : KIND == GK_GATE ? p.wide : p.wide / 2;
       if (i == 0 || KIND == GK_SUM)
@@ -694,36 +777,47 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   const int np = KIND == GK_GATE ? 2 : 1, products = KIND == GK_PAIR ? 2 : 1;
   static OncePerDevice oncePair, onceFew;
   static int roomPair, roomFew;
-  int smem;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = s;
   if (p.large) {
     A.wide = p.wide;
     A.tilesM = (int)((c.M + 255) / 256);
     A.tilesN = (int)((c.N + p.wide - 1) / p.wide) * products;
     A.idesc = base | (uint32_t)c.a[0].mn << 15 | (uint32_t)c.b[0].mn << 16 | (uint32_t)(p.wide * np >> 3) << 17 | (256u >> 4) << 24;
-    if (const int64_t e = smem_for(oncePair, &roomPair, c.device, 512, k_gemm_pair<KIND, O>, smem); e < 0) return e;
-    static_assert(GP_STAGES * GP_STAGE + 1024 + 8 * 4096 <= GM_SM_SMEM - GM_CTA_SMEM - 1024, "the ring and the warps' rooms fit");
-    cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, sms / 2);
+    if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
+    static_assert(GP_STAGES * GP_STAGE + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
+    cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
     cfg.blockDim = GP_T;
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = roomPair;
     CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
   }
   A.nc = p.nc;
   A.stages = p.stages;
+  A.ctas = p.ctas;
+  A.whole = p.whole;
+  A.early = c.aLate;
   A.tilesM = (int)((c.M + A.nc - 1) / A.nc);
   A.tilesN = (int)((c.N + 127) / 128) * products;
   A.idesc = base | (uint32_t)c.b[0].mn << 15 | (uint32_t)c.a[0].mn << 16 | (uint32_t)(A.nc >> 3) << 17 | (128u >> 4) << 24;
-  if (const int64_t e = smem_for(onceFew, &roomFew, c.device, std::max(32, np * A.nc), k_gemm_few<KIND, O>, smem); e < 0) return e;
-  smem = std::max(smem, std::max(A.stages * (np * (int)GM_OPERAND + A.nc * 128), p.split > 1 ? np * A.nc * 512 : 0) + 1024);
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)p.split, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cfg.gridDim = (unsigned)((int64_t)A.tilesM * A.tilesN * p.split);
+  if (const int64_t e = all_smem(onceFew, &roomFew, c.device, k_gemm_few<KIND, O>); e < 0) return e;
+  static_assert(GF_RING + 1024 <= 226 * 1024, "the ring fits");
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = c.aLate ? 1 : 0;
+  cfg.gridDim = p.ctas;
   cfg.blockDim = GF_T;
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = roomFew;
   CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_few<KIND, O>, A));
+  if (!p.whole) {
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)A.tilesM * A.tilesN, (unsigned)std::min<int64_t>(c.M, A.nc));
+    cfg.blockDim = 128;
+    cfg.dynamicSmemBytes = 0;
+    CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_join<KIND, O>, A));
+  }
   return CLA_OK;
 }
 
