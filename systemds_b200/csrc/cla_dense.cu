@@ -383,8 +383,9 @@ template <class F> void with_type(int type, F&& f) {
 }
 
 int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t cols, bool byCols, int8_t* q, int64_t ldq, float* scale,
-                 cudaStream_t s) {
+                 int device, cudaStream_t s) {
   if ((byCols ? cols : rows) == 0) return CLA_OK;
+  int64_t rc = CLA_OK;
   with_type(type, [&](auto t) {
     using T = decltype(t);
     if (byCols) {
@@ -392,6 +393,12 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
       return;
     }
     constexpr int V = DN_V<T>, C = sizeof(T) == 8 ? 8 : 4;
+    static OncePerDevice once;
+    rc = once(device, [] {
+      const int64_t e = like_products(k_quantize_rows<T, 32, C>);
+      return e < 0 ? e : like_products(k_quantize_rows<T, DN_T, C>);
+    });
+    if (rc < 0) return;
     const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
     // a warp per row, without a barrier, where it holds the row and there are rows enough
     if (cols <= 32 * C * V && rows >= 148)
@@ -399,6 +406,7 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
     else
       k_quantize_rows<T, DN_T, C><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale, vec);
   });
+  if (rc < 0) return rc;
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;
 }
@@ -467,7 +475,7 @@ int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s, bool split = 
     const int64_t ld = round_up(c.K, 16);
     int8_t* q = (int8_t*)w.take(c.M * ld);
     float* sc = (float*)w.take(c.M * 4);
-    if (run) DN_CHECK(quantize(c.aType, c.a, c.lda, c.M, c.K, false, q, ld, sc, s));
+    if (run) DN_CHECK(quantize(c.aType, c.a, c.lda, c.M, c.K, false, q, ld, sc, c.device, s));
     g.a[0] = {q, ld, false};
     g.aScale = sc;
     g.aLate = c.K > 0;  // (the last kernel before the product)
@@ -641,7 +649,7 @@ int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t ro
   if (rows > 1 << 30 || cols > 1 << 30) return fail(CLA_ERR_UNSUPPORTED, "quantize: more than 2^30 rows or columns");
   OnDevice on(device);
   if (on.rc < 0) return on.rc;
-  return quantize(type, x, ldx, rows, cols, byCols, q, ldq, scale, (cudaStream_t)stream);
+  return quantize(type, x, ldx, rows, cols, byCols, q, ldq, scale, device, (cudaStream_t)stream);
 }
 
 int64_t cla_q8_workspace(const cla_q8* c) {

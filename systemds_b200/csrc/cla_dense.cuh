@@ -9,6 +9,12 @@ namespace cla {
 inline int type_bytes(int type) {
   return type == CLA_T_F64 ? 8 : type == CLA_T_F32 ? 4 : type == CLA_T_I8 ? 1 : 2;
 }
+// Kernels that run just before or after a product, with the split of an SM's memory that the product has: no SM is emptied to change it
+template <class K>
+int64_t like_products(K kernel) {
+  CLA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  return CLA_OK;
+}
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 template <class T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }

@@ -125,7 +125,8 @@ struct alignas(64) GemmArgs {
   int kBlocks;           // stages of a segment
   int tilesM, tilesN;    // PAIR: tilesN of both products
   int wide;              // k_gemm_pair: columns of a tile (GATE: of each product)
-  int nc, stages;        // k_gemm_few: rows of a tile, stages of the ring,
+  int stages;            // of the ring
+  int nc;                // k_gemm_few: rows of a tile,
   int ctas, whole;       // CTAs, and whether each has whole tiles
   int early;             // whether the weights need not wait for the kernel before
   uint32_t idesc;
@@ -200,7 +201,7 @@ __device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa,
 // brings 128 rows and 128 columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight take the sums out of one half of
 // tensor memory while the other fills. A launch's pairs take tiles in turn, along the rows within groups of GP_GROUP row tiles, so that what
 // runs at once shares operands in L2.
-constexpr int GP_T = 384, GP_STAGES = 6, GP_STAGE = 2 * GM_OPERAND, GP_GROUP = 8;
+constexpr int GP_T = 384, GP_STAGES = 10, GP_RING = 6 * 2 * GM_OPERAND, GP_GROUP = 8;
 
 __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& tn) {
   const int per = GP_GROUP * A.tilesN, g = t / per, first = g * GP_GROUP, n = min(GP_GROUP, A.tilesM - first), r = t - g * per;
@@ -220,7 +221,8 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
   const int pairs = gridDim.x / 2, pair = blockIdx.x / 2, tiles = A.tilesM * A.tilesN;
   const int segments = KIND == GK_SUM ? 2 : 1, nk = A.kBlocks * segments;
   const bool aMn = !I8 && c.a[0].mn, bMn = !I8 && c.b[0].mn;
-  const int mine = KIND == GK_GATE ? A.wide : A.wide / 2;  // columns that a CTA brings
+  const int mine = KIND == GK_GATE ? A.wide : A.wide / 2, stages = A.stages;  // columns that a CTA brings
+  const uint32_t stage = GM_OPERAND + mine * 128;
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -258,8 +260,8 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
           ok = gm_wait(gm_smem(empty + s), ph);
           if (!ok) break;
           const int seg = KIND == GK_SUM && kb >= A.kBlocks, k0 = (kb - seg * A.kBlocks) * A.depth;
-          const uint32_t bar = gm_peer(gm_smem(full + s), 0), da = smem + s * GP_STAGE, db = da + GM_OPERAND;
-          if (rank == 0) gm_expect(gm_smem(full + s), 2 * (GM_OPERAND + mine * 128));
+          const uint32_t bar = gm_peer(gm_smem(full + s), 0), da = smem + s * stage, db = da + GM_OPERAND;
+          if (rank == 0) gm_expect(gm_smem(full + s), 2 * stage);
           const CUtensorMap *ma = A.a + seg, *mb = A.b + (KIND == GK_SUM ? seg : which);
           if (aMn) {
             gm_load<true>(da, ma, m0, k0, bar);
@@ -273,12 +275,12 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
             gm_load<true>(db, mb, k0, n0, bar);
           }
           issued++;
-          if (++s == GP_STAGES) s = 0, ph ^= 1;
+          if (++s == stages) s = 0, ph ^= 1;
         }
       }
       // what is still on its way, here and to the other CTA's barriers
-      for (int i = 0; i < GP_STAGES; i++) {
-        const int64_t n = (issued - i + GP_STAGES - 1) / GP_STAGES;  // times stage i was filled
+      for (int i = 0; i < stages; i++) {
+        const int64_t n = (issued - i + stages - 1) / stages;  // times stage i was filled
         if (n <= 0) break;
         if (!ok && rank == 0) gm_wait(gm_smem(full + i), (uint32_t)(n - 1) & 1u);
         if (ok && !gm_wait(gm_smem(empty + i), (uint32_t)(n - 1) & 1u)) ok = false;
@@ -298,11 +300,11 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
           ok = gm_wait(gm_smem(full + s), ph);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          uint64_t a = gm_desc(smem + s * GP_STAGE, aMn), b = gm_desc(smem + s * GP_STAGE + GM_OPERAND, bMn);
+          uint64_t a = gm_desc(smem + s * stage, aMn), b = gm_desc(smem + s * stage + GM_OPERAND, bMn);
 #pragma unroll
           for (int i = 0; i < 4; i++, a += gm_step(aMn), b += gm_step(bMn)) gm_mma<true, I8>(tmem + buf * 256, a, b, A.idesc, kb > 0 || i > 0);
           gm_commit<true>(gm_smem(empty + s));
-          if (++s == GP_STAGES) s = 0, ph ^= 1;
+          if (++s == stages) s = 0, ph ^= 1;
         }
         if (ok) gm_commit<true>(gm_smem(sumFull + buf));
       }
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
       gp_tile(A, t, tm, tn);
       const int64_t m0 = (int64_t)tm * 256 + rank * 128 + quarter * 32, m = m0 + lane;
       const int rows = (int)max((int64_t)0, min((int64_t)32, c.M - m0)), width = A.wide / 2;
-      const uint32_t at = tmem + buf * 256 + half * width + ((uint32_t)quarter << 21), room = smem + GP_STAGES * GP_STAGE + (warp - 4) * 4096;
+      const uint32_t at = tmem + buf * 256 + half * width + ((uint32_t)quarter << 21), room = smem + GP_RING + (warp - 4) * 4096;
       auto aligned = [&](int o) { return ((uintptr_t)c.out[o] | (uintptr_t)(c.ldo[o] * sizeof(O))) % 16 == 0; };
       if constexpr (KIND == GK_GATE) {
         const int64_t n0 = (int64_t)tn * A.wide + half * width;
@@ -399,8 +401,8 @@ __device__ __forceinline__ void gm_after_previous() { asm volatile("griddepcontr
 __device__ __forceinline__ void gm_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // The first stage of CTA i's range; `whole`: of tiles. (of n stages in tiles of nk)
-__host__ __device__ inline int64_t gf_start(int64_t i, int ctas, int64_t n, int nk, bool whole) {
-  return whole ? n / nk * i / ctas * nk : n * i / ctas;
+__host__ __device__ inline int gf_start(int i, int ctas, int n, int nk, bool whole) {
+  return whole ? (int)((int64_t)(n / nk) * i / ctas) * nk : (int)((int64_t)n * i / ctas);
 }
 
 template <int KIND, class O>
@@ -423,9 +425,9 @@ __device__ __forceinline__ void gm_finish(const GemmCall& c, int which, int64_t 
 
 // Tile t: its product (PAIR), first column and first row. Tiles of the same columns lie next to each other: their CTAs share the weights in L2.
 template <int KIND>
-__device__ __forceinline__ void gf_tile(const GemmArgs& A, int64_t t, int& which, int& n0, int64_t& m0) {
-  int tn = (int)(t / A.tilesM);
-  m0 = (t - (int64_t)tn * A.tilesM) * A.nc;
+__device__ __forceinline__ void gf_tile(const GemmArgs& A, int t, int& which, int& n0, int64_t& m0) {
+  const int tn = t / A.tilesM;
+  m0 = (int64_t)(t - tn * A.tilesM) * A.nc;
   which = KIND == GK_PAIR && tn >= A.tilesN / 2;
   n0 = (which ? tn - A.tilesN / 2 : tn) * 128;
 }
@@ -442,8 +444,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
   const uint32_t smem = (gm_smem(gmsm) + 1023u) & ~1023u;
   const int nk = max(1, A.kBlocks * (KIND == GK_SUM ? 2 : 1));  // (a depth of zero: one stage that nothing is added from)
   const bool none = A.kBlocks == 0;
-  const int64_t n = (int64_t)A.tilesM * A.tilesN * nk;
-  const int64_t b0 = gf_start(blockIdx.x, gridDim.x, n, nk, A.whole), b1 = gf_start(blockIdx.x + 1, gridDim.x, n, nk, A.whole);
+  const int n = A.tilesM * A.tilesN * nk, b0 = gf_start(blockIdx.x, gridDim.x, n, nk, A.whole), b1 = gf_start(blockIdx.x + 1, gridDim.x, n, nk, A.whole);
   const bool cMn = !I8 && c.a[0].mn, lMn = !I8 && c.b[0].mn;  // the result's rows and columns
   const uint32_t stage = NP * GM_OPERAND + A.nc * 128;
   if (!A.whole) gm_let_next();
@@ -470,59 +471,71 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
   bool ok = true;
   if (warp == 0) {
     if (!none && gm_elect()) {
-      auto at = [&](int64_t b, int& which, int& n0, int64_t& m0, int& seg, int& k0) {
-        const int64_t t = b / nk;
-        const int kb = (int)(b - t * nk);
-        gf_tile<KIND>(A, t, which, n0, m0);
-        seg = KIND == GK_SUM && kb >= A.kBlocks;
-        k0 = (kb - seg * A.kBlocks) * A.depth;
-      };
-      auto columns = [&](int64_t b, int s) {
-        int which, n0, seg, k0;
+      // the place of a stage in the tiles, kept from one to the next
+      struct Place {
+        int t, kb, which, n0;
         int64_t m0;
-        at(b, which, n0, m0, seg, k0);
+      };
+      auto place = [&](int b) {
+        Place p;
+        p.t = b / nk;
+        p.kb = b - p.t * nk;
+        gf_tile<KIND>(A, p.t, p.which, p.n0, p.m0);
+        return p;
+      };
+      auto next = [&](Place& p) {
+        if (++p.kb == nk) {
+          p.kb = 0;
+          gf_tile<KIND>(A, ++p.t, p.which, p.n0, p.m0);
+        }
+      };
+      auto columns = [&](const Place& q, int s) {
+        const int seg = KIND == GK_SUM && q.kb >= A.kBlocks, k0 = (q.kb - seg * A.kBlocks) * A.depth;
         const uint32_t bar = gm_smem(full + s), dl = smem + s * stage;
         gm_expect(bar, stage);
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-          const CUtensorMap* ml = A.b + (KIND == GK_GATE ? p : KIND == GK_SUM ? seg : which);
+          const CUtensorMap* ml = A.b + (KIND == GK_GATE ? p : KIND == GK_SUM ? seg : q.which);
           if (lMn) {
-            gm_load<false>(dl + p * GM_OPERAND, ml, n0, k0, bar);
-            gm_load<false>(dl + p * GM_OPERAND + 8192, ml, n0 + 64, k0, bar);
+            gm_load<false>(dl + p * GM_OPERAND, ml, q.n0, k0, bar);
+            gm_load<false>(dl + p * GM_OPERAND + 8192, ml, q.n0 + 64, k0, bar);
           } else {
-            gm_load<false>(dl + p * GM_OPERAND, ml, k0, n0, bar);
+            gm_load<false>(dl + p * GM_OPERAND, ml, k0, q.n0, bar);
           }
         }
       };
-      auto rows = [&](int64_t b, int s) {
-        int which, n0, seg, k0;
-        int64_t m0;
-        at(b, which, n0, m0, seg, k0);
+      auto rows = [&](const Place& q, int s) {
+        const int seg = KIND == GK_SUM && q.kb >= A.kBlocks, k0 = (q.kb - seg * A.kBlocks) * A.depth;
         const uint32_t bar = gm_smem(full + s), dc = smem + s * stage + NP * GM_OPERAND;
         if (cMn) {
-          for (int i = 0; i < A.nc; i += 64) gm_load<false>(dc + i * 128, A.a + seg, (int)m0 + i, k0, bar);
+          for (int i = 0; i < A.nc; i += 64) gm_load<false>(dc + i * 128, A.a + seg, (int)q.m0 + i, k0, bar);
         } else {
-          gm_load<false>(dc, A.a + seg, k0, (int)m0, bar);
+          gm_load<false>(dc, A.a + seg, k0, (int)q.m0, bar);
         }
       };
-      const int64_t ahead = A.early ? min((int64_t)A.stages, b1 - b0) : 0;  // stages whose weights do not wait for the kernel before
-      for (int64_t i = 0; i < ahead; i++) columns(b0 + i, (int)i);
+      const int ahead = A.early ? min(A.stages, b1 - b0) : 0;  // stages whose weights do not wait for the kernel before
+      Place q = place(b0);
+      for (int i = 0; i < ahead; i++) {
+        columns(q, i);
+        next(q);
+      }
       gm_after_previous();
-      int s = 0;
-      int64_t issued = 0;
+      q = place(b0);
+      int s = 0, issued = 0;
       uint32_t ph = 1;
-      for (int64_t b = b0; b < b1; b++) {
+      for (int b = b0; b < b1; b++) {
         if (issued >= ahead) {
           ok = gm_wait(gm_smem(empty + s), ph);
           if (!ok) break;
-          columns(b, s);
+          columns(q, s);
         }
-        rows(b, s);
+        rows(q, s);
+        next(q);
         issued++;
         if (++s == A.stages) s = 0, ph ^= 1;
       }
       for (int i = 0; i < A.stages; i++) {
-        const int64_t times = (issued - i + A.stages - 1) / A.stages;  // that stage i was filled
+        const int times = (issued - i + A.stages - 1) / A.stages;  // that stage i was filled
         if (times <= 0) break;
         if (!ok) gm_wait(gm_smem(full + i), (uint32_t)(times - 1) & 1u);
         else if (!gm_wait(gm_smem(empty + i), (uint32_t)(times - 1) & 1u)) ok = false;
@@ -532,8 +545,8 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
     if (!none && gm_elect()) {
       int s = 0, buf = 0;
       uint32_t ph = 0, phSum = 1;
-      for (int64_t b = b0; b < b1 && ok;) {
-        const int64_t end = min(b1, (b / nk + 1) * nk);  // of this tile's part of the range
+      for (int b = b0; b < b1 && ok;) {
+        const int end = min(b1, (b / nk + 1) * nk);  // of this tile's part of the range
         ok = gm_wait(gm_smem(sumEmpty + buf), phSum);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -567,8 +580,8 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
     const int quarter = warp - 4;
     int buf = 0;
     uint32_t ph = 0;
-    for (int64_t b = b0; b < b1;) {
-      const int64_t t = b / nk, end = min(b1, (t + 1) * nk);
+    for (int b = b0; b < b1;) {
+      const int t = b / nk, end = min(b1, (t + 1) * nk);
       const bool mine = b == t * nk && end == (t + 1) * nk;
       int which, n0;
       int64_t m0;
@@ -632,12 +645,12 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
   constexpr int NP = KIND == GK_GATE ? 2 : 1;
   const GemmCall& c = A.c;
   const int nk = A.kBlocks * (KIND == GK_SUM ? 2 : 1);
-  const int64_t t = blockIdx.x, n = (int64_t)A.tilesM * A.tilesN * nk;
+  const int t = blockIdx.x, n = A.tilesM * A.tilesN * nk;
   int which, n0;
   int64_t m0;
   gf_tile<KIND>(A, t, which, n0, m0);
   // the CTAs that hold the tile's first and last stage: start(i) <= stage < start(i + 1)
-  auto holder = [&](int64_t b) { return (int)(((b + 1) * A.ctas - 1) / n); };
+  auto holder = [&](int b) { return (int)(((int64_t)(b + 1) * A.ctas - 1) / n); };
   const int first = holder(t * nk), last = holder(t * nk + nk - 1);
   gm_after_previous();
   if (first == last) return;
@@ -740,6 +753,7 @@ static GemmPlan gemm_plan(const GemmCall& c) {
     if (nc > least && nc / 2 >= c.M) break;
     const int stage = np * (int)GM_OPERAND + nc * 128;
     const int64_t tiles = ceil_div(c.M, nc) * ceil_div(c.N, 128) * products;
+    if (tiles * std::max(1, nk) > INT32_MAX / 2) continue;  // (counted in 32 bits)
     const double step = std::max(2.0 * nc * np, stage / 40.0), out = 1000 + nc * np * 20;
     for (int whole = 1; whole >= (c.split && nk > 0 ? 0 : 1); whole--) {
       const int64_t ctas = whole ? std::min<int64_t>(tiles, GM_SMS) : std::min<int64_t>(GM_SMS, tiles * ceil_div(nk, 4));
@@ -781,11 +795,12 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   cfg.stream = s;
   if (p.large) {
     A.wide = p.wide;
+    A.stages = std::min(GP_STAGES, GP_RING / ((int)GM_OPERAND + (KIND == GK_GATE ? p.wide : p.wide / 2) * 128));
     A.tilesM = (int)((c.M + 255) / 256);
     A.tilesN = (int)((c.N + p.wide - 1) / p.wide) * products;
     A.idesc = base | (uint32_t)c.a[0].mn << 15 | (uint32_t)c.b[0].mn << 16 | (uint32_t)(p.wide * np >> 3) << 17 | (256u >> 4) << 24;
     if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
-    static_assert(GP_STAGES * GP_STAGE + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
+    static_assert(GP_RING + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
     cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
     cfg.blockDim = GP_T;
     cfg.dynamicSmemBytes = roomPair;
@@ -809,9 +824,11 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   cfg.numAttrs = c.aLate ? 1 : 0;
   cfg.gridDim = p.ctas;
   cfg.blockDim = GF_T;
-  cfg.dynamicSmemBytes = roomFew;
+  cfg.dynamicSmemBytes = GF_RING + 1024;  // (all but 5 KB: CTAs of k_gemm_join may wait next to it, none with tensor memory)
   CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_few<KIND, O>, A));
   if (!p.whole) {
+    static OncePerDevice onceJoin;
+    if (const int64_t e = onceJoin(c.device, [] { return like_products(k_gemm_join<KIND, O>); }); e < 0) return e;
     cfg.numAttrs = 1;
     cfg.gridDim = dim3((unsigned)A.tilesM * A.tilesN, (unsigned)std::min<int64_t>(c.M, A.nc));
     cfg.blockDim = 128;
