@@ -37,56 +37,94 @@ inline bool rows_aligned(const void* p, int64_t ld, int64_t rows, int bytes, int
 }
 
 // Which pieces of a matrix a thread takes: 2^log adjacent threads along a row, the others of the block down the rows, U rows at a time so
-// that U loads are on their way before the first is used. f(r, c, n): rows r, r + step, .. (n of them), piece c of each.
+// that U loads are on their way before the first is used. columns(c): what a thread keeps for piece c of its rows; f(kept, r, step, n): rows
+// r, r + step, .. (n of them).
 struct Walk {
   int log;         // threads along a row
   int64_t rows;
   int per;         // pieces of a row
 };
-template <int U, class F>
-__device__ __forceinline__ void walk(const Walk& w, F&& f) {
-  const int tx = threadIdx.x & ((1 << w.log) - 1), down = DN_T >> w.log;
-  const int64_t step = (int64_t)gridDim.y * down;
-  for (int c = blockIdx.x * (1 << w.log) + tx; c < w.per; c += gridDim.x << w.log)
-    for (int64_t r = (int64_t)blockIdx.y * down + (threadIdx.x >> w.log); r < w.rows; r += U * step)
-      f(r, c, step, (int)min((int64_t)U, (w.rows - r + step - 1) / step));
+__device__ __forceinline__ int64_t walk_first(const Walk& w) { return (int64_t)blockIdx.y * (DN_T >> w.log) + (threadIdx.x >> w.log); }
+__device__ __forceinline__ int64_t walk_step(const Walk& w) { return (int64_t)gridDim.y * (DN_T >> w.log); }
+template <int U, class C, class F>
+__device__ __forceinline__ void walk(const Walk& w, C&& columns, F&& f) {
+  const int tx = threadIdx.x & ((1 << w.log) - 1);
+  const int64_t step = walk_step(w);
+  for (int c = blockIdx.x * (1 << w.log) + tx; c < w.per; c += gridDim.x << w.log) {
+    auto kept = columns(c);
+    for (int64_t r = walk_first(w); r < w.rows; r += U * step)
+      f(kept, r, step, (int)min((int64_t)U, (w.rows - r + step - 1) / step));
+  }
+}
+template <int N> struct DropPieces {  // of 4 N columns
+  DropColumns c[N];
+};
+template <int N>
+__device__ __forceinline__ DropPieces<N> drop_pieces(const DropDev& d, int64_t c) {
+  if constexpr (N == 1) return {{DropColumns(d, (uint32_t)(c / 4))}};
+  else return {{DropColumns(d, (uint32_t)(c / 4)), DropColumns(d, (uint32_t)(c / 4) + 1)}};
 }
 
 // ---- dropout --------------------------------------------------------------------------------------------------------
-// Pieces of 16 bytes (F64: 32, the four columns of a counter). Bound: the words (twenty 64-bit products and as many three-way logic
+// Pieces of 16 bytes (F64: 32, the four columns of a counter). Bound: the words (sixteen 64-bit products and as many three-way logic
 // operations for four columns) next to memory.
-template <class T, int U>
-__global__ void __launch_bounds__(DN_T) k_dropout(const T* x, int64_t ldx, int64_t cols, T* y, int64_t ldy, const __grid_constant__ DropDev d,
-                                                  const __grid_constant__ Walk w, int vec) {
-  constexpr int P = DN_V<T>, V = P < 4 ? 4 : P;
-  walk<U>(w, [&](int64_t r, int piece, int64_t step, int n) {
-    const int64_t c = (int64_t)piece * V;
-    alignas(16) T v[U][V];
-    const int left = (int)min((int64_t)V, cols - c);
+template <class T>
+__global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, int64_t cols, T* y, int64_t ldy, const __grid_constant__ DropDev d,
+                                                     const __grid_constant__ Walk w, int vec) {
+  constexpr int P = DN_V<T>, V = P < 4 ? 4 : P, N = V / 4;
+  struct Kept {
+    const T* x;
+    T* y;
+    int64_t stepX, stepY;
+    int left;
+    DropPieces<N> drop;
+    alignas(16) T next[V];  // the next row's values: on their way while a row's are worked on
+  };
+  auto load = [&](Kept& k) {
 #pragma unroll
-    for (int u = 0; u < U; u++)
-      if (u < n)
+    for (int h = 0; h < V; h += P) load_vec(k.x + h, k.left - h, vec, (T(&)[P])k.next[h]);
+  };
+  const int64_t r0 = walk_first(w), step = walk_step(w);
+  walk<1>(
+      w,
+      [&](int piece) {
+        const int64_t c = (int64_t)piece * V;
+        Kept k{x + r0 * ldx + c, y + r0 * ldy + c, step * ldx, step * ldy, (int)min((int64_t)V, cols - c), drop_pieces<N>(d, c), {}};
+        if (r0 < w.rows) load(k);
+        return k;
+      },
+      [&](Kept& k, int64_t r, int64_t, int) {
+        alignas(16) T v[V];
 #pragma unroll
-        for (int h = 0; h < V; h += P) load_vec(x + (r + u * step) * ldx + c + h, left - h, vec && left - h >= P, (T(&)[P])v[u][h]);
+        for (int i = 0; i < V; i++) v[i] = k.next[i];
+        k.x += k.stepX;
+        if (r + step < w.rows) load(k);
+        if (d.on) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (u >= n) break;
-      if (d.on) {
+          for (int q = 0; q < V; q += 4) {
+            const uint4 words = k.drop.c[q / 4].words(d, (uint32_t)r);
+            if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int q = 0; q < V; q += 4) {
-          const uint4 words = drop_words(d, (uint32_t)(r + u * step), (uint32_t)((c + q) / 4));
+              for (int j = 0; j < 4; j += 2) {
+                uint32_t& w = *(uint32_t*)(v + q + j);
+                float a, b;
+                from_word<T>(w, a, b);
+                a *= d.scale, b *= d.scale;
+                w = to_word<T>(word_of(words, j) >= d.cut ? a : 0.f, word_of(words, j + 1) >= d.cut ? b : 0.f);
+              }
+            } else {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const bool keep = word_of(words, j) >= d.cut;
-            if constexpr (sizeof(T) == 8) v[u][q + j] = keep ? v[u][q + j] * d.scale64 : 0.0;
-            else v[u][q + j] = from_f32<T>(keep ? to_f32(v[u][q + j]) * d.scale : 0.f);
+              for (int j = 0; j < 4; j++) {
+                if constexpr (sizeof(T) == 8) v[q + j] = word_of(words, j) >= d.cut ? v[q + j] * d.scale64 : 0.0;
+                else v[q + j] = word_of(words, j) >= d.cut ? v[q + j] * d.scale : 0.f;
+              }
+            }
           }
         }
-      }
 #pragma unroll
-      for (int h = 0; h < V; h += P) store_vec(y + (r + u * step) * ldy + c + h, left - h, vec && left - h >= P, (const T(&)[P])v[u][h]);
-    }
-  });
+        for (int h = 0; h < V; h += P) store_vec(k.y + h, k.left - h, vec, (const T(&)[P])v[h]);
+        k.y += k.stepY;
+      });
 }
 
 // ---- quantisation -----------------------------------------------------------------------------------------------------
@@ -100,54 +138,60 @@ __device__ __forceinline__ unsigned long long magnitude(double v) { return (unsi
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ float q8_scale(unsigned long long most) { return (float)(__longlong_as_double((long long)most) / 127.0); }
 __device__ __forceinline__ float q8_scale(uint32_t most) { return __uint_as_float(most) / 127.f; }
-__device__ __forceinline__ int whole(double v) { return __double2int_rn(v); }
-__device__ __forceinline__ int whole(float v) { return __float2int_rn(v); }
-// The nearest whole number of x / scale. The product with the reciprocal is off by three roundings of a value below 128: unless it comes that
-// near to a half, where the quotient itself decides, both have the same nearest whole number.
+// The nearest whole number of x / scale, as the low byte of the result. The product with the reciprocal is off by three roundings of a value
+// below 128: unless it comes that near to a half, where the quotient itself decides, both have the same nearest whole number. So the product
+// is taken first, rounded by adding 1.5 times the power of two whose unit is 1, and whether some value came near is asked once
+// for many of them: the quotients are then taken for all.
 template <class W> struct Q8Row {
   W scale, inv;
-  bool some;
-  __device__ __forceinline__ explicit Q8Row(float s) : scale((W)s), inv((W)1 / (W)s), some(s > 0.f && s < INFINITY) {}
-  __device__ __forceinline__ int operator()(W x) const {
-    constexpr W FAR = (W)0.5 - (sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-14);  // 2^7 times 2^-50, 2^-21
-    const W t = x * inv;
-    int q = whole(t);
-    if (!(fabs(t - (W)q) <= FAR)) q = whole(x / scale);  // (also where the reciprocal is not finite)
-    return some ? min(127, max(-127, q)) : 0;
+  bool some, quick;  // a scale to divide by; whose reciprocal is finite
+  __device__ __forceinline__ explicit Q8Row(float s)
+      : scale((W)s), inv((W)1 / (W)s), some(s > 0.f && s < INFINITY), quick(s >= 0x1p-126f && s < INFINITY) {}
+  __device__ __forceinline__ uint32_t product(W x, bool& near) const {
+    constexpr W MAGIC = sizeof(W) == 8 ? (W)0x1.8p52 : (W)0x1.8p23;
+    constexpr W FAR = (W)0.5 - (sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-15);  // above 3/2 of 127 roundings of 2^-52, 2^-23
+    const W t = x * inv, r = t + MAGIC;
+    near |= !(fabs(t - (r - MAGIC)) <= FAR);
+    if constexpr (sizeof(W) == 8) return (uint32_t)__double2loint(r);
+    else return __float_as_uint(r);
   }
 };
+template <class W> __device__ __noinline__ uint32_t q8_quotient(W x, W scale, bool some) {
+  return some ? (uint32_t)(int)fmin((W)127, fmax((W)-127, rint(x / scale))) : 0u;
+}
 
 // G threads per row, which they keep in registers: its largest magnitude, then its quotients. One pass over x; rows longer than G * C pieces are
-// read a second time. Where rows do not start on 16-byte boundaries the threads take single values in turn. Bound: memory.
-template <class T, int G, int C>
-__global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int8_t* __restrict__ q,
-                                                        int64_t ldq, float* __restrict__ scale, int vec) {
+// read a second time. VEC: rows start on 16-byte boundaries, a piece is 16 bytes; else the threads take single values in turn. Bound: memory.
+template <class T, int G, int C, bool VEC>
+__global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int8_t* __restrict__ q,
+                                                        int64_t ldq, float* __restrict__ scale) {
   using W = typename WideOf<T>::type;
   using Bits = decltype(magnitude(W()));
-  constexpr int V = DN_V<T>;
+  constexpr int V = DN_V<T>, ROUND = G * V * C;
   __shared__ Bits part[DN_T / 32];
   const int lane = threadIdx.x % G, warp = threadIdx.x / 32;
   const int64_t r = (int64_t)blockIdx.x * (DN_T / G) + threadIdx.x / G;
   if (G == 32 && r >= rows) return;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the product's weights may come meanwhile)
-  const T* p = x + r * ldx;
+  const T* p = x + r * ldx + (VEC ? lane * V : lane);
+  int8_t* to = q + r * ldq + (VEC ? lane * V : lane);
   alignas(16) T v[C][V];
+  // value i of piece k of a round is at k * G * V + (VEC ? i : i * G) from p; how many from p on are there: left
   auto load = [&](int first) {
+    const int left = cols - first - (VEC ? lane * V : lane);
 #pragma unroll
     for (int k = 0; k < C; k++) {
-      const int at = first + k * G * V, c = at + lane * V;
-      if (vec && c + V <= cols) {
-        *(uint4*)v[k] = *(const uint4*)(p + c);
+      if (VEC && left >= k * G * V + V) {
+        *(uint4*)v[k] = *(const uint4*)(p + first + k * G * V);
       } else {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          const int e = vec ? c + i : at + i * G + lane;
-          v[k][i] = e < cols ? p[e] : from_f32<T>(0.f);
+          const int at = k * G * V + (VEC ? i : i * G);
+          v[k][i] = at < left ? p[first + at] : from_f32<T>(0.f);
         }
       }
     }
   };
-  constexpr int ROUND = G * V * C;
   Bits most = 0;
   for (int first = 0; first < cols; first += ROUND) {
     load(first);
@@ -168,26 +212,29 @@ __global__ void __launch_bounds__(DN_T) k_quantize_rows(const T* __restrict__ x,
   const float s = q8_scale(most);
   const Q8Row<W> q8(s);
   if (lane == 0) scale[r] = s;
-  int8_t* to = q + r * ldq;
   for (int first = 0; first < cols; first += ROUND) {
     if (cols > ROUND) load(first);
+    const int left = cols - first - (VEC ? lane * V : lane);
 #pragma unroll
     for (int j = 0; j < C; j++) {
-      const int at = first + j * G * V, c = at + lane * V;
-      if (at >= cols) break;
-      alignas(16) int8_t o[V];
+      if (first + j * G * V >= cols) break;
+      alignas(16) uint8_t o[V];
+      bool near = !q8.quick;
 #pragma unroll
-      for (int i = 0; i < V; i++) o[i] = (int8_t)q8(widen(v[j][i]));
-      if (vec && c + V <= cols) {
-        if constexpr (V == 8) *(uint2*)(to + c) = *(const uint2*)o;
-        else if constexpr (V == 4) *(uint32_t*)(to + c) = *(const uint32_t*)o;
-        else *(uint16_t*)(to + c) = *(const uint16_t*)o;
+      for (int i = 0; i < V; i++) o[i] = (uint8_t)q8.product(widen(v[j][i]), near);
+      if (near) {  // (calls, which are not made before it is known whether they are wanted)
+#pragma unroll
+        for (int i = 0; i < V; i++) o[i] = (uint8_t)q8_quotient(widen(v[j][i]), q8.scale, q8.some);
+      }
+      int8_t* t = to + first + j * G * V;
+      if (VEC && left >= j * G * V + V) {
+        if constexpr (V == 8) *(uint2*)t = *(const uint2*)o;
+        else if constexpr (V == 4) *(uint32_t*)t = *(const uint32_t*)o;
+        else *(uint16_t*)t = *(const uint16_t*)o;
       } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          const int e = vec ? c + i : at + i * G + lane;
-          if (e < cols) to[e] = o[i];
-        }
+        for (int i = 0; i < V; i++)
+          if (j * G * V + (VEC ? i : i * G) < left) t[VEC ? i : i * G] = (int8_t)o[i];
       }
     }
   }
@@ -220,7 +267,7 @@ __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x,
 #pragma unroll
     for (int i = 0; i < 128; i += 32) {
       const int64_t r = r0 + i + ty;
-      tile[tx][i + ty] = c < cols && r < rows ? (int8_t)q8(widen(x[r * ldx + c])) : 0;
+      tile[tx][i + ty] = c < cols && r < rows ? (int8_t)q8_quotient(widen(x[r * ldx + c]), q8.scale, q8.some) : 0;
     }
     __syncthreads();
     const int64_t oc = (int64_t)blockIdx.x * 32 + ty;
@@ -233,48 +280,66 @@ __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x,
 }
 
 // ---- the gated block's elementwise gradients ----------------------------------------------------------------------------
-template <class T, int U>
-__global__ void __launch_bounds__(DN_T) k_gate_grad(const T* __restrict__ dh, int64_t lddh, const T* __restrict__ g, int64_t ldg,
-                                                    const T* __restrict__ u, int64_t ldu, int64_t cols, T* __restrict__ dg, T* __restrict__ du,
-                                                    int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w, int vec) {
-  constexpr int V = DN_V<T>;
-  walk<U>(w, [&](int64_t r, int piece, int64_t step, int n) {
-    const int64_t c = (int64_t)piece * V;
-    const int left = (int)min((int64_t)V, cols - c);
-    alignas(16) T vh[U][V], vg[U][V], vu[U][V];
+// (the next row's values are on their way while a row's are worked on)
+template <class T>
+__global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh, int64_t lddh, const T* __restrict__ g, int64_t ldg,
+                                                       const T* __restrict__ u, int64_t ldu, int64_t cols, T* __restrict__ dg, T* __restrict__ du,
+                                                       int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w, int vec) {
+  constexpr int V = DN_V<T>, N = V / 4;
+  const int64_t r0 = walk_first(w), step = walk_step(w);
+  struct Values {
+    alignas(16) T h[V];
+    alignas(16) T g[V];
+    alignas(16) T u[V];
+  };
+  struct Kept {
+    int64_t c;
+    int left;
+    DropPieces<N> drop;
+    Values next;
+  };
+  auto load = [&](int64_t r, int64_t c, int left, Values& v) {
+    load_vec(dh + r * lddh + c, left, vec, v.h);
+    load_vec(g + r * ldg + c, left, vec, v.g);
+    load_vec(u + r * ldu + c, left, vec, v.u);
+  };
+  with_act(act, [&](auto name) {
+    walk<1>(
+        w,
+        [&](int piece) {
+          const int64_t c = (int64_t)piece * V;
+          Kept k{c, (int)min((int64_t)V, cols - c), drop_pieces<N>(d, c), {}};
+          if (r0 < w.rows) load(r0, c, k.left, k.next);
+          return k;
+        },
+        [&](Kept& k, int64_t r, int64_t, int) {
+          Values v = k.next;
+          if (r + step < w.rows) load(r + step, k.c, k.left, k.next);
 #pragma unroll
-    for (int k = 0; k < U; k++)
-      if (k < n) {
-        const int64_t at = r + k * step;
-        load_vec(dh + at * lddh + c, left, vec, vh[k]);
-        load_vec(g + at * ldg + c, left, vec, vg[k]);
-        load_vec(u + at * ldu + c, left, vec, vu[k]);
-      }
-    with_act(act, [&](auto name) {
+          for (int q = 0; q < V; q += 4) {
+            uint4 words;
+            if (d.on) words = k.drop.c[q / 4].words(d, (uint32_t)r);
 #pragma unroll
-      for (int k = 0; k < U; k++) {
-        if (k >= n) break;
+            for (int j = 0; j < 4; j += 2) {
+              float h[2], gate[2], up[2];
+              from_word<T>(*(const uint32_t*)(v.h + q + j), h[0], h[1]);
+              from_word<T>(*(const uint32_t*)(v.g + q + j), gate[0], gate[1]);
+              from_word<T>(*(const uint32_t*)(v.u + q + j), up[0], up[1]);
 #pragma unroll
-        for (int q = 0; q < V; q += 4) {
-          uint4 words;
-          if (d.on) words = drop_words(d, (uint32_t)(r + k * step), (uint32_t)((c + q) / 4));
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            float h = to_f32(vh[k][q + j]), a;
-            if (d.on) h = word_of(words, j) >= d.cut ? h * d.scale : 0.f;
-            const float slope = act_slope(decltype(name)::value, to_f32(vg[k][q + j]), a);
-            vg[k][q + j] = from_f32<T>(h * to_f32(vu[k][q + j]) * slope);
-            vu[k][q + j] = from_f32<T>(h * a);
+              for (int i = 0; i < 2; i++) {
+                float a;
+                if (d.on) h[i] = word_of(words, j + i) >= d.cut ? h[i] * d.scale : 0.f;
+                const float slope = act_slope(decltype(name)::value, gate[i], a);
+                gate[i] = h[i] * up[i] * slope;
+                up[i] = h[i] * a;
+              }
+              *(uint32_t*)(v.g + q + j) = to_word<T>(gate[0], gate[1]);
+              *(uint32_t*)(v.u + q + j) = to_word<T>(up[0], up[1]);
+            }
           }
-        }
-      }
-    });
-#pragma unroll
-    for (int k = 0; k < U; k++)
-      if (k < n) {
-        store_vec(dg + (r + k * step) * ldo + c, left, true, vg[k]);
-        store_vec(du + (r + k * step) * ldo + c, left, true, vu[k]);
-      }
+          store_vec(dg + r * ldo + k.c, k.left, true, v.g);
+          store_vec(du + r * ldo + k.c, k.left, true, v.u);
+        });
   });
 }
 
@@ -284,30 +349,33 @@ template <class T, int U>
 __global__ void __launch_bounds__(DN_T) k_repitch(const T* __restrict__ x, int64_t ldx, int64_t cols, T* __restrict__ y, int64_t ldy,
                                                   const __grid_constant__ Walk w) {
   constexpr int V = DN_V<T>;
-  walk<U>(w, [&](int64_t r, int piece, int64_t step, int n) {
-    const int64_t c = (int64_t)piece * V;
-    const int left = (int)min((int64_t)V, cols - c);
-    alignas(16) T v[U][V];
+  walk<U>(
+      w, [](int piece) { return (int64_t)piece * V; },
+      [&](int64_t c, int64_t r, int64_t step, int n) {
+        const int left = (int)min((int64_t)V, cols - c);
+        alignas(16) T v[U][V];
 #pragma unroll
-    for (int k = 0; k < U; k++)
-      if (k < n) load_vec(x + (r + k * step) * ldx + c, left, false, v[k]);
+        for (int k = 0; k < U; k++)
+          if (k < n) load_vec(x + (r + k * step) * ldx + c, left, false, v[k]);
 #pragma unroll
-    for (int k = 0; k < U; k++)
-      if (k < n) store_vec(y + (r + k * step) * ldy + c, left, true, v[k]);
-  });
+        for (int k = 0; k < U; k++)
+          if (k < n) store_vec(y + (r + k * step) * ldy + c, left, true, v[k]);
+      });
 }
 template <class T, int U>
 __global__ void __launch_bounds__(DN_T) k_narrow(const double* __restrict__ x, int64_t cols, T* __restrict__ y, int64_t ldy,
                                                  const __grid_constant__ Walk w) {
-  walk<U>(w, [&](int64_t r, int c, int64_t step, int n) {
-    double v[U];
+  walk<U>(
+      w, [](int piece) { return piece; },
+      [&](int c, int64_t r, int64_t step, int n) {
+        double v[U];
 #pragma unroll
-    for (int k = 0; k < U; k++)
-      if (k < n) v[k] = x[(r + k * step) * cols + c];
+        for (int k = 0; k < U; k++)
+          if (k < n) v[k] = x[(r + k * step) * cols + c];
 #pragma unroll
-    for (int k = 0; k < U; k++)
-      if (k < n) y[(r + k * step) * ldy + c] = from_f64<T>(v[k]);
-  });
+        for (int k = 0; k < U; k++)
+          if (k < n) y[(r + k * step) * ldy + c] = from_f64<T>(v[k]);
+      });
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -393,18 +461,19 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
       return;
     }
     constexpr int V = DN_V<T>, C = sizeof(T) == 8 ? 8 : 4;
-    static OncePerDevice once;
-    rc = once(device, [] {
-      const int64_t e = like_products(k_quantize_rows<T, 32, C>);
-      return e < 0 ? e : like_products(k_quantize_rows<T, DN_T, C>);
-    });
-    if (rc < 0) return;
-    const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
+    const bool vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
     // a warp per row, without a barrier, where it holds the row and there are rows enough
-    if (cols <= 32 * C * V && rows >= 148)
-      k_quantize_rows<T, 32, C><<<(unsigned)((rows + DN_T / 32 - 1) / (DN_T / 32)), DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale, vec);
-    else
-      k_quantize_rows<T, DN_T, C><<<(unsigned)rows, DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale, vec);
+    const bool warps = cols <= 32 * C * V && rows >= 148;
+    auto go = [&](auto kernel, OncePerDevice& once, unsigned grid) {
+      rc = once(device, [&] { return like_products(kernel); });
+      if (rc >= 0) kernel<<<grid, DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale);
+    };
+    const unsigned grid = (unsigned)(warps ? (rows + DN_T / 32 - 1) / (DN_T / 32) : rows);
+    static OncePerDevice once[4];
+    if (warps && vec) go(k_quantize_rows<T, 32, C, true>, once[0], grid);
+    else if (warps) go(k_quantize_rows<T, 32, C, false>, once[1], grid);
+    else if (vec) go(k_quantize_rows<T, DN_T, C, true>, once[2], grid);
+    else go(k_quantize_rows<T, DN_T, C, false>, once[3], grid);
   });
   if (rc < 0) return rc;
   CLA_CUDA(cudaGetLastError());
@@ -543,7 +612,7 @@ int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
     const dim3 grid = walk_grid(k, c.M, ld / 8, 1);
     auto go = [&](auto t) {
       using T = decltype(t);
-      k_gate_grad<T, 1><<<grid, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld, d, c.act, k,
+      k_gate_grad<T><<<grid, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld, d, c.act, k,
                                               vec);
     };
     if (c.type == CLA_T_BF16) go(__nv_bfloat16());
@@ -633,7 +702,7 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
     const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(y, ldy, rows, sizeof(T));
     Walk w;
     const dim3 grid = walk_grid(w, rows, (cols + V - 1) / V, 1);
-    k_dropout<T, 1><<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w, vec);
+    k_dropout<T><<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w, vec);
   });
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "cla_common.cuh"
 
 namespace cla {
@@ -28,6 +29,27 @@ template <class T> __device__ __forceinline__ T from_f64(double v) { return (T)v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f64(double v) { return __double2bfloat16(v); }
 template <> __device__ __forceinline__ __half from_f64(double v) { return __double2half(v); }
 
+// Two 16-bit values of a word, and back. (The lower bfloat16 by a byte permutation: the compiler's choice is a product, of which the words
+// of dropout leave the pipe few.)
+template <class T> __device__ __forceinline__ void from_word(uint32_t w, float& a, float& b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const float2 f = __half22float2(*(const __half2*)&w);
+    a = f.x, b = f.y;
+  } else {
+    a = __uint_as_float(__byte_perm(w, 0, 0x1044));
+    b = __uint_as_float(w & 0xffff0000u);
+  }
+}
+template <class T> __device__ __forceinline__ uint32_t to_word(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&h;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&h;
+  }
+}
+
 // ---- dropout --------------------------------------------------------------------------------------------------------
 struct DropDev {
   uint32_t cut = 0;  // kept where word >= cut
@@ -50,6 +72,34 @@ __device__ __forceinline__ uint4 drop_words(const DropDev& d, uint32_t row, uint
   }
   return make_uint4(x0, x1, x2, x3);
 }
+// The same for many rows of four columns. Of the twenty products four depend on the columns alone: those of the first round, and one each
+// of the second and third (a counter's words reach one another a round apart).
+struct DropColumns {
+  uint32_t first, second, third, hi, lo;  // what the rounds' words are xored with, and the third round's known product
+  __device__ __forceinline__ DropColumns(const DropDev& d, uint32_t c) {
+    const uint64_t a1 = (uint64_t)0xD2511F53u * c, b1 = (uint64_t)0xCD9E8D57u * d.step[0];
+    const uint64_t b2 = (uint64_t)0xCD9E8D57u * ((uint32_t)(a1 >> 32) ^ d.step[1] ^ d.key[1]);
+    const uint64_t a3 = (uint64_t)0xD2511F53u * ((uint32_t)(b2 >> 32) ^ (uint32_t)b1 ^ d.key[2]);
+    first = (uint32_t)(b1 >> 32) ^ d.key[0];
+    second = (uint32_t)a1 ^ d.key[3];
+    third = (uint32_t)b2 ^ d.key[4];
+    hi = (uint32_t)(a3 >> 32) ^ d.key[5];
+    lo = (uint32_t)a3;
+  }
+  __device__ __forceinline__ uint4 words(const DropDev& d, uint32_t row) const {
+    const uint64_t a2 = (uint64_t)0xD2511F53u * (first ^ (d.row0 + row)), b3 = (uint64_t)0xCD9E8D57u * ((uint32_t)(a2 >> 32) ^ second);
+    uint32_t x0 = (uint32_t)(b3 >> 32) ^ third, x1 = (uint32_t)b3, x2 = hi ^ (uint32_t)a2, x3 = lo;
+#pragma unroll
+    for (int i = 3; i < 10; i++) {
+      const uint64_t a = (uint64_t)0xD2511F53u * x0, b = (uint64_t)0xCD9E8D57u * x2;
+      x0 = (uint32_t)(b >> 32) ^ x1 ^ d.key[2 * i];
+      x1 = (uint32_t)b;
+      x2 = (uint32_t)(a >> 32) ^ x3 ^ d.key[2 * i + 1];
+      x3 = (uint32_t)a;
+    }
+    return make_uint4(x0, x1, x2, x3);
+  }
+};
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 
 // ---- the activation, in FP32 ------------------------------------------------------------------------------------------
