@@ -271,7 +271,7 @@ int64_t cla_group_counts(cla_handle h, int32_t g, int64_t* counts);
 /* ---- dense operators beside the compressed products ---------------------------------------------
  * What follows a compressed product in a model's training and scoring: the hidden layer of a gated feed-forward block with its
  * gradients, dropout, and products in 8-bit integers. They have no counterpart in the reference. Matrices are device memory in rows
- * of `ld` elements (ld >= the row's length; rows need no alignment), types CLA_T_*; sums are 32 bits or wider. Calls enqueue
+ * of `ld` elements (ld >= the row's length; rows need no alignment), of at most 2^30 rows and columns, types CLA_T_*; sums are 32 bits or wider. Calls enqueue
  * on `stream` of `device` and return CLA_OK without waiting or allocating; the current device stays what it was. Calls share nothing:
  * any number may run at once on any streams, captured or not, as long as their buffers differ. `work` is the caller's, 256-byte aligned,
  * of the size that the *_workspace function gives for the same arguments (0: none needed, work may be NULL); a call uses it until its
@@ -305,8 +305,7 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
 /* Quantises rows (byCols 0) or columns (1) of x [rows x cols] (F64, F32, BF16, F16): scale[i] = fl32(largest magnitude / 127), q = x / scale[i]
  * to the nearest whole number (even on ties, within -127..127; the division in FP64 for F64, else FP32). Where scale[i] is 0 or not finite q
  * is 0: a row of zeros gives zeros, one with an infinity or a NaN gives NaN in the product. byCols 0: q [rows x cols];
- * byCols 1: q [cols x rows], a row per column of x, as cla_q8_mm_dev takes weights. ldq: elements between the rows of q. At most 2^30 rows
- * and columns. */
+ * byCols 1: q [cols x rows], a row per column of x, as cla_q8_mm_dev takes weights. ldq: elements between the rows of q. */
 int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t byCols, int8_t* q, int64_t ldq,
                             float* scale, int32_t device, void* stream);
 

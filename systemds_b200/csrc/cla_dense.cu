@@ -215,26 +215,36 @@ __global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__
   for (int first = 0; first < cols; first += ROUND) {
     if (cols > ROUND) load(first);
     const int left = cols - first - (VEC ? lane * V : lane);
+    // how many pieces are asked about together: FP64 values hardly ever come near, the others' in one of a hundred pieces of a warp
+    constexpr int ASK = sizeof(T) == 8 ? C : 1;
 #pragma unroll
-    for (int j = 0; j < C; j++) {
-      if (first + j * G * V >= cols) break;
-      alignas(16) uint8_t o[V];
+    for (int j0 = 0; j0 < C; j0 += ASK) {
+      if (first + j0 * G * V >= cols) break;
+      alignas(16) uint8_t o[ASK][V];
       bool near = !q8.quick;
 #pragma unroll
-      for (int i = 0; i < V; i++) o[i] = (uint8_t)q8.product(widen(v[j][i]), near);
+      for (int j = 0; j < ASK; j++)
+#pragma unroll
+        for (int i = 0; i < V; i++) o[j][i] = (uint8_t)q8.product(widen(v[j0 + j][i]), near);
       if (near) {  // (calls, which are not made before it is known whether they are wanted)
 #pragma unroll
-        for (int i = 0; i < V; i++) o[i] = (uint8_t)q8_quotient(widen(v[j][i]), q8.scale, q8.some);
-      }
-      int8_t* t = to + first + j * G * V;
-      if (VEC && left >= j * G * V + V) {
-        if constexpr (V == 8) *(uint2*)t = *(const uint2*)o;
-        else if constexpr (V == 4) *(uint32_t*)t = *(const uint32_t*)o;
-        else *(uint16_t*)t = *(const uint16_t*)o;
-      } else {
+        for (int j = 0; j < ASK; j++)
 #pragma unroll
-        for (int i = 0; i < V; i++)
-          if (j * G * V + (VEC ? i : i * G) < left) t[VEC ? i : i * G] = (int8_t)o[i];
+          for (int i = 0; i < V; i++) o[j][i] = (uint8_t)q8_quotient(widen(v[j0 + j][i]), q8.scale, q8.some);
+      }
+#pragma unroll
+      for (int j = 0; j < ASK; j++) {
+        const int at = (j0 + j) * G * V;
+        int8_t* t = to + first + at;
+        if (VEC && left >= at + V) {
+          if constexpr (V == 8) *(uint2*)t = *(const uint2*)o[j];
+          else if constexpr (V == 4) *(uint32_t*)t = *(const uint32_t*)o[j];
+          else *(uint16_t*)t = *(const uint16_t*)o[j];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i++)
+            if (at + (VEC ? i : i * G) < left) t[VEC ? i : i * G] = (int8_t)o[j][i];
+        }
       }
     }
   }
@@ -412,7 +422,7 @@ dim3 walk_grid(Walk& w, int64_t rows, int64_t per, int at) {
 
 int64_t check_matrix(const char* what, const void* p, int64_t rows, int64_t cols, int64_t ld, int bytes) {
   if (rows < 0 || cols < 0) return fail(CLA_ERR_SHAPE, std::string(what) + ": negative size");
-  if (rows > INT32_MAX || cols > INT32_MAX) return fail(CLA_ERR_UNSUPPORTED, std::string(what) + ": more than 2^31 - 1 rows or columns");
+  if (rows > 1 << 30 || cols > 1 << 30) return fail(CLA_ERR_UNSUPPORTED, std::string(what) + ": more than 2^30 rows or columns");
   if (rows == 0 || cols == 0) return CLA_OK;
   if (!p) return fail(CLA_ERR_BAD_ARG, std::string(what) + ": null buffer");
   if (ld < cols) return fail(CLA_ERR_SHAPE, std::string(what) + ": rows overlap (ld below the row's length)");
@@ -715,7 +725,6 @@ int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t ro
   DN_CHECK(check_matrix("quantize, x", x, rows, cols, ldx, type_bytes(type)));
   DN_CHECK(check_matrix("quantize, q", q, byCols ? cols : rows, byCols ? rows : cols, ldq, 1));
   if ((byCols ? cols : rows) && !scale) return fail(CLA_ERR_BAD_ARG, "quantize: null scales");
-  if (rows > 1 << 30 || cols > 1 << 30) return fail(CLA_ERR_UNSUPPORTED, "quantize: more than 2^30 rows or columns");
   OnDevice on(device);
   if (on.rc < 0) return on.rc;
   return quantize(type, x, ldx, rows, cols, byCols, q, ldq, scale, device, (cudaStream_t)stream);

@@ -33,6 +33,11 @@ __device__ __forceinline__ uint32_t gm_rank() {
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
   return r;
 }
+// The warp's number, of which the compiler knows that all lanes have it: what depends on it alone then stays in the warp's own registers, where the
+// copies and products take their operands (a loop of one lane spent 600 clocks a stage on bringing them there; this one 300)
+__device__ __forceinline__ int gm_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+// A wait of the whole warp
+__device__ __forceinline__ bool gm_wait_all(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, gm_wait(bar, parity)); }
 __device__ __forceinline__ uint32_t gm_peer(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -107,6 +112,16 @@ __device__ __forceinline__ void gm_loaded(uint32_t (&v)[N]) {
   for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
 }
 
+// The end of a copying warp: every stage that it filled `issued` times in turn has been read (its own copies, and the products from it, are over). After a
+// wait that ran out, the copies alone, where this CTA's barriers tell of them.
+__device__ __forceinline__ void gm_drain(bool& ok, bool own, uint32_t fullAt, uint32_t emptyAt, int issued, int stages) {
+  for (int i = 0; i < stages && i < issued; i++) {
+    const uint32_t last = (uint32_t)((issued - i + stages - 1) / stages - 1) & 1u;
+    if (ok) ok = gm_wait_all(emptyAt + i * 8, last);
+    else if (own) gm_wait_all(fullAt + i * 8, last);
+  }
+}
+
 // ---- operands in shared memory ----------------------------------------------------------------------------------------
 // A stage is 128 bytes deep: 64 values of 16 bits, 128 of 8. Rows of 128 bytes, swizzled over 1024-byte groups of eight.
 // Depth contiguous (K-major): a row per index, groups of eight indexes 1024 bytes apart; the next 32 bytes of depth lie 32 bytes on.
@@ -135,56 +150,60 @@ struct alignas(64) GemmArgs {
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f32<O>(v); }
 
-// 32 rows (a lane each) of `width` columns to memory. f(j, o): columns j .. j + 15 of the lane's row, all lanes together. vec: the rows' pieces
-// start on 16-byte boundaries, and a lane writes its own; else they go through the warp's 4 KB of shared memory, 128 bytes of every row at
-// a time, and are written row by row, a word or its two halves a lane.
+// 32 rows (a lane each) of `width` columns to memory. f(j, o): columns j .. j + 15 of the lane's row, all lanes together. They go through the warp's
+// 4 KB of shared memory, 128 bytes of every row at a time, and from there in whole lines: four rows an instruction where rows start on
+// 16-byte boundaries (vec), else row by row, a word or its two halves a lane. Pieces of 16 bytes are swizzled over eight rows.
 template <class O, class F>
 __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t cols, int width, bool vec, uint32_t buf, F&& f) {
+  constexpr int LINE = 128 / (int)sizeof(O), PIECES = (int)sizeof(O);  // columns of 128 bytes; 16-byte pieces of 16 columns
   const int lane = threadIdx.x & 31;
-  if (vec) {
-    O* p = out + lane * ld;
 #pragma unroll 1
-    for (int j = 0; j < width; j += 16) {
-      alignas(16) O o[16];
-      f(j, o);
-      const int valid = lane < rows ? (int)min((int64_t)16, cols - j) : 0;
-      if (valid == 16) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 16 / (int)sizeof(O)) *(uint4*)(p + j + i) = *(const uint4*)(o + i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (i < valid) p[j + i] = o[i];
-      }
-      __syncwarp();
-    }
-    return;
-  }
-  constexpr int PIECE = 128 / (int)sizeof(O), WORDS = 16 * (int)sizeof(O) / 4;
+  for (int c0 = 0; c0 < width; c0 += LINE) {
+    const int some = min(LINE, width - c0);
 #pragma unroll 1
-  for (int c0 = 0; c0 < width; c0 += PIECE) {
-#pragma unroll 1
-    for (int j = 0; j < min(PIECE, width - c0); j += 16) {
+    for (int j = 0; j < some; j += 16) {
       alignas(16) O o[16];
       f(c0 + j, o);
-      const int w0 = j * (int)sizeof(O) / 4;
+      const int p0 = j * (int)sizeof(O) / 16;
 #pragma unroll
-      for (int i = 0; i < WORDS; i++)
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + (lane * 32 + ((w0 + i) ^ lane)) * 4), "r"(((const uint32_t*)o)[i]) : "memory");
+      for (int i = 0; i < PIECES; i++) {
+        const uint4 x = *(const uint4*)(o + i * (16 / PIECES));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + (((p0 + i) ^ (lane & 7)) * 16)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                     : "memory");
+      }
     }
     __syncwarp();
-    // the elements of word `lane`
-    const int64_t left = min((int64_t)min(PIECE, width - c0), cols - c0) * (int)sizeof(O) - 4 * lane;
-    for (int r = 0; r < rows; r++) {
-      uint32_t v;
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buf + (r * 32 + (lane ^ r)) * 4) : "memory");
-      char* p = (char*)(out + r * ld + c0) + 4 * lane;
-      if (sizeof(O) >= 4 || ((uintptr_t)p & 3) == 0) {
-        if (left >= 4) *(uint32_t*)p = v;
-        else if (left > 0) *(uint16_t*)p = (uint16_t)v;
-      } else {
-        if (left > 0) *(uint16_t*)p = (uint16_t)v;
-        if (left > 2) *(uint16_t*)(p + 2) = (uint16_t)(v >> 16);
+    const int64_t there = min((int64_t)some, cols - c0) * (int)sizeof(O);  // bytes of a row
+    if (vec) {
+      const int piece = lane & 7;
+      const int64_t left = there - piece * 16;
+#pragma unroll 2
+      for (int r = lane >> 3; r < rows; r += 4) {
+        uint4 x;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(buf + r * 128 + ((piece ^ (r & 7)) * 16)) : "memory");
+        char* p = (char*)(out + r * ld + c0) + piece * 16;
+        if (left >= 16) {
+          *(uint4*)p = x;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 / (int)sizeof(O); i++)
+            if ((i + 1) * (int)sizeof(O) <= left) ((O*)p)[i] = ((const O*)&x)[i];
+        }
+      }
+    } else {
+      const int64_t left = there - 4 * lane;
+#pragma unroll 2
+      for (int r = 0; r < rows; r++) {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4) : "memory");
+        char* p = (char*)(out + r * ld + c0) + 4 * lane;
+        if (sizeof(O) >= 4 || ((uintptr_t)p & 3) == 0) {
+          if (left >= 4) *(uint32_t*)p = v;
+          else if (left > 0) *(uint16_t*)p = (uint16_t)v;
+        } else {
+          if (left > 0) *(uint16_t*)p = (uint16_t)v;
+          if (left > 2) *(uint16_t*)(p + 2) = (uint16_t)(v >> 16);
+        }
       }
     }
     __syncwarp();
@@ -216,7 +235,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
   __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
   const GemmCall& c = A.c;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = gm_warp();
   const uint32_t rank = gm_rank(), smem = (gm_smem(gmsm) + 1023u) & ~1023u;
   const int pairs = gridDim.x / 2, pair = blockIdx.x / 2, tiles = A.tilesM * A.tilesN;
   const int segments = KIND == GK_SUM ? 2 : 1, nk = A.kBlocks * segments;
@@ -245,68 +264,70 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmemAt;
   bool ok = true;
+  const uint32_t fullAt = gm_smem(full), emptyAt = gm_smem(empty);
   if (warp == 0) {
-    if (gm_elect()) {
-      int s = 0;
-      uint32_t ph = 1;
-      int64_t issued = 0;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        int tm, tn;
-        gp_tile(A, t, tm, tn);
-        const int m0 = tm * 256 + rank * 128;
-        const int halfN = A.tilesN / 2, which = KIND == GK_GATE ? (int)rank : KIND == GK_PAIR && tn >= halfN;
-        const int n0 = KIND == GK_GATE ? tn * A.wide : (KIND == GK_PAIR && tn >= halfN ? tn - halfN : tn) * A.wide + rank * mine;
-        for (int kb = 0; kb < nk; kb++) {
-          ok = gm_wait(gm_smem(empty + s), ph);
+    const uint32_t barAt = gm_peer(fullAt, 0);  // the first CTA's
+    int s = 0, issued = 0;
+    uint32_t ph = 1;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      int tm, tn;
+      gp_tile(A, t, tm, tn);
+      const int m0 = tm * 256 + rank * 128;
+      const int halfN = A.tilesN / 2, which = KIND == GK_GATE ? (int)rank : KIND == GK_PAIR && tn >= halfN;
+      const int n0 = KIND == GK_GATE ? tn * A.wide : (KIND == GK_PAIR && tn >= halfN ? tn - halfN : tn) * A.wide + rank * mine;
+      for (int seg = 0; seg < segments && ok; seg++) {
+        const CUtensorMap *ma = A.a + seg, *mb = A.b + (KIND == GK_SUM ? seg : which);
+        for (int k0 = 0; k0 < A.kBlocks * A.depth; k0 += A.depth) {
+          ok = gm_wait_all(emptyAt + s * 8, ph);
           if (!ok) break;
-          const int seg = KIND == GK_SUM && kb >= A.kBlocks, k0 = (kb - seg * A.kBlocks) * A.depth;
-          const uint32_t bar = gm_peer(gm_smem(full + s), 0), da = smem + s * stage, db = da + GM_OPERAND;
-          if (rank == 0) gm_expect(gm_smem(full + s), 2 * stage);
-          const CUtensorMap *ma = A.a + seg, *mb = A.b + (KIND == GK_SUM ? seg : which);
-          if (aMn) {
-            gm_load<true>(da, ma, m0, k0, bar);
-            gm_load<true>(da + 8192, ma, m0 + 64, k0, bar);
-          } else {
-            gm_load<true>(da, ma, k0, m0, bar);
+          const uint32_t bar = barAt + s * 8, da = smem + s * stage, db = da + GM_OPERAND;
+          if (gm_elect()) {
+            if (rank == 0) gm_expect(fullAt + s * 8, 2 * stage);
+            if (aMn) {
+              gm_load<true>(da, ma, m0, k0, bar);
+              gm_load<true>(da + 8192, ma, m0 + 64, k0, bar);
+            } else {
+              gm_load<true>(da, ma, k0, m0, bar);
+            }
+            if (bMn) {
+              gm_load<true>(db, mb, n0, k0, bar);
+              if (mine > 64) gm_load<true>(db + 8192, mb, n0 + 64, k0, bar);
+            } else {
+              gm_load<true>(db, mb, k0, n0, bar);
+            }
           }
-          if (bMn) {
-            for (int i = 0; i < mine; i += 64) gm_load<true>(db + i * 128, mb, n0 + i, k0, bar);
-          } else {
-            gm_load<true>(db, mb, k0, n0, bar);
-          }
+          __syncwarp();
           issued++;
           if (++s == stages) s = 0, ph ^= 1;
         }
       }
-      // what is still on its way, here and to the other CTA's barriers
-      for (int i = 0; i < stages; i++) {
-        const int64_t n = (issued - i + stages - 1) / stages;  // times stage i was filled
-        if (n <= 0) break;
-        if (!ok && rank == 0) gm_wait(gm_smem(full + i), (uint32_t)(n - 1) & 1u);
-        if (ok && !gm_wait(gm_smem(empty + i), (uint32_t)(n - 1) & 1u)) ok = false;
-      }
     }
+    gm_drain(ok, rank == 0, fullAt, emptyAt, issued, stages);
   } else if (warp == 1) {
-    if (rank == 0 && gm_elect()) {
-      int s = 0;
+    if (rank == 0) {
+      const uint64_t a0 = gm_desc(smem, aMn), b0 = gm_desc(smem + GM_OPERAND, bMn);
+      const uint32_t da = gm_step(aMn), db = gm_step(bMn);
+      int s = 0, n = 0;
       uint32_t ph = 0;
-      int n = 0;
       for (int t = pair; t < tiles && ok; t += pairs, n++) {
         const int buf = n & 1;
-        ok = gm_wait(gm_smem(sumEmpty + buf), ((n >> 1) & 1) ^ 1);
+        ok = gm_wait_all(gm_smem(sumEmpty + buf), ((n >> 1) & 1) ^ 1);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         for (int kb = 0; kb < nk; kb++) {
-          ok = gm_wait(gm_smem(full + s), ph);
+          ok = gm_wait_all(fullAt + s * 8, ph);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          uint64_t a = gm_desc(smem + s * stage, aMn), b = gm_desc(smem + s * stage + GM_OPERAND, bMn);
+          const uint64_t a = a0 + (uint32_t)s * (stage >> 4), b = b0 + (uint32_t)s * (stage >> 4);
+          if (gm_elect()) {
 #pragma unroll
-          for (int i = 0; i < 4; i++, a += gm_step(aMn), b += gm_step(bMn)) gm_mma<true, I8>(tmem + buf * 256, a, b, A.idesc, kb > 0 || i > 0);
-          gm_commit<true>(gm_smem(empty + s));
+            for (int i = 0; i < 4; i++) gm_mma<true, I8>(tmem + buf * 256, a + i * da, b + i * db, A.idesc, kb > 0 || i > 0);
+            gm_commit<true>(emptyAt + s * 8);
+            if (kb == nk - 1) gm_commit<true>(gm_smem(sumFull + buf));
+          }
+          __syncwarp();
           if (++s == stages) s = 0, ph ^= 1;
         }
-        if (ok) gm_commit<true>(gm_smem(sumFull + buf));
       }
     }
   } else if (warp >= 4) {
@@ -440,7 +461,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
   __shared__ __align__(8) uint64_t full[GF_STAGES], empty[GF_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
   const GemmCall& c = A.c;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = gm_warp();
   const uint32_t smem = (gm_smem(gmsm) + 1023u) & ~1023u;
   const int nk = max(1, A.kBlocks * (KIND == GK_SUM ? 2 : 1));  // (a depth of zero: one stage that nothing is added from)
   const bool none = A.kBlocks == 0;
@@ -469,8 +490,9 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmemAt;
   bool ok = true;
+  const uint32_t fullAt = gm_smem(full), emptyAt = gm_smem(empty);
   if (warp == 0) {
-    if (!none && gm_elect()) {
+    if (!none) {
       // the place of a stage in the tiles, kept from one to the next
       struct Place {
         int t, kb, which, n0;
@@ -489,9 +511,10 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
           gf_tile<KIND>(A, ++p.t, p.which, p.n0, p.m0);
         }
       };
+      // one lane's
       auto columns = [&](const Place& q, int s) {
         const int seg = KIND == GK_SUM && q.kb >= A.kBlocks, k0 = (q.kb - seg * A.kBlocks) * A.depth;
-        const uint32_t bar = gm_smem(full + s), dl = smem + s * stage;
+        const uint32_t bar = fullAt + s * 8, dl = smem + s * stage;
         gm_expect(bar, stage);
 #pragma unroll
         for (int p = 0; p < NP; p++) {
@@ -506,9 +529,10 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       };
       auto rows = [&](const Place& q, int s) {
         const int seg = KIND == GK_SUM && q.kb >= A.kBlocks, k0 = (q.kb - seg * A.kBlocks) * A.depth;
-        const uint32_t bar = gm_smem(full + s), dc = smem + s * stage + NP * GM_OPERAND;
+        const uint32_t bar = fullAt + s * 8, dc = smem + s * stage + NP * GM_OPERAND;
         if (cMn) {
-          for (int i = 0; i < A.nc; i += 64) gm_load<false>(dc + i * 128, A.a + seg, (int)q.m0 + i, k0, bar);
+          gm_load<false>(dc, A.a + seg, (int)q.m0, k0, bar);
+          if (A.nc > 64) gm_load<false>(dc + 8192, A.a + seg, (int)q.m0 + 64, k0, bar);
         } else {
           gm_load<false>(dc, A.a + seg, k0, (int)q.m0, bar);
         }
@@ -516,7 +540,8 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       const int ahead = A.early ? min(A.stages, b1 - b0) : 0;  // stages whose weights do not wait for the kernel before
       Place q = place(b0);
       for (int i = 0; i < ahead; i++) {
-        columns(q, i);
+        if (gm_elect()) columns(q, i);
+        __syncwarp();
         next(q);
       }
       gm_after_previous();
@@ -524,53 +549,48 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       int s = 0, issued = 0;
       uint32_t ph = 1;
       for (int b = b0; b < b1; b++) {
-        if (issued >= ahead) {
-          ok = gm_wait(gm_smem(empty + s), ph);
-          if (!ok) break;
-          columns(q, s);
+        const bool fresh = issued >= ahead;
+        if (fresh) ok = gm_wait_all(emptyAt + s * 8, ph);
+        if (!ok) break;
+        if (gm_elect()) {
+          if (fresh) columns(q, s);
+          rows(q, s);
         }
-        rows(q, s);
+        __syncwarp();
         next(q);
         issued++;
         if (++s == A.stages) s = 0, ph ^= 1;
       }
-      for (int i = 0; i < A.stages; i++) {
-        const int times = (issued - i + A.stages - 1) / A.stages;  // that stage i was filled
-        if (times <= 0) break;
-        if (!ok) gm_wait(gm_smem(full + i), (uint32_t)(times - 1) & 1u);
-        else if (!gm_wait(gm_smem(empty + i), (uint32_t)(times - 1) & 1u)) ok = false;
-      }
+      gm_drain(ok, true, fullAt, emptyAt, issued, A.stages);
     }
   } else if (warp == 1) {
-    if (!none && gm_elect()) {
+    if (!none) {
+      const uint64_t d0 = gm_desc(smem + NP * GM_OPERAND, cMn), l0 = gm_desc(smem, lMn);
+      const uint32_t dd = gm_step(cMn), dl = gm_step(lMn);
       int s = 0, buf = 0;
       uint32_t ph = 0, phSum = 1;
       for (int b = b0; b < b1 && ok;) {
-        const int end = min(b1, (b / nk + 1) * nk);  // of this tile's part of the range
-        ok = gm_wait(gm_smem(sumEmpty + buf), phSum);
+        const int first = b, end = min(b1, (b / nk + 1) * nk);  // of this tile's part of the range
+        ok = gm_wait_all(gm_smem(sumEmpty + buf), phSum);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        bool add = false;
         for (; b < end; b++) {
-          ok = gm_wait(gm_smem(full + s), ph);
+          ok = gm_wait_all(fullAt + s * 8, ph);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t dl = smem + s * stage;
-          uint64_t d = gm_desc(dl + NP * GM_OPERAND, cMn);
-          uint64_t l[NP];
+          const uint64_t d = d0 + (uint32_t)s * (stage >> 4), l = l0 + (uint32_t)s * (stage >> 4);
+          if (gm_elect()) {
 #pragma unroll
-          for (int p = 0; p < NP; p++) l[p] = gm_desc(dl + p * GM_OPERAND, lMn);
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-          for (int i = 0; i < 4; i++, d += gm_step(cMn), add = true)
-#pragma unroll
-            for (int p = 0; p < NP; p++) {
-              gm_mma<false, I8>(tmem + buf * 256 + p * A.nc, l[p], d, A.idesc, add);
-              l[p] += gm_step(lMn);
-            }
-          gm_commit<false>(gm_smem(empty + s));
+              for (int p = 0; p < NP; p++)
+                gm_mma<false, I8>(tmem + buf * 256 + p * A.nc, l + (p * GM_OPERAND >> 4) + i * dl, d + i * dd, A.idesc, b > first || i > 0);
+            gm_commit<false>(emptyAt + s * 8);
+            if (b == end - 1) gm_commit<false>(gm_smem(sumFull + buf));
+          }
+          __syncwarp();
           if (++s == A.stages) s = 0, ph ^= 1;
         }
-        if (ok) gm_commit<false>(gm_smem(sumFull + buf));
         buf ^= 1;
         if (buf == 0) phSum ^= 1;
       }
@@ -657,16 +677,21 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
   const int64_t col = n0 + threadIdx.x;
   if (col >= c.N) return;
   const float sb = I8 ? c.bScale[col] : 0.f;
+  // the first CTA's range starts in this tile or before it, the others' in it
+  const int64_t room = (int64_t)NP * A.nc * 128;
+  const int64_t head = (int64_t)first * 2 + (gf_start(first, A.ctas, n, nk, false) < t * nk);
   for (int r = blockIdx.y; r < A.nc && m0 + r < c.M; r += gridDim.y) {
-    float f[2] = {};
-    uint32_t u = 0;
-    for (int q = first; q <= last; q++) {
-      const int second = gf_start(q, A.ctas, n, nk, false) < t * nk;
-      const uint32_t* room = (const uint32_t*)c.parts + ((int64_t)q * 2 + second) * NP * A.nc * 128 + threadIdx.x;
-      if (I8) u += room[r * 128];
+    const uint32_t* at = (const uint32_t*)c.parts + r * 128 + threadIdx.x;
+    uint32_t u = at[head * room];
+    float f[2];
+#pragma unroll
+    for (int p = 0; p < NP; p++) f[p] = __uint_as_float(at[head * room + p * A.nc * 128]);
+#pragma unroll 8
+    for (int q = first + 1; q <= last; q++) {
+      if (I8) u += at[q * 2 * room];
       else
 #pragma unroll
-        for (int p = 0; p < NP; p++) f[p] += __uint_as_float(room[(p * A.nc + r) * 128]);
+        for (int p = 0; p < NP; p++) f[p] += __uint_as_float(at[q * 2 * room + p * A.nc * 128]);
     }
     gm_finish<KIND, O>(c, which, m0 + r, col, I8 ? u : __float_as_uint(f[0]), __float_as_uint(f[NP - 1]), sb);
   }
@@ -722,13 +747,13 @@ static int64_t all_smem(OncePerDevice& once, int* room, int device, K kernel) {
   });
 }
 
-// Which kernel and tile: the one that a count of clocks makes the fastest. For 148 SMs: the workspace does not depend on the device.
+// Which kernel and tile: the one that an estimate in microseconds makes the fastest. For 148 SMs: the workspace does not depend on the device.
 struct GemmPlan {
   bool large = false;
   int wide = 0;                      // k_gemm_pair
   int nc = 0, ctas = 0, stages = 1;  // k_gemm_few
   bool whole = true;
-  double clocks = 1e30;
+  double us = 1e30;
 };
 constexpr int GM_SMS = 148;
 static int gemm_blocks(const GemmCall& c) {  // stages of a segment
@@ -740,26 +765,34 @@ static GemmPlan gemm_plan(const GemmCall& c) {
   const int nk = gemm_blocks(c) * (c.kind == GK_SUM ? 2 : 1);
   const int np = c.kind == GK_GATE ? 2 : 1, products = c.kind == GK_PAIR ? 2 : 1;
   const auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  for (int wide = 256 / np; wide >= 64 && nk > 0; wide /= 2) {
+  // The terms were measured over 1 to 2048 rows, 1000 to 16384 columns, depths of 500 to 5504, weights not in L2 (both sides of every
+  // choice; the choice was the fastest or within a tenth of it in nine of ten). What the operands take from memory at 6.2 GB a ms:
+  const double memory = (double)type_bytes(c.type) * c.K * (c.kind == GK_SUM ? 2 : 1) * (c.M + c.N * (c.kind == GK_Q8 ? 1 : 2)) / 6.2e6;
+  // k_gemm_pair: a stage takes 0.17 us (waits and issue) or its products' time, 4 clocks a column that a CTA brings, at 1.85 GHz
+  // (32 rows and fewer leave its copies of them nearly empty, which take up to twice the time: not for deep products of so few)
+  for (int wide = 256 / np; wide >= 64 && nk > 0 && (c.M > 32 || nk <= 8); wide /= 2) {
     const int mine = np == 2 ? wide : wide / 2;
     if (c.b[0].mn && mine < 64) break;
     const int64_t tiles = ceil_div(c.M, 256) * ceil_div(c.N, wide) * products, turns = ceil_div(tiles, GM_SMS / 2);
-    const double step = std::max(4.0 * mine, (GM_OPERAND + mine * 128) / 60.0), t = 5000 + turns * (nk * step + 600);
-    if (t < best.clocks) best.large = true, best.wide = wide, best.clocks = t;
+    const double t = 8.0 + std::max(memory, turns * (nk * std::max(0.17, 4 * mine / 1850.0) + 0.5));
+    if (t < best.us) best.large = true, best.wide = wide, best.us = t;
   }
+  // k_gemm_few: a stage takes 0.26 us (two products 0.32), more with more rows; all SMs' stages together come at 7 GB a ms, and a depth that is
+  // shared costs the second kernel
   for (int nc = 16; nc <= 128; nc *= 2) {
     const int least = c.a[0].mn ? 64 : 16;
     if (nc < least) continue;
     if (nc > least && nc / 2 >= c.M) break;
     const int stage = np * (int)GM_OPERAND + nc * 128;
-    const int64_t tiles = ceil_div(c.M, nc) * ceil_div(c.N, 128) * products;
-    if (tiles * std::max(1, nk) > INT32_MAX / 2) continue;  // (counted in 32 bits)
-    const double step = std::max(2.0 * nc * np, stage / 40.0), out = 1000 + nc * np * 20;
+    const int64_t tiles = ceil_div(c.M, nc) * ceil_div(c.N, 128) * products, n = tiles * std::max(1, nk);
+    if (n > INT32_MAX / 2) continue;  // (counted in 32 bits)
+    const double step = (np == 2 ? 0.32 : 0.26) + nc * np * 0.0012, out = 0.2 + std::min<int64_t>(nc, c.M) * np * 0.05;
     for (int whole = 1; whole >= (c.split && nk > 0 ? 0 : 1); whole--) {
       const int64_t ctas = whole ? std::min<int64_t>(tiles, GM_SMS) : std::min<int64_t>(GM_SMS, tiles * ceil_div(nk, 4));
-      const double t = whole ? 4000 + ceil_div(tiles, ctas) * std::max(nk * step, out) + out : 9000 + (double)ceil_div(tiles * nk, ctas) * step + out;
-      if (t >= best.clocks) continue;
-      best.large = false, best.nc = nc, best.ctas = (int)ctas, best.whole = whole, best.clocks = t;
+      const double chain = whole ? ceil_div(tiles, ctas) * std::max(nk * step, out) : ceil_div(n, ctas) * step;
+      const double t = 5.5 + std::max({memory, chain, n * stage / 7.0e6}) + out + (whole ? 0.0 : 3.0);
+      if (t >= best.us) continue;
+      best.large = false, best.nc = nc, best.ctas = (int)ctas, best.whole = whole, best.us = t;
       best.stages = (int)std::min<int64_t>(GF_STAGES, GF_RING / stage);
     }
   }
