@@ -105,6 +105,12 @@ __device__ __forceinline__ void gm_tmem16(uint32_t addr, uint32_t* v) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void gm_tmem8(uint32_t addr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(addr)
+               : "memory");
+}
 template <int N>
 __device__ __forceinline__ void gm_loaded(uint32_t (&v)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -150,37 +156,36 @@ struct alignas(64) GemmArgs {
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f32<O>(v); }
 
-// 32 rows (a lane each) of `width` columns to memory. f(j, o): columns j .. j + 15 of the lane's row, all lanes together. They go through the warp's
-// 4 KB of shared memory, 128 bytes of every row at a time, and from there in whole lines: four rows an instruction where rows start on
-// 16-byte boundaries (vec), else row by row, a word or its two halves a lane. Pieces of 16 bytes are swizzled over eight rows.
-template <class O, class F>
+// 32 rows (a lane each) of `width` columns to memory. f(j, o): columns j .. j + CH - 1 of the lane's row, all lanes together. They go through the
+// warp's shared memory, LINE bytes (128 or 64) of every row at a time, and from there in whole lines: pieces of 16 bytes where rows start
+// on 16-byte boundaries (vec), else a word a lane. The pieces are swizzled over the rows.
+template <class O, int CH, int LINE, class F>
 __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t cols, int width, bool vec, uint32_t buf, F&& f) {
-  constexpr int LINE = 128 / (int)sizeof(O), PIECES = (int)sizeof(O);  // columns of 128 bytes; 16-byte pieces of 16 columns
+  constexpr int COLS = LINE / (int)sizeof(O), PIECES = CH * (int)sizeof(O) / 16, PER = LINE / 16;  // columns; pieces of a chunk, of a line
   const int lane = threadIdx.x & 31;
+  const auto place = [&](int r, int piece) { return buf + r * LINE + (LINE == 128 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) * 16; };
 #pragma unroll 1
-  for (int c0 = 0; c0 < width; c0 += LINE) {
-    const int some = min(LINE, width - c0);
+  for (int c0 = 0; c0 < width; c0 += COLS) {
+    const int some = min(COLS, width - c0);
 #pragma unroll 1
-    for (int j = 0; j < some; j += 16) {
-      alignas(16) O o[16];
+    for (int j = 0; j < some; j += CH) {
+      alignas(16) O o[CH];
       f(c0 + j, o);
-      const int p0 = j * (int)sizeof(O) / 16;
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
-        const uint4 x = *(const uint4*)(o + i * (16 / PIECES));
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + (((p0 + i) ^ (lane & 7)) * 16)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
-                     : "memory");
+        const uint4 x = *(const uint4*)(o + i * (CH / PIECES));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, j * (int)sizeof(O) / 16 + i)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
       }
     }
     __syncwarp();
     const int64_t there = min((int64_t)some, cols - c0) * (int)sizeof(O);  // bytes of a row
     if (vec) {
-      const int piece = lane & 7;
+      const int piece = lane % PER;
       const int64_t left = there - piece * 16;
 #pragma unroll 2
-      for (int r = lane >> 3; r < rows; r += 4) {
+      for (int r = lane / PER; r < rows; r += 32 / PER) {
         uint4 x;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(buf + r * 128 + ((piece ^ (r & 7)) * 16)) : "memory");
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(place(r, piece)) : "memory");
         char* p = (char*)(out + r * ld + c0) + piece * 16;
         if (left >= 16) {
           *(uint4*)p = x;
@@ -191,18 +196,29 @@ __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t co
         }
       }
     } else {
-      const int64_t left = there - 4 * lane;
+      constexpr int WORDS = LINE / 4;
+      const int word = lane % WORDS;
+      const int64_t left = there - 4 * word;  // bytes from the lane's word on
 #pragma unroll 2
-      for (int r = 0; r < rows; r++) {
+      for (int r0 = 0; r0 < rows; r0 += 32 / WORDS) {
+        const int r = r0 + lane / WORDS;
         uint32_t v;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4) : "memory");
-        char* p = (char*)(out + r * ld + c0) + 4 * lane;
-        if (sizeof(O) >= 4 || ((uintptr_t)p & 3) == 0) {
-          if (left >= 4) *(uint32_t*)p = v;
-          else if (left > 0) *(uint16_t*)p = (uint16_t)v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(place(r, word / 4) + (word % 4) * 4) : "memory");
+        char* p = (char*)(out + r * ld + c0) + 4 * word;
+        if (sizeof(O) >= 4) {
+          if (left >= 4 && r < rows) *(uint32_t*)p = v;
         } else {
-          if (left > 0) *(uint16_t*)p = (uint16_t)v;
-          if (left > 2) *(uint16_t*)(p + 2) = (uint16_t)(v >> 16);
+          // a row that starts in the middle of a word: the words are the upper half of a lane's and the lower half of the next one's
+          const bool odd = (uintptr_t)p & 2;  // (of the whole row)
+          const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
+          if (r < rows) {
+            if (odd && word == 0 && left >= 2) *(uint16_t*)p = (uint16_t)v;
+            const int64_t mine = left - (odd ? 2 : 0);
+            const uint32_t w = odd ? __byte_perm(v, next, 0x5432) : v;
+            char* q = p + (odd ? 2 : 0);
+            if (mine >= 4 && !(odd && word == WORDS - 1)) *(uint32_t*)q = w;
+            else if (mine >= 2) *(uint16_t*)q = (uint16_t)w;
+          }
         }
       }
     }
@@ -220,7 +236,11 @@ __device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa,
 // brings 128 rows and 128 columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight take the sums out of one half of
 // tensor memory while the other fills. A launch's pairs take tiles in turn, along the rows within groups of GP_GROUP row tiles, so that what
 // runs at once shares operands in L2.
-constexpr int GP_T = 384, GP_STAGES = 10, GP_RING = 6 * 2 * GM_OPERAND, GP_GROUP = 8;
+constexpr int GP_STAGES = 10, GP_RING = 6 * 2 * GM_OPERAND, GP_GROUP = 8;
+
+// Warps that take the sums out. GATE: 16, for the activation and the dropout of a tile keep eight busy for twice as long as its products take at a
+// depth of 2048 (18 against 9 us: few instructions of a warp at a time are independent).
+__host__ __device__ constexpr int gp_out(int kind) { return kind == GK_GATE ? 16 : 8; }
 
 __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& tn) {
   const int per = GP_GROUP * A.tilesN, g = t / per, first = g * GP_GROUP, n = min(GP_GROUP, A.tilesM - first), r = t - g * per;
@@ -229,8 +249,9 @@ __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& 
 }
 
 template <int KIND, class O>
-__global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
+__global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
   constexpr bool I8 = KIND == GK_Q8;
+  constexpr int OUT = gp_out(KIND), ROOM = 8 * 4096 / OUT;  // warps, and bytes of shared memory for each
   extern __shared__ __align__(1024) unsigned char gmsm[];
   __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
@@ -253,7 +274,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
     }
     for (int i = 0; i < 2; i++) {
       gm_init(gm_smem(sumFull + i), 1);
-      gm_init(gm_smem(sumEmpty + i), 16);  // the eight warps of both CTAs
+      gm_init(gm_smem(sumEmpty + i), 2 * OUT);  // the warps of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -331,7 +352,7 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
       }
     }
   } else if (warp >= 4) {
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int quarter = warp & 3, part = (warp - 4) >> 2;  // of the rows, of the columns
     int n = 0;
     for (int t = pair; t < tiles; t += pairs, n++) {
       const int buf = n & 1;
@@ -341,55 +362,57 @@ __global__ void __launch_bounds__(GP_T, 1) __cluster_dims__(2) k_gemm_pair(const
       int tm, tn;
       gp_tile(A, t, tm, tn);
       const int64_t m0 = (int64_t)tm * 256 + rank * 128 + quarter * 32, m = m0 + lane;
-      const int rows = (int)max((int64_t)0, min((int64_t)32, c.M - m0)), width = A.wide / 2;
-      const uint32_t at = tmem + buf * 256 + half * width + ((uint32_t)quarter << 21), room = smem + GP_RING + (warp - 4) * 4096;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, c.M - m0)), width = A.wide / (OUT / 4);
+      const uint32_t at = tmem + buf * 256 + part * width + ((uint32_t)quarter << 21), room = smem + GP_RING + (warp - 4) * ROOM;
       auto aligned = [&](int o) { return ((uintptr_t)c.out[o] | (uintptr_t)(c.ldo[o] * sizeof(O))) % 16 == 0; };
       if constexpr (KIND == GK_GATE) {
-        const int64_t n0 = (int64_t)tn * A.wide + half * width;
-        gm_rows((O*)c.out[0] + m0 * c.ldo[0] + n0, c.ldo[0], rows, c.N - n0, width, aligned(0), room, [&](int j, O(&o)[16]) {
-          uint32_t v[32];
-          gm_tmem16(at + j, v);
-          gm_tmem16(at + A.wide + j, v + 16);
+        const int64_t n0 = (int64_t)tn * A.wide + part * width;
+        gm_rows<O, 8, ROOM / 32>((O*)c.out[0] + m0 * c.ldo[0] + n0, c.ldo[0], rows, c.N - n0, width, aligned(0), room, [&](int j, O(&o)[8]) {
+          uint32_t v[16];
+          gm_tmem8(at + j, v);
+          gm_tmem8(at + A.wide + j, v + 8);
           gm_loaded(v);
-          float h[16];
+          float h[8];
           with_act(c.act, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) h[i] = act_value(decltype(act)::value, __uint_as_float(v[i])) * __uint_as_float(v[16 + i]);
+            for (int i = 0; i < 8; i++) h[i] = act_value(decltype(act)::value, __uint_as_float(v[i])) * __uint_as_float(v[8 + i]);
           });
           if (c.drop.on) {
 #pragma unroll
-            for (int q = 0; q < 16; q += 4) {
+            for (int q = 0; q < 8; q += 4) {
               const uint4 w = drop_words(c.drop, (uint32_t)m, (uint32_t)((n0 + j + q) / 4));
 #pragma unroll
               for (int i = 0; i < 4; i++) h[q + i] = word_of(w, i) >= c.drop.cut ? h[q + i] * c.drop.scale : 0.f;
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(h[i]);
+          for (int i = 0; i < 8; i += 2) *(uint32_t*)(o + i) = to_word<O>(h[i], h[i + 1]);
         });
         if (c.out[1])
           for (int p = 0; p < 2; p++)
-            gm_rows((O*)c.out[1 + p] + m0 * c.ldo[1 + p] + n0, c.ldo[1 + p], rows, c.N - n0, width, aligned(1 + p), room, [&](int j, O(&o)[16]) {
-              uint32_t v[16];
-              gm_tmem16(at + p * A.wide + j, v);
-              gm_loaded(v);
+            gm_rows<O, 8, ROOM / 32>((O*)c.out[1 + p] + m0 * c.ldo[1 + p] + n0, c.ldo[1 + p], rows, c.N - n0, width, aligned(1 + p), room,
+                                     [&](int j, O(&o)[8]) {
+                                       uint32_t v[8];
+                                       gm_tmem8(at + p * A.wide + j, v);
+                                       gm_loaded(v);
 #pragma unroll
-              for (int i = 0; i < 16; i++) o[i] = gm_cast<O>(__uint_as_float(v[i]));
-            });
+                                       for (int i = 0; i < 8; i += 2) *(uint32_t*)(o + i) = to_word<O>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                                     });
       } else {
         const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
-        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * A.wide + half * width;
+        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * A.wide + part * width;
         const float sa = I8 && m < c.M ? c.aScale[m] : 0.f;
-        gm_rows((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, width, aligned(which), room, [&](int j, O(&o)[16]) {
-          uint32_t v[16];
-          gm_tmem16(at + j, v);
-          gm_loaded(v);
+        gm_rows<O, 16, ROOM / 32>((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, width, aligned(which), room,
+                                  [&](int j, O(&o)[16]) {
+                                    uint32_t v[16];
+                                    gm_tmem16(at + j, v);
+                                    gm_loaded(v);
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
-            else o[i] = gm_cast<O>(__uint_as_float(v[i]));
-          }
-        });
+                                    for (int i = 0; i < 16; i++) {
+                                      if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
+                                      else o[i] = gm_cast<O>(__uint_as_float(v[i]));
+                                    }
+                                  });
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -768,29 +791,34 @@ static GemmPlan gemm_plan(const GemmCall& c) {
   // The terms were measured over 1 to 2048 rows, 1000 to 16384 columns, depths of 500 to 5504, weights not in L2 (both sides of every
   // choice; the choice was the fastest or within a tenth of it in nine of ten). What the operands take from memory at 6.2 GB a ms:
   const double memory = (double)type_bytes(c.type) * c.K * (c.kind == GK_SUM ? 2 : 1) * (c.M + c.N * (c.kind == GK_Q8 ? 1 : 2)) / 6.2e6;
-  // k_gemm_pair: a stage takes 0.17 us (waits and issue) or its products' time, 4 clocks a column that a CTA brings, at 1.85 GHz
+  // k_gemm_pair: a stage takes 0.17 us (waits and issue) or its products' time, 4 clocks a column that a CTA brings, at 1.85 GHz; a tile's results
+  // leave in 12 ns a column while the next tile's come
   // (32 rows and fewer leave its copies of them nearly empty, which take up to twice the time: not for deep products of so few)
   for (int wide = 256 / np; wide >= 64 && nk > 0 && (c.M > 32 || nk <= 8); wide /= 2) {
     const int mine = np == 2 ? wide : wide / 2;
     if (c.b[0].mn && mine < 64) break;
     const int64_t tiles = ceil_div(c.M, 256) * ceil_div(c.N, wide) * products, turns = ceil_div(tiles, GM_SMS / 2);
-    const double t = 8.0 + std::max(memory, turns * (nk * std::max(0.17, 4 * mine / 1850.0) + 0.5));
+    const double out = wide * np * 0.012, chain = nk * std::max(0.17, 4 * mine / 1850.0) + 0.5;
+    const double t = 7.0 + std::max(memory, turns * std::max(chain, out)) + out;
     if (t < best.us) best.large = true, best.wide = wide, best.us = t;
   }
-  // k_gemm_few: a stage takes 0.26 us (two products 0.32), more with more rows; all SMs' stages together come at 7 GB a ms, and a depth that is
-  // shared costs the second kernel
+  // k_gemm_few: a stage takes 0.24 us (two products 0.32), more with more rows; all SMs' stages together come at 10 GB a ms. A row of results
+  // leaves in 50 ns a product, of sums to be joined in 10, and joining costs a second kernel that moves the sums at 4 GB a ms
+  // (two products: never the faster one for more than 32 rows)
   for (int nc = 16; nc <= 128; nc *= 2) {
     const int least = c.a[0].mn ? 64 : 16;
-    if (nc < least) continue;
+    if (nc < least || (best.large && c.M > 32 && c.kind != GK_Q8 && c.kind != GK_SUM)) continue;
     if (nc > least && nc / 2 >= c.M) break;
     const int stage = np * (int)GM_OPERAND + nc * 128;
     const int64_t tiles = ceil_div(c.M, nc) * ceil_div(c.N, 128) * products, n = tiles * std::max(1, nk);
     if (n > INT32_MAX / 2) continue;  // (counted in 32 bits)
-    const double step = (np == 2 ? 0.32 : 0.26) + nc * np * 0.0012, out = 0.2 + std::min<int64_t>(nc, c.M) * np * 0.05;
+    const double step = (np == 2 ? 0.32 : 0.24) + nc * np * 0.0012;
     for (int whole = 1; whole >= (c.split && nk > 0 ? 0 : 1); whole--) {
       const int64_t ctas = whole ? std::min<int64_t>(tiles, GM_SMS) : std::min<int64_t>(GM_SMS, tiles * ceil_div(nk, 4));
+      const double out = 0.2 + std::min<int64_t>(nc, c.M) * np * (whole ? 0.05 : 0.01);
       const double chain = whole ? ceil_div(tiles, ctas) * std::max(nk * step, out) : ceil_div(n, ctas) * step;
-      const double t = 5.5 + std::max({memory, chain, n * stage / 7.0e6}) + out + (whole ? 0.0 : 3.0);
+      const double join = 3.0 + (double)tiles * std::min<int64_t>(nc, c.M) * np * 512 * 2.5 / 4.0e6;
+      const double t = 5.5 + std::max({memory, chain, (double)n * stage / 10.0e6}) + out + (whole ? 0.0 : join);
       if (t >= best.us) continue;
       best.large = false, best.nc = nc, best.ctas = (int)ctas, best.whole = whole, best.us = t;
       best.stages = (int)std::min<int64_t>(GF_STAGES, GF_RING / stage);
@@ -835,7 +863,7 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
     if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
     static_assert(GP_RING + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
     cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
-    cfg.blockDim = GP_T;
+    cfg.blockDim = 128 + gp_out(KIND) * 32;
     cfg.dynamicSmemBytes = roomPair;
     CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
