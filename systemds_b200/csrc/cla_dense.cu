@@ -11,12 +11,24 @@ std::shared_ptr<Matrix> lookup(cla_handle h);
 
 constexpr int DN_T = 256;
 
-// 16 bytes of a row of T: vectors where every row starts on a 16-byte boundary, else element by element
+// 16 bytes of a row of T: one vector where every row starts on a 16-byte boundary (vec), else out of the two vectors that hold them (each has some of
+// the wanted bytes, so neither reaches beyond what can be read), and at a row's end element by element.
 template <class T> constexpr int DN_V = 16 / (int)sizeof(T);
+__device__ __forceinline__ uint4 load_across(const void* p) {
+  const uint4* a = (const uint4*)((uintptr_t)p & ~(uintptr_t)15);
+  const uint4 lo = a[0], hi = a[1];
+  const uint32_t words = ((uint32_t)(uintptr_t)p >> 2) & 3, bits = ((uint32_t)(uintptr_t)p & 3) * 8;
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 7; i++) w[i] = words & 1 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; i++) w[i] = words & 2 ? w[i + 2] : w[i];
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
 template <class T>
 __device__ __forceinline__ void load_vec(const T* p, int n, bool vec, T (&v)[DN_V<T>]) {
-  if (vec && n >= DN_V<T>) {
-    *(uint4*)v = *(const uint4*)p;
+  if (n >= DN_V<T>) {
+    *(uint4*)v = vec || ((uintptr_t)p & 15) == 0 ? *(const uint4*)p : load_across(p);
   } else {
 #pragma unroll
     for (int i = 0; i < DN_V<T>; i++) v[i] = i < n ? p[i] : from_f32<T>(0.f);
@@ -68,9 +80,9 @@ __device__ __forceinline__ DropPieces<N> drop_pieces(const DropDev& d, int64_t c
 // ---- dropout --------------------------------------------------------------------------------------------------------
 // Pieces of 16 bytes (F64: 32, the four columns of a counter). Bound: the words (sixteen 64-bit products and as many three-way logic
 // operations for four columns) next to memory.
-template <class T>
+template <class T, bool VEC>
 __global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, int64_t cols, T* y, int64_t ldy, const __grid_constant__ DropDev d,
-                                                     const __grid_constant__ Walk w, int vec) {
+                                                     const __grid_constant__ Walk w) {
   constexpr int P = DN_V<T>, V = P < 4 ? 4 : P, N = V / 4;
   struct Kept {
     const T* x;
@@ -82,7 +94,7 @@ __global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, in
   };
   auto load = [&](Kept& k) {
 #pragma unroll
-    for (int h = 0; h < V; h += P) load_vec(k.x + h, k.left - h, vec, (T(&)[P])k.next[h]);
+    for (int h = 0; h < V; h += P) load_vec(k.x + h, k.left - h, VEC, (T(&)[P])k.next[h]);
   };
   const int64_t r0 = walk_first(w), step = walk_step(w);
   walk<1>(
@@ -122,7 +134,7 @@ __global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, in
           }
         }
 #pragma unroll
-        for (int h = 0; h < V; h += P) store_vec(k.y + h, k.left - h, vec, (const T(&)[P])v[h]);
+        for (int h = 0; h < V; h += P) store_vec(k.y + h, k.left - h, VEC, (const T(&)[P])v[h]);
         k.y += k.stepY;
       });
 }
@@ -172,7 +184,7 @@ __global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__
   const int lane = threadIdx.x % G, warp = threadIdx.x / 32;
   const int64_t r = (int64_t)blockIdx.x * (DN_T / G) + threadIdx.x / G;
   if (G == 32 && r >= rows) return;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the product's weights may come meanwhile)
+  gm_let_next();  // (the product's weights may come meanwhile)
   const T* p = x + r * ldx + (VEC ? lane * V : lane);
   int8_t* to = q + r * ldq + (VEC ? lane * V : lane);
   alignas(16) T v[C][V];
@@ -291,10 +303,10 @@ __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x,
 
 // ---- the gated block's elementwise gradients ----------------------------------------------------------------------------
 // (the next row's values are on their way while a row's are worked on)
-template <class T>
+template <class T, bool VEC>
 __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh, int64_t lddh, const T* __restrict__ g, int64_t ldg,
                                                        const T* __restrict__ u, int64_t ldu, int64_t cols, T* __restrict__ dg, T* __restrict__ du,
-                                                       int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w, int vec) {
+                                                       int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w) {
   constexpr int V = DN_V<T>, N = V / 4;
   const int64_t r0 = walk_first(w), step = walk_step(w);
   struct Values {
@@ -308,10 +320,11 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
     DropPieces<N> drop;
     Values next;
   };
+  gm_let_next();
   auto load = [&](int64_t r, int64_t c, int left, Values& v) {
-    load_vec(dh + r * lddh + c, left, vec, v.h);
-    load_vec(g + r * ldg + c, left, vec, v.g);
-    load_vec(u + r * ldu + c, left, vec, v.u);
+    load_vec(dh + r * lddh + c, left, VEC, v.h);
+    load_vec(g + r * ldg + c, left, VEC, v.g);
+    load_vec(u + r * ldu + c, left, VEC, v.u);
   };
   with_act(act, [&](auto name) {
     walk<1>(
@@ -351,26 +364,38 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
           store_vec(du + r * ldo + k.c, k.left, true, v.u);
         });
   });
+  gm_after_previous();  // (the copies next to this: who waits for this kernel has waited for both)
 }
 
 // ---- copies -----------------------------------------------------------------------------------------------------------
-// Rows to rows that start on 16-byte boundaries, as the products read them.
-template <class T, int U>
-__global__ void __launch_bounds__(DN_T) k_repitch(const T* __restrict__ x, int64_t ldx, int64_t cols, T* __restrict__ y, int64_t ldy,
-                                                  const __grid_constant__ Walk w) {
-  constexpr int V = DN_V<T>;
-  walk<U>(
-      w, [](int piece) { return (int64_t)piece * V; },
-      [&](int64_t c, int64_t r, int64_t step, int n) {
-        const int left = (int)min((int64_t)V, cols - c);
-        alignas(16) T v[U][V];
-#pragma unroll
-        for (int k = 0; k < U; k++)
-          if (k < n) load_vec(x + (r + k * step) * ldx + c, left, false, v[k]);
-#pragma unroll
-        for (int k = 0; k < U; k++)
-          if (k < n) store_vec(y + (r + k * step) * ldy + c, left, true, v[k]);
-      });
+// Rows to rows that start on lines of 128 bytes, as the products read them; up to three matrices a launch. In bytes: the elements' size is of no matter.
+struct Copies {
+  const void* from[3];
+  void* to[3];
+  int64_t ldFrom[3], ldTo[3];
+  int bytes[3];  // of a row
+  Walk walk[3];
+  int ctas[4];   // the first CTA of each, down the rows
+};
+__global__ void __launch_bounds__(DN_T) k_repitch(const __grid_constant__ Copies c) {
+  gm_let_next();
+  const int k = (int)blockIdx.y >= c.ctas[2] ? 2 : (int)blockIdx.y >= c.ctas[1] ? 1 : 0;
+  const Walk& w = c.walk[k];
+  const uint8_t* x = (const uint8_t*)c.from[k];
+  uint8_t* y = (uint8_t*)c.to[k];
+  const int tx = threadIdx.x & ((1 << w.log) - 1), down = DN_T >> w.log, ctas = c.ctas[k + 1] - c.ctas[k];
+  const int64_t step = (int64_t)ctas * down, ldx = c.ldFrom[k], ldy = c.ldTo[k];
+  for (int piece = blockIdx.x * (1 << w.log) + tx; piece < w.per; piece += gridDim.x << w.log) {
+    const int left = c.bytes[k] - piece * 16;
+    for (int64_t r = (int64_t)(blockIdx.y - c.ctas[k]) * down + (threadIdx.x >> w.log); r < w.rows; r += 2 * step) {
+      alignas(16) uint8_t v[2][16];
+      const bool two = r + step < w.rows;
+      load_vec(x + r * ldx + piece * 16, left, false, v[0]);
+      if (two) load_vec(x + (r + step) * ldx + piece * 16, left, false, v[1]);
+      store_vec(y + r * ldy + piece * 16, left, true, v[0]);
+      if (two) store_vec(y + (r + step) * ldy + piece * 16, left, true, v[1]);
+    }
+  }
 }
 template <class T, int U>
 __global__ void __launch_bounds__(DN_T) k_narrow(const double* __restrict__ x, int64_t cols, T* __restrict__ y, int64_t ldy,
@@ -500,26 +525,50 @@ struct Work {
     return r;
   }
 };
-// The operand as the products read it: itself, or a copy in the workspace where its rows do not start on 16-byte boundaries.
-int64_t aligned(GemmOperand& o, int64_t i, int64_t k, int type, Work& w, bool run, cudaStream_t s) {
-  const int bytes = type_bytes(type);
-  const int64_t rows = o.mn ? k : i, cols = o.mn ? i : k;
-  if (rows <= 1 && (uintptr_t)o.p % 16 == 0) o.ld = round_up(o.ld, 16 / bytes);  // (no second row)
-  if (rows_aligned(o.p, o.ld, 2, bytes)) return CLA_OK;
-  const int64_t ld = round_up(cols, 16 / bytes);
-  void* to = w.take(rows * ld * bytes);
-  if (run && rows && cols) {
-    Walk k;
-    const dim3 grid = walk_grid(k, rows, (cols * bytes + 15) / 16, 2);
-    if (bytes == 1) k_repitch<int8_t, 2><<<grid, DN_T, 0, s>>>((const int8_t*)o.p, o.ld, cols, (int8_t*)to, ld, k);
-    else k_repitch<__half, 2><<<grid, DN_T, 0, s>>>((const __half*)o.p, o.ld, cols, (__half*)to, ld, k);
-    CLA_CUDA(cudaGetLastError());
+// Rows of copies and intermediate results: on lines of 128 bytes, which is what the products read of a row at a time (4095 x 2048 x 5461, weights with
+// rows on 16-byte boundaries only: 188 us; on lines: 182 us)
+constexpr int PITCH = 128;
+// Operands as the products read them: themselves, or copies in the workspace where their rows do not start on 16-byte boundaries. The copies are made in
+// one launch, by run().
+struct Aligned {
+  Copies c = {};
+  int n = 0;
+  Work& w;
+  explicit Aligned(Work& work) : w(work) {}
+  void operator()(GemmOperand& o, int64_t i, int64_t k, int type) {
+    const int bytes = type_bytes(type);
+    const int64_t rows = o.mn ? k : i, cols = o.mn ? i : k;
+    if (rows <= 1 && (uintptr_t)o.p % 16 == 0) o.ld = round_up(o.ld, 16 / bytes);  // (no second row)
+    if (rows_aligned(o.p, o.ld, 2, bytes)) return;
+    const int64_t ld = round_up(cols, PITCH / bytes);
+    void* to = w.take(rows * ld * bytes);
+    if (rows && cols) {
+      c.from[n] = o.p, c.to[n] = to;
+      c.ldFrom[n] = o.ld * bytes, c.ldTo[n] = ld * bytes;
+      c.bytes[n] = (int)(cols * bytes);
+      c.walk[n].rows = rows;
+      n++;
+    }
+    o.p = to;
+    o.ld = ld;
   }
-  o.p = to;
-  o.ld = ld;
-  return CLA_OK;
-}
-
+  int64_t run(int device, cudaStream_t s) {
+    if (n == 0) return CLA_OK;
+    static OncePerDevice once;
+    DN_CHECK(once(device, [] { return like_products(k_repitch); }));
+    unsigned x = 1;
+    for (int k = 0; k < n; k++) {
+      const dim3 g = walk_grid(c.walk[k], c.walk[k].rows, (c.bytes[k] + 15) / 16, 2);
+      x = std::max(x, g.x);
+      c.ctas[k + 1] = c.ctas[k] + (int)g.y;
+    }
+    const unsigned y = (unsigned)c.ctas[n];
+    for (int k = n + 1; k < 4; k++) c.ctas[k] = (int)y;
+    k_repitch<<<dim3(x, y), DN_T, 0, s>>>(c);
+    CLA_CUDA(cudaGetLastError());
+    return CLA_OK;
+  }
+};
 int64_t product(GemmCall& g, Work& w, bool run, cudaStream_t s) {
   if (const int64_t n = gemm_workspace(g)) g.parts = w.take(n);
   return run ? launch_gemm(g, s) : CLA_OK;
@@ -549,17 +598,19 @@ int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s, bool split = 
   g.device = c.device;
   g.split = split;
   if (c.M == 0 || c.N == 0) return CLA_OK;
-  DN_CHECK(aligned(g.b[0], c.N, c.K, CLA_T_I8, w, run, s));
+  Aligned aligned(w);
+  aligned(g.b[0], c.N, c.K, CLA_T_I8);
+  if (c.aType == CLA_T_I8) aligned(g.a[0], c.M, c.K, CLA_T_I8);
+  if (run) DN_CHECK(aligned.run(c.device, s));
+  if (aligned.n) g.after = AFTER_ALL;
   if (c.aType != CLA_T_I8) {
-    const int64_t ld = round_up(c.K, 16);
+    const int64_t ld = round_up(c.K, PITCH);
     int8_t* q = (int8_t*)w.take(c.M * ld);
     float* sc = (float*)w.take(c.M * 4);
     if (run) DN_CHECK(quantize(c.aType, c.a, c.lda, c.M, c.K, false, q, ld, sc, c.device, s));
     g.a[0] = {q, ld, false};
     g.aScale = sc;
-    g.aLate = c.K > 0;  // (the last kernel before the product)
-  } else {
-    DN_CHECK(aligned(g.a[0], c.M, c.K, CLA_T_I8, w, run, s));
+    g.after = AFTER_A;  // (the last kernel before the product)
   }
   return product(g, w, run, s);
 }
@@ -605,50 +656,59 @@ int64_t gated_fwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaS
   g.a[0] = {c.x, c.ldx, false};
   g.b[0] = {c.wg, c.ldwg, !c.wTrans};
   g.b[1] = {c.wu, c.ldwu, !c.wTrans};
-  DN_CHECK(aligned(g.a[0], c.M, c.D, c.type, w, run, s));
-  for (int i = 0; i < 2; i++) DN_CHECK(aligned(g.b[i], c.F, c.D, c.type, w, run, s));
+  Aligned aligned(w);
+  aligned(g.a[0], c.M, c.D, c.type);
+  for (int i = 0; i < 2; i++) aligned(g.b[i], c.F, c.D, c.type);
+  if (run) DN_CHECK(aligned.run(c.device, s));
+  if (aligned.n) g.after = AFTER_ALL;
   g.out[0] = c.h, g.out[1] = c.g, g.out[2] = c.u;
   g.ldo[0] = c.ldh, g.ldo[1] = c.ldg, g.ldo[2] = c.ldu;
   g.drop = d;
   return product(g, w, run, s);
 }
 int64_t gated_bwd(const cla_gated& c, const DropDev& d, bool run, Work& w, cudaStream_t s) {
-  const int64_t ld = round_up(c.F, 8);
+  const int64_t ld = round_up(c.F, PITCH / 2);
   void* dg = w.take(c.M * ld * 2);
   void* du = w.take(c.M * ld * 2);
-  if (run && c.M && c.F) {
-    const int vec = rows_aligned(c.dh, c.lddh, c.M, 2) && rows_aligned(c.g, c.ldg, c.M, 2) && rows_aligned(c.u, c.ldu, c.M, 2);
+  const bool wantX = c.dx && c.M && c.D, wantW = c.dwg && c.D && c.F;
+  GemmCall x = gated_call(c, GK_SUM, c.M, c.D, c.F), wt = gated_call(c, GK_PAIR, c.D, c.F, c.M);
+  x.a[0] = {dg, ld, false};
+  x.a[1] = {du, ld, false};
+  x.b[0] = {c.wg, c.ldwg, (bool)c.wTrans};
+  x.b[1] = {c.wu, c.ldwu, (bool)c.wTrans};
+  x.out[0] = c.dx, x.ldo[0] = c.lddx;
+  wt.a[0] = {c.x, c.ldx, true};
+  wt.b[0] = {dg, ld, true};
+  wt.b[1] = {du, ld, true};
+  wt.out[0] = c.dwg, wt.out[1] = c.dwu;
+  wt.ldo[0] = c.lddwg, wt.ldo[1] = c.lddwu;
+  Aligned aligned(w);
+  if (wantX)
+    for (int i = 0; i < 2; i++) aligned(x.b[i], c.D, c.F, c.type);
+  if (wantW) aligned(wt.a[0], c.D, c.M, c.type);
+  if (run) DN_CHECK(aligned.run(c.device, s));
+  const bool grads = c.M && c.F;
+  if (run && grads) {
+    const bool vec = rows_aligned(c.dh, c.lddh, c.M, 2) && rows_aligned(c.g, c.ldg, c.M, 2) && rows_aligned(c.u, c.ldu, c.M, 2);
     Walk k;
-    const dim3 grid = walk_grid(k, c.M, ld / 8, 1);
-    auto go = [&](auto t) {
+    const dim3 grid = walk_grid(k, c.M, (c.F + 7) / 8, 1);
+    auto go = [&](auto t, auto kernel, OncePerDevice& once) -> int64_t {
       using T = decltype(t);
-      k_gate_grad<T><<<grid, DN_T, 0, s>>>((const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld, d, c.act, k,
-                                              vec);
+      DN_CHECK(once(c.device, [&] { return like_products(kernel); }));
+      EarlyLaunch l(grid, DN_T, 0, s, aligned.n > 0);  // (next to the copies)
+      CLA_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, (const T*)c.dh, c.lddh, (const T*)c.g, c.ldg, (const T*)c.u, c.ldu, c.F, (T*)dg, (T*)du, ld,
+                                  d, (int)c.act, k));
+      return CLA_OK;
     };
-    if (c.type == CLA_T_BF16) go(__nv_bfloat16());
-    else go(__half());
-    CLA_CUDA(cudaGetLastError());
+    static OncePerDevice once[4];
+    using B = __nv_bfloat16;
+    if (c.type == CLA_T_BF16) DN_CHECK(vec ? go(B(), k_gate_grad<B, true>, once[0]) : go(B(), k_gate_grad<B, false>, once[1]));
+    else DN_CHECK(vec ? go(__half(), k_gate_grad<__half, true>, once[2]) : go(__half(), k_gate_grad<__half, false>, once[3]));
   }
-  if (c.dx && c.M && c.D) {
-    GemmCall g = gated_call(c, GK_SUM, c.M, c.D, c.F);
-    g.a[0] = {dg, ld, false};
-    g.a[1] = {du, ld, false};
-    g.b[0] = {c.wg, c.ldwg, (bool)c.wTrans};
-    g.b[1] = {c.wu, c.ldwu, (bool)c.wTrans};
-    for (int i = 0; i < 2; i++) DN_CHECK(aligned(g.b[i], c.D, c.F, c.type, w, run, s));
-    g.out[0] = c.dx, g.ldo[0] = c.lddx;
-    DN_CHECK(product(g, w, run, s));
-  }
-  if (c.dwg && c.D && c.F) {
-    GemmCall g = gated_call(c, GK_PAIR, c.D, c.F, c.M);
-    g.a[0] = {c.x, c.ldx, true};
-    g.b[0] = {dg, ld, true};
-    g.b[1] = {du, ld, true};
-    DN_CHECK(aligned(g.a[0], c.D, c.M, c.type, w, run, s));
-    g.out[0] = c.dwg, g.out[1] = c.dwu;
-    g.ldo[0] = c.lddwg, g.ldo[1] = c.lddwu;
-    DN_CHECK(product(g, w, run, s));
-  }
+  x.after = wt.after = grads || aligned.n ? AFTER_ALL : AFTER_CALL;
+  if (wantX && c.F) wt.after = AFTER_NONE;
+  if (wantX) DN_CHECK(product(x, w, run, s));
+  if (wantW) DN_CHECK(product(wt, w, run, s));
   return CLA_OK;
 }
 int64_t check_work(const Work& need, const void* work, int64_t bytes) {
@@ -678,7 +738,7 @@ int64_t chunk_rows(const Matrix* m, int64_t rows) {
 }
 // What the 8-bit product of a chunk of so many rows needs: their cells, q and scales
 int64_t q8_chunk_bytes(const Matrix* m, int64_t rows) {
-  return round_up(rows * round_up(m->nCols, 16), 256) + round_up(rows * 4, 256) + round_up(rows * m->nCols * 8, 256);
+  return round_up(rows * round_up(m->nCols, PITCH), 256) + round_up(rows * 4, 256) + round_up(rows * m->nCols * 8, 256);
 }
 
 }  // namespace
@@ -709,10 +769,10 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
   with_type(type, [&](auto t) {
     using T = decltype(t);
     constexpr int V = std::max(4, DN_V<T>);
-    const int vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(y, ldy, rows, sizeof(T));
+    const bool vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(y, ldy, rows, sizeof(T));
     Walk w;
     const dim3 grid = walk_grid(w, rows, (cols + V - 1) / V, 1);
-    k_dropout<T><<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w, vec);
+    (vec ? k_dropout<T, true> : k_dropout<T, false>)<<<grid, DN_T, 0, (cudaStream_t)stream>>>((const T*)x, ldx, cols, (T*)y, ldy, d, w);
   });
   CLA_CUDA(cudaGetLastError());
   return CLA_OK;
@@ -805,7 +865,7 @@ int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_
 int64_t cla_q8_rmm_workspace(cla_handle h, int64_t N) {
   DN_MATRIX(h);
   if (N < 0) return fail(CLA_ERR_SHAPE, "8-bit right product: negative size");
-  return q8_chunk_bytes(m, chunk_rows(m, m->nRows)) + round_up(N * round_up(m->nCols, 16), 256);
+  return q8_chunk_bytes(m, chunk_rows(m, m->nRows)) + round_up(N * round_up(m->nCols, PITCH), 256);
 }
 int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* bScale, int64_t N, int32_t outType, void* out, int64_t ldo,
                        void* work, int64_t workBytes, void* stream) {
@@ -821,7 +881,7 @@ int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* 
   Work w{(char*)work};
   GemmOperand bo{b, ldb, false};
   if ((uintptr_t)work % 256) return fail(CLA_ERR_BAD_ARG, "workspace not 256-byte aligned");
-  const int64_t room = workBytes - round_up(N * round_up(m->nCols, 16), 256);
+  const int64_t room = workBytes - round_up(N * round_up(m->nCols, PITCH), 256);
   int64_t cap = room / std::max<int64_t>(1, q8_chunk_bytes(m, SKIP_ROWS)) * SKIP_ROWS;
   if (!work || cap < SKIP_ROWS) return fail(CLA_ERR_BAD_ARG, "8-bit right product: workspace below 1024 rows");
   cap = std::min(cap, round_up(c.M, SKIP_ROWS));
@@ -830,7 +890,9 @@ int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* 
   cudaStream_t s = (cudaStream_t)stream;
   m->stats.calls_rmm++;
   DN_CHECK(order_begin(m, s));
-  int64_t rc = aligned(bo, N, c.K, CLA_T_I8, w, true, s);
+  Aligned aligned(w);
+  aligned(bo, N, c.K, CLA_T_I8);
+  int64_t rc = aligned.run(c.device, s);
   c.b = (const int8_t*)bo.p, c.ldb = bo.ld;
   double* X = (double*)w.take(cap * m->nCols * 8);
   if (rc >= 0)

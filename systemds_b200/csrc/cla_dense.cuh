@@ -177,8 +177,31 @@ struct GemmCall {
   int device = 0;
   bool split = true;      // whether the depth may be split (gemm_workspace() is 0 if not)
   void* parts = nullptr;  // gemm_workspace() bytes, 256-byte aligned
-  bool aLate = false;     // the kernel before this one in the stream writes a (and aScale) and nothing else that is read here, and
-                          // itself started after everything before it was done
+  int after = 0;          // AFTER_*
+};
+// What a kernel has to do with the one that the same call has launched just before it (which itself came after all that the stream held). The kernel may
+// then start while that one still runs, and waits for its end where it says; the one before lets it by gm_let_next().
+enum After {
+  AFTER_CALL,  // there is none: an ordinary launch
+  AFTER_ALL,   // it writes operands: before they are read
+  AFTER_A,     // it writes a and aScale alone: the weights are read before
+  AFTER_NONE   // the two read and write nothing that the other writes: at the end, so that who waits for this one has waited for both. The one
+               // before has let this one by only after its own wait, so that what came before both is over when this one starts
+};
+__device__ __forceinline__ void gm_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void gm_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// A launch configuration with the kernel before still running, or not (After)
+struct EarlyLaunch {
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = {};
+  EarlyLaunch(dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool early) {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = early ? 1 : 0;
+  }
+  EarlyLaunch(const EarlyLaunch&) = delete;
 };
 int64_t gemm_workspace(const GemmCall& c);  // goes by the sizes, the types and which index is contiguous
 int64_t launch_gemm(const GemmCall& c, cudaStream_t s);

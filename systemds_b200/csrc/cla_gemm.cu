@@ -149,26 +149,36 @@ struct alignas(64) GemmArgs {
   int stages;            // of the ring
   int nc;                // k_gemm_few: rows of a tile,
   int ctas, whole;       // CTAs, and whether each has whole tiles
-  int early;             // whether the weights need not wait for the kernel before
   uint32_t idesc;
 };
 
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f32<O>(v); }
 
-// 32 rows (a lane each) of `width` columns to memory. f(j, o): columns j .. j + CH - 1 of the lane's row, all lanes together. They go through the
-// warp's shared memory, LINE bytes (128 or 64) of every row at a time, and from there in whole lines: pieces of 16 bytes where rows start
-// on 16-byte boundaries (vec), else a word a lane. The pieces are swizzled over the rows.
-template <class O, int CH, int LINE, class F>
-__device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t cols, int width, bool vec, uint32_t buf, F&& f) {
-  constexpr int COLS = LINE / (int)sizeof(O), PIECES = CH * (int)sizeof(O) / 16, PER = LINE / 16;  // columns; pieces of a chunk, of a line
-  const int lane = threadIdx.x & 31;
-  const auto place = [&](int r, int piece) { return buf + r * LINE + (LINE == 128 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) * 16; };
+// The warps that hold the same 32 rows of a tile (a lane each), G of them, write `width` columns of these rows. f(j, o): columns j .. j + CH - 1 of
+// the lane's row, all lanes together. The warps take LINE / G bytes of a row in turn into the shared memory of the group; from there whole rows
+// of up to LINE bytes go out, 32 / G rows a warp: in pieces of 16 bytes where rows start on 16-byte boundaries (vec), else a word a
+// lane. (Long pieces count where rows do not start on sectors: each piece then writes parts of two sectors.) The pieces of shared
+// memory are swizzled over the rows.
+__device__ __forceinline__ void gm_group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// Whether all of them say so
+__device__ __forceinline__ bool gm_group_all(int id, int threads, bool ok) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(id), "r"(threads), "r"((uint32_t)ok)
+               : "memory");
+  return r != 0;
+}
+template <class O, int CH, int G, class F>
+__device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t cols, int width, bool vec, uint32_t buf, int part, int id, F&& f) {
+  constexpr int LINE = 256, PIECES = CH * (int)sizeof(O) / 16;
+  const int lane = threadIdx.x & 31, mine = min(LINE / G / (int)sizeof(O), width / G), all = mine * G;  // columns of a warp, of the group
+  const auto place = [&](int r, int piece) { return buf + r * LINE + (piece ^ (r & 7)) * 16; };
 #pragma unroll 1
-  for (int c0 = 0; c0 < width; c0 += COLS) {
-    const int some = min(COLS, width - c0);
+  for (int c0 = 0; c0 < width; c0 += all) {
 #pragma unroll 1
-    for (int j = 0; j < some; j += CH) {
+    for (int j = part * mine; j < (part + 1) * mine; j += CH) {
       alignas(16) O o[CH];
       f(c0 + j, o);
 #pragma unroll
@@ -177,13 +187,14 @@ __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t co
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, j * (int)sizeof(O) / 16 + i)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
       }
     }
-    __syncwarp();
-    const int64_t there = min((int64_t)some, cols - c0) * (int)sizeof(O);  // bytes of a row
+    gm_group_sync(id, G * 32);
+    const int there = (int)max((int64_t)0, min((int64_t)all, cols - c0)) * (int)sizeof(O);  // bytes of a row
+    const int end = min(rows, (part + 1) * (32 / G));
     if (vec) {
-      const int piece = lane % PER;
-      const int64_t left = there - piece * 16;
+      const int per = all * (int)sizeof(O) / 16, down = 32 / per;  // pieces of a row, rows at a time (all powers of two)
+      const int piece = lane & (per - 1), left = there - piece * 16;
 #pragma unroll 2
-      for (int r = lane / PER; r < rows; r += 32 / PER) {
+      for (int r = part * (32 / G) + lane / per; r < end; r += down) {
         uint4 x;
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(place(r, piece)) : "memory");
         char* p = (char*)(out + r * ld + c0) + piece * 16;
@@ -196,33 +207,29 @@ __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t co
         }
       }
     } else {
-      constexpr int WORDS = LINE / 4;
-      const int word = lane % WORDS;
-      const int64_t left = there - 4 * word;  // bytes from the lane's word on
-#pragma unroll 2
-      for (int r0 = 0; r0 < rows; r0 += 32 / WORDS) {
-        const int r = r0 + lane / WORDS;
-        uint32_t v;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(place(r, word / 4) + (word % 4) * 4) : "memory");
-        char* p = (char*)(out + r * ld + c0) + 4 * word;
-        if (sizeof(O) >= 4) {
-          if (left >= 4 && r < rows) *(uint32_t*)p = v;
-        } else {
-          // a row that starts in the middle of a word: the words are the upper half of a lane's and the lower half of the next one's
-          const bool odd = (uintptr_t)p & 2;  // (of the whole row)
-          const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
-          if (r < rows) {
-            if (odd && word == 0 && left >= 2) *(uint16_t*)p = (uint16_t)v;
-            const int64_t mine = left - (odd ? 2 : 0);
-            const uint32_t w = odd ? __byte_perm(v, next, 0x5432) : v;
-            char* q = p + (odd ? 2 : 0);
-            if (mine >= 4 && !(odd && word == WORDS - 1)) *(uint32_t*)q = w;
-            else if (mine >= 2) *(uint16_t*)q = (uint16_t)w;
+      for (int r = part * (32 / G); r < end; r++) {
+        char* const row = (char*)(out + r * ld + c0);
+        const auto word = [&](int w) {
+          uint32_t v;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(place(r, w >> 2) + (w & 3) * 4) : "memory");
+          return v;
+        };
+        if (sizeof(O) >= 4 || ((uintptr_t)row & 2) == 0) {
+          for (int w = lane; 4 * w < there; w += 32) {
+            if (4 * w + 4 <= there) *(uint32_t*)(row + 4 * w) = word(w);
+            else *(uint16_t*)(row + 4 * w) = (uint16_t)word(w);
+          }
+        } else {  // the row starts in the middle of a word: the words are the upper half of one and the lower half of the next
+          if (lane == 0 && there > 0) *(uint16_t*)row = (uint16_t)word(0);
+          for (int w = lane; 4 * w + 2 < there; w += 32) {
+            const uint32_t v = word(w);
+            if (4 * w + 6 <= there) *(uint32_t*)(row + 4 * w + 2) = __byte_perm(v, word(w + 1), 0x5432);
+            else *(uint16_t*)(row + 4 * w + 2) = (uint16_t)(v >> 16);
           }
         }
       }
     }
-    __syncwarp();
+    gm_group_sync(id, G * 32);
   }
 }
 template <int KIND, class O>
@@ -251,7 +258,7 @@ __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& 
 template <int KIND, class O>
 __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
   constexpr bool I8 = KIND == GK_Q8;
-  constexpr int OUT = gp_out(KIND), ROOM = 8 * 4096 / OUT;  // warps, and bytes of shared memory for each
+  constexpr int OUT = gp_out(KIND), G = OUT / 4;  // warps that write results, and of each 32 rows of a tile
   extern __shared__ __align__(1024) unsigned char gmsm[];
   __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
@@ -286,6 +293,10 @@ __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2
   const uint32_t tmem = tmemAt;
   bool ok = true;
   const uint32_t fullAt = gm_smem(full), emptyAt = gm_smem(empty);
+  if (c.after != AFTER_NONE) {
+    gm_after_previous();
+    gm_let_next();  // (not before: an AFTER_NONE kernel relies on the ones before this one)
+  }
   if (warp == 0) {
     const uint32_t barAt = gm_peer(fullAt, 0);  // the first CTA's
     int s = 0, issued = 0;
@@ -356,18 +367,18 @@ __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2
     int n = 0;
     for (int t = pair; t < tiles; t += pairs, n++) {
       const int buf = n & 1;
-      ok = gm_wait(gm_smem(sumFull + buf), (n >> 1) & 1);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      ok = gm_group_all(1 + quarter, G * 32, gm_wait(gm_smem(sumFull + buf), (n >> 1) & 1));  // (together: they wait for one another below)
+      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       int tm, tn;
       gp_tile(A, t, tm, tn);
       const int64_t m0 = (int64_t)tm * 256 + rank * 128 + quarter * 32, m = m0 + lane;
-      const int rows = (int)max((int64_t)0, min((int64_t)32, c.M - m0)), width = A.wide / (OUT / 4);
-      const uint32_t at = tmem + buf * 256 + part * width + ((uint32_t)quarter << 21), room = smem + GP_RING + (warp - 4) * ROOM;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, c.M - m0));
+      const uint32_t at = tmem + buf * 256 + ((uint32_t)quarter << 21), room = smem + GP_RING + quarter * 8192;
       auto aligned = [&](int o) { return ((uintptr_t)c.out[o] | (uintptr_t)(c.ldo[o] * sizeof(O))) % 16 == 0; };
       if constexpr (KIND == GK_GATE) {
-        const int64_t n0 = (int64_t)tn * A.wide + part * width;
-        gm_rows<O, 8, ROOM / 32>((O*)c.out[0] + m0 * c.ldo[0] + n0, c.ldo[0], rows, c.N - n0, width, aligned(0), room, [&](int j, O(&o)[8]) {
+        const int64_t n0 = (int64_t)tn * A.wide;
+        gm_rows<O, 8, G>((O*)c.out[0] + m0 * c.ldo[0] + n0, c.ldo[0], rows, c.N - n0, A.wide, aligned(0), room, part, 1 + quarter, [&](int j, O(&o)[8]) {
           uint32_t v[16];
           gm_tmem8(at + j, v);
           gm_tmem8(at + A.wide + j, v + 8);
@@ -390,29 +401,29 @@ __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2
         });
         if (c.out[1])
           for (int p = 0; p < 2; p++)
-            gm_rows<O, 8, ROOM / 32>((O*)c.out[1 + p] + m0 * c.ldo[1 + p] + n0, c.ldo[1 + p], rows, c.N - n0, width, aligned(1 + p), room,
-                                     [&](int j, O(&o)[8]) {
-                                       uint32_t v[8];
-                                       gm_tmem8(at + p * A.wide + j, v);
-                                       gm_loaded(v);
+            gm_rows<O, 8, G>((O*)c.out[1 + p] + m0 * c.ldo[1 + p] + n0, c.ldo[1 + p], rows, c.N - n0, A.wide, aligned(1 + p), room, part, 1 + quarter,
+                             [&](int j, O(&o)[8]) {
+                               uint32_t v[8];
+                               gm_tmem8(at + p * A.wide + j, v);
+                               gm_loaded(v);
 #pragma unroll
-                                       for (int i = 0; i < 8; i += 2) *(uint32_t*)(o + i) = to_word<O>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                                     });
+                               for (int i = 0; i < 8; i += 2) *(uint32_t*)(o + i) = to_word<O>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                             });
       } else {
         const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
-        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * A.wide + part * width;
+        const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * A.wide;
         const float sa = I8 && m < c.M ? c.aScale[m] : 0.f;
-        gm_rows<O, 16, ROOM / 32>((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, width, aligned(which), room,
-                                  [&](int j, O(&o)[16]) {
-                                    uint32_t v[16];
-                                    gm_tmem16(at + j, v);
-                                    gm_loaded(v);
+        gm_rows<O, 16, G>((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, A.wide, aligned(which), room, part, 1 + quarter,
+                          [&](int j, O(&o)[16]) {
+                            uint32_t v[16];
+                            gm_tmem16(at + j, v);
+                            gm_loaded(v);
 #pragma unroll
-                                    for (int i = 0; i < 16; i++) {
-                                      if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
-                                      else o[i] = gm_cast<O>(__uint_as_float(v[i]));
-                                    }
-                                  });
+                            for (int i = 0; i < 16; i++) {
+                              if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
+                              else o[i] = gm_cast<O>(__uint_as_float(v[i]));
+                            }
+                          });
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -420,6 +431,7 @@ __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gm_peer(gm_smem(sumEmpty + buf), 0)) : "memory");
     }
   }
+  if (c.after == AFTER_NONE) gm_after_previous();
   if (!ok) atomicExch(&denseErr, 201);
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -440,9 +452,6 @@ __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2
 // The operand of the rows may come from the kernel before (quantised activations), whose end is waited for only where they are
 // needed: the weights are on their way by then.
 constexpr int GF_T = 256, GF_STAGES = 16, GF_RING = 220 * 1024;
-
-__device__ __forceinline__ void gm_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void gm_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // The first stage of CTA i's range; `whole`: of tiles. (of n stages in tiles of nk)
 __host__ __device__ inline int gf_start(int i, int ctas, int n, int nk, bool whole) {
@@ -491,7 +500,6 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
   const int n = A.tilesM * A.tilesN * nk, b0 = gf_start(blockIdx.x, gridDim.x, n, nk, A.whole), b1 = gf_start(blockIdx.x + 1, gridDim.x, n, nk, A.whole);
   const bool cMn = !I8 && c.a[0].mn, lMn = !I8 && c.b[0].mn;  // the result's rows and columns
   const uint32_t stage = NP * GM_OPERAND + A.nc * 128;
-  if (!A.whole) gm_let_next();
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -560,14 +568,14 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
           gm_load<false>(dc, A.a + seg, k0, (int)q.m0, bar);
         }
       };
-      const int ahead = A.early ? min(A.stages, b1 - b0) : 0;  // stages whose weights do not wait for the kernel before
+      const int ahead = c.after == AFTER_A ? min(A.stages, b1 - b0) : 0;  // stages whose weights do not wait for the kernel before
       Place q = place(b0);
       for (int i = 0; i < ahead; i++) {
         if (gm_elect()) columns(q, i);
         __syncwarp();
         next(q);
       }
-      gm_after_previous();
+      if (c.after != AFTER_NONE) gm_after_previous();
       q = place(b0);
       int s = 0, issued = 0;
       uint32_t ph = 1;
@@ -619,7 +627,8 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       }
     }
   } else if (warp >= 4) {
-    gm_after_previous();
+    if (c.after != AFTER_NONE) gm_after_previous();
+    gm_let_next();  // (not before, see k_gemm_pair)
     const int quarter = warp - 4;
     int buf = 0;
     uint32_t ph = 0;
@@ -671,6 +680,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       b = end;
     }
   }
+  if (c.after == AFTER_NONE) gm_after_previous();
   if (!ok) atomicExch(&denseErr, 202);
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -852,8 +862,6 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   const int np = KIND == GK_GATE ? 2 : 1, products = KIND == GK_PAIR ? 2 : 1;
   static OncePerDevice oncePair, onceFew;
   static int roomPair, roomFew;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = s;
   if (p.large) {
     A.wide = p.wide;
     A.stages = std::min(GP_STAGES, GP_RING / ((int)GM_OPERAND + (KIND == GK_GATE ? p.wide : p.wide / 2) * 128));
@@ -862,39 +870,28 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
     A.idesc = base | (uint32_t)c.a[0].mn << 15 | (uint32_t)c.b[0].mn << 16 | (uint32_t)(p.wide * np >> 3) << 17 | (256u >> 4) << 24;
     if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
     static_assert(GP_RING + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
-    cfg.gridDim = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
-    cfg.blockDim = 128 + gp_out(KIND) * 32;
-    cfg.dynamicSmemBytes = roomPair;
-    CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_pair<KIND, O>, A));
+    const unsigned ctas = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
+    EarlyLaunch pair(ctas, 128 + gp_out(KIND) * 32, roomPair, s, c.after != AFTER_CALL);
+    CLA_CUDA(cudaLaunchKernelEx(&pair.cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
   }
   A.nc = p.nc;
   A.stages = p.stages;
   A.ctas = p.ctas;
   A.whole = p.whole;
-  A.early = c.aLate;
   A.tilesM = (int)((c.M + A.nc - 1) / A.nc);
   A.tilesN = (int)((c.N + 127) / 128) * products;
   A.idesc = base | (uint32_t)c.b[0].mn << 15 | (uint32_t)c.a[0].mn << 16 | (uint32_t)(A.nc >> 3) << 17 | (128u >> 4) << 24;
   if (const int64_t e = all_smem(onceFew, &roomFew, c.device, k_gemm_few<KIND, O>); e < 0) return e;
   static_assert(GF_RING + 1024 <= 226 * 1024, "the ring fits");
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = c.aLate ? 1 : 0;
-  cfg.gridDim = p.ctas;
-  cfg.blockDim = GF_T;
-  cfg.dynamicSmemBytes = GF_RING + 1024;  // (all but 5 KB: CTAs of k_gemm_join may wait next to it, none with tensor memory)
-  CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_few<KIND, O>, A));
+  // (all but 5 KB: CTAs of k_gemm_join may wait next to it, none with tensor memory)
+  EarlyLaunch few(p.ctas, GF_T, GF_RING + 1024, s, c.after != AFTER_CALL);
+  CLA_CUDA(cudaLaunchKernelEx(&few.cfg, k_gemm_few<KIND, O>, A));
   if (!p.whole) {
     static OncePerDevice onceJoin;
     if (const int64_t e = onceJoin(c.device, [] { return like_products(k_gemm_join<KIND, O>); }); e < 0) return e;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)A.tilesM * A.tilesN, (unsigned)std::min<int64_t>(c.M, A.nc));
-    cfg.blockDim = 128;
-    cfg.dynamicSmemBytes = 0;
-    CLA_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_join<KIND, O>, A));
+    EarlyLaunch join(dim3((unsigned)A.tilesM * A.tilesN, (unsigned)std::min<int64_t>(c.M, A.nc)), 128, 0, s, true);
+    CLA_CUDA(cudaLaunchKernelEx(&join.cfg, k_gemm_join<KIND, O>, A));
   }
   return CLA_OK;
 }

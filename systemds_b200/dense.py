@@ -107,10 +107,10 @@ class CLALibQ8:
         px, ldx = _rows(x, "quantize, x")
         t = _type(x.dtype, "quantize")
         rows, cols = x.shape
-        q = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=x.device)[:, :cols]
+        q = torch.empty((rows, -(-cols // 128) * 128), dtype=torch.int8, device=x.device)[:, :cols]
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
         dev = x.device.index
-        check(native.lib().cla_q8_quantize_dev(t, px, ldx, rows, cols, 0, q.data_ptr(), -(-cols // 16) * 16, scale.data_ptr(), dev, _stream(dev)))
+        check(native.lib().cla_q8_quantize_dev(t, px, ldx, rows, cols, 0, q.data_ptr(), -(-cols // 128) * 128, scale.data_ptr(), dev, _stream(dev)))
         return q, scale
 
     @staticmethod
@@ -119,10 +119,10 @@ class CLALibQ8:
         pw, ldw = _rows(w, "quantize, w")
         t = _type(w.dtype, "quantize")
         rows, cols = w.shape
-        q = torch.empty((cols, -(-rows // 16) * 16), dtype=torch.int8, device=w.device)[:, :rows]
+        q = torch.empty((cols, -(-rows // 128) * 128), dtype=torch.int8, device=w.device)[:, :rows]
         scale = torch.empty(cols, dtype=torch.float32, device=w.device)
         dev = w.device.index
-        check(native.lib().cla_q8_quantize_dev(t, pw, ldw, rows, cols, 1, q.data_ptr(), -(-rows // 16) * 16, scale.data_ptr(), dev, _stream(dev)))
+        check(native.lib().cla_q8_quantize_dev(t, pw, ldw, rows, cols, 1, q.data_ptr(), -(-rows // 128) * 128, scale.data_ptr(), dev, _stream(dev)))
         return q, scale
 
     @staticmethod
