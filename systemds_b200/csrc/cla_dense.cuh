@@ -29,6 +29,30 @@ template <class T> __device__ __forceinline__ T from_f64(double v) { return (T)v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f64(double v) { return __double2bfloat16(v); }
 template <> __device__ __forceinline__ __half from_f64(double v) { return __double2half(v); }
 
+// 16 bytes of a row of T: one vector where every row starts on a 16-byte boundary (vec), else out of the two vectors that hold them (each has some of
+// the wanted bytes, so neither reaches beyond what can be read), and at a row's end element by element.
+template <class T> constexpr int DN_V = 16 / (int)sizeof(T);
+__device__ __forceinline__ uint4 load_across(const void* p) {
+  const uint4* a = (const uint4*)((uintptr_t)p & ~(uintptr_t)15);
+  const uint4 lo = a[0], hi = a[1];
+  const uint32_t words = ((uint32_t)(uintptr_t)p >> 2) & 3, bits = ((uint32_t)(uintptr_t)p & 3) * 8;
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 7; i++) w[i] = words & 1 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; i++) w[i] = words & 2 ? w[i + 2] : w[i];
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+template <class T>
+__device__ __forceinline__ void load_vec(const T* p, int n, bool vec, T (&v)[DN_V<T>]) {
+  if (n >= DN_V<T>) {
+    *(uint4*)v = vec || ((uintptr_t)p & 15) == 0 ? *(const uint4*)p : load_across(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < DN_V<T>; i++) v[i] = i < n ? p[i] : from_f32<T>(0.f);
+  }
+}
+
 // Two 16-bit values of a word, and back. (The lower bfloat16 by a byte permutation: the compiler's choice is a product, of which the words
 // of dropout leave the pipe few.)
 template <class T> __device__ __forceinline__ void from_word(uint32_t w, float& a, float& b) {
@@ -101,6 +125,39 @@ struct DropColumns {
   }
 };
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+// ---- quantisation ---------------------------------------------------------------------------------------------------
+template <class T> struct WideOf { using type = float; };
+template <> struct WideOf<double> { using type = double; };
+template <class T> __device__ __forceinline__ typename WideOf<T>::type widen(T v) { return to_f32(v); }
+template <> __device__ __forceinline__ double widen(double v) { return v; }
+
+// Magnitudes as whole numbers, which have the values' order with infinity and then NaN as the largest
+__device__ __forceinline__ unsigned long long magnitude(double v) { return (unsigned long long)__double_as_longlong(v) & 0x7fffffffffffffffull; }
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float q8_scale(unsigned long long most) { return (float)(__longlong_as_double((long long)most) / 127.0); }
+__device__ __forceinline__ float q8_scale(uint32_t most) { return __uint_as_float(most) / 127.f; }
+// The nearest whole number of x / scale, as the low byte of the result. The product with the reciprocal is off by three roundings of a value
+// below 128: unless it comes that near to a half, where the quotient itself decides, both have the same nearest whole number. So the product
+// is taken first, rounded by adding 1.5 times the power of two whose unit is 1, and whether some value came near is asked once
+// for many of them: the quotients are then taken for all.
+template <class W> struct Q8Row {
+  W scale, inv;
+  bool some, quick;  // a scale to divide by; whose reciprocal is finite
+  __device__ __forceinline__ explicit Q8Row(float s)
+      : scale((W)s), inv((W)1 / (W)s), some(s > 0.f && s < INFINITY), quick(s >= 0x1p-126f && s < INFINITY) {}
+  __device__ __forceinline__ uint32_t product(W x, bool& near) const {
+    constexpr W MAGIC = sizeof(W) == 8 ? (W)0x1.8p52 : (W)0x1.8p23;
+    constexpr W FAR = (W)0.5 - (sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-15);  // above 3/2 of 127 roundings of 2^-52, 2^-23
+    const W t = x * inv, r = t + MAGIC;
+    near |= !(fabs(t - (r - MAGIC)) <= FAR);
+    if constexpr (sizeof(W) == 8) return (uint32_t)__double2loint(r);
+    else return __float_as_uint(r);
+  }
+};
+template <class W> __device__ __noinline__ uint32_t q8_quotient(W x, W scale, bool some) {
+  return some ? (uint32_t)(int)fmin((W)127, fmax((W)-127, rint(x / scale))) : 0u;
+}
 
 // ---- the activation, in FP32 ------------------------------------------------------------------------------------------
 // With the fast exponential and quotient: off by some units of 2^-23, under 2^-20 of the value where |g| < 10 (beyond, a unit more for each
@@ -178,6 +235,7 @@ struct GemmCall {
   bool split = true;      // whether the depth may be split (gemm_workspace() is 0 if not)
   void* parts = nullptr;  // gemm_workspace() bytes, 256-byte aligned
   int after = 0;          // AFTER_*
+  bool quantize = false;  // Q8: a holds rows of outType, which the product quantises itself (gemm_quantizes())
 };
 // What a kernel has to do with the one that the same call has launched just before it (which itself came after all that the stream held). The kernel may
 // then start while that one still runs, and waits for its end where it says; the one before lets it by gm_let_next().
@@ -203,6 +261,8 @@ struct EarlyLaunch {
   }
   EarlyLaunch(const EarlyLaunch&) = delete;
 };
+// Whether a product quantises so many rows itself, of the type that the results have
+bool gemm_quantizes(int64_t M, int64_t K, int type);
 int64_t gemm_workspace(const GemmCall& c);  // goes by the sizes, the types and which index is contiguous
 int64_t launch_gemm(const GemmCall& c, cudaStream_t s);
 int64_t dense_status(int device);  // the self-check word of the product kernels, cleared

@@ -459,9 +459,9 @@ __host__ __device__ inline int gf_start(int i, int ctas, int n, int nk, bool who
 }
 
 template <int KIND, class O>
-__device__ __forceinline__ void gm_finish(const GemmCall& c, int which, int64_t m, int64_t n, uint32_t v0, uint32_t v1, float sb) {
+__device__ __forceinline__ void gm_finish(const GemmCall& c, int which, int64_t m, int64_t n, uint32_t v0, uint32_t v1, float sa, float sb) {
   if constexpr (KIND == GK_Q8) {
-    ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<KIND, O>(c, (int32_t)v0, c.aScale[m], sb);
+    ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<KIND, O>(c, (int32_t)v0, sa, sb);
   } else if constexpr (KIND == GK_GATE) {
     const float g = __uint_as_float(v0), u = __uint_as_float(v1);
     float h = act_value(c.act, g) * u;
@@ -485,10 +485,19 @@ __device__ __forceinline__ void gf_tile(const GemmArgs& A, int t, int& which, in
   n0 = (which ? tn - A.tilesN / 2 : tn) * 128;
 }
 
-template <int KIND, class O>
+// The scales of rows that the product quantises itself: behind the parts of the sums
+__host__ __device__ inline int64_t gf_parts_bytes(int ctas, int np, int nc) { return (int64_t)ctas * 2 * np * nc * 128 * 4; }
+__device__ __forceinline__ float* gf_scales(const GemmArgs& A) { return (float*)((char*)A.c.parts + gf_parts_bytes(A.ctas, 1, A.nc)); }
+
+// X: the type of rows that the kernel quantises itself (void: they come in 8 bits), at most 16. The warps that write the results first find
+// the rows' scales, every CTA for itself, and bring a stage's share of the rows where else the copying warp does: no kernel before, no
+// copy of the rows in memory. One row of 4096 values: 1 us until the first stage, next to 4 us and a launch of the quantisation's own.
+template <int KIND, class O, class X>
 __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ GemmArgs A) {
-  constexpr bool I8 = KIND == GK_Q8;
+  constexpr bool I8 = KIND == GK_Q8, OWN = !std::is_void_v<X>;
   constexpr int NP = KIND == GK_GATE ? 2 : 1;
+  __shared__ float ownScale[16];
+  __shared__ unsigned long long ownMost[16];
   extern __shared__ __align__(1024) unsigned char gmsm[];
   __shared__ __align__(8) uint64_t full[GF_STAGES], empty[GF_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
@@ -504,9 +513,10 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (OWN && threadIdx.x >= 128 && threadIdx.x < 144) ownMost[threadIdx.x - 128] = 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < A.stages; i++) {
-      gm_init(gm_smem(full + i), 1);
+      gm_init(gm_smem(full + i), OWN ? 2 : 1);  // the copies, and the warp that quantises
       gm_init(gm_smem(empty + i), 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -546,7 +556,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       auto columns = [&](const Place& q, int s) {
         const int seg = KIND == GK_SUM && q.kb >= A.kBlocks, k0 = (q.kb - seg * A.kBlocks) * A.depth;
         const uint32_t bar = fullAt + s * 8, dl = smem + s * stage;
-        gm_expect(bar, stage);
+        gm_expect(bar, OWN ? NP * GM_OPERAND : stage);
 #pragma unroll
         for (int p = 0; p < NP; p++) {
           const CUtensorMap* ml = A.b + (KIND == GK_GATE ? p : KIND == GK_SUM ? seg : q.which);
@@ -585,7 +595,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
         if (!ok) break;
         if (gm_elect()) {
           if (fresh) columns(q, s);
-          rows(q, s);
+          if (!OWN) rows(q, s);
         }
         __syncwarp();
         next(q);
@@ -630,14 +640,73 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
     if (c.after != AFTER_NONE) gm_after_previous();
     gm_let_next();  // (not before, see k_gemm_pair)
     const int quarter = warp - 4;
-    int buf = 0;
-    uint32_t ph = 0;
+    int buf = 0, s = 0, turn = quarter;  // (the warps quantise stages in turn)
+    uint32_t ph = 0, phStage = 1;
+    using V = std::conditional_t<OWN, X, float>;
+    using W = typename WideOf<V>::type;
+    constexpr int P = DN_V<V>;
+    if constexpr (OWN) {
+      for (int r = 0; r < c.M; r++) {
+        const V* p = (const V*)c.a[0].p + r * c.a[0].ld;
+        decltype(magnitude(W())) most = 0;
+#pragma unroll 4
+        for (int k = (threadIdx.x - 128) * P; k < c.K; k += 128 * P) {
+          alignas(16) V v[P];
+          load_vec(p + k, (int)min((int64_t)P, c.K - k), false, v);
+#pragma unroll
+          for (int i = 0; i < P; i++) most = max(most, magnitude(widen(v[i])));
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        if (lane == 0) atomicMax(ownMost + r, (unsigned long long)most);
+      }
+      gm_group_sync(1, 128);
+      if (const int r = threadIdx.x - 128; r < c.M) {
+        ownScale[r] = q8_scale((decltype(magnitude(W())))ownMost[r]);
+        if (!A.whole && blockIdx.x == 0) gf_scales(A)[r] = ownScale[r];
+      }
+      gm_group_sync(1, 128);
+    }
     for (int b = b0; b < b1;) {
       const int t = b / nk, end = min(b1, (t + 1) * nk);
-      const bool mine = b == t * nk && end == (t + 1) * nk;
+      const bool mine = b == t * nk && end == (t + 1) * nk, head = b == b0;
       int which, n0;
       int64_t m0;
       gf_tile<KIND>(A, t, which, n0, m0);
+      if constexpr (OWN) {
+        for (int kb = b - t * nk; b < end; b++, kb++) {
+          if (turn == 0) {
+            ok = gm_wait_all(emptyAt + s * 8, phStage);
+            if (!ok) break;
+            for (int row = 0; row < c.M; row++) {  // four values a lane
+              const int k0 = kb * 128 + lane * 4;
+              const V* x = (const V*)c.a[0].p + row * c.a[0].ld + k0;
+              const Q8Row<W> q8(ownScale[row]);
+              W v[4];
+              uint32_t o[4];
+              bool near = !q8.quick;
+#pragma unroll
+              for (int j = 0; j < 4; j++) v[j] = k0 + j < c.K ? widen(x[j]) : (W)0;
+#pragma unroll
+              for (int j = 0; j < 4; j++) o[j] = q8.product(v[j], near);
+              if (near) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = q8_quotient(v[j], q8.scale, q8.some);
+              }
+              const uint32_t w = __byte_perm(__byte_perm(o[0], o[1], 0x0040), __byte_perm(o[2], o[3], 0x0040), 0x5410);
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem + s * stage + NP * GM_OPERAND + row * 128 + (((lane >> 2) ^ (row & 7)) * 16) + (lane & 3) * 4),
+                           "r"(w)
+                           : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(fullAt + s * 8) : "memory");
+          }
+          turn = (turn + 3) & 3;
+          if (++s == A.stages) s = 0, phStage ^= 1;
+        }
+        if (!ok) break;
+      }
       if (!none) {
         ok = gm_wait(gm_smem(sumFull + buf), ph);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -647,7 +716,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
       const int64_t col = n0 + quarter * 32 + lane;  // the lane's column of the result
       const float sb = I8 && col < c.N ? c.bScale[col] : 0.f;
       const uint32_t at = tmem + buf * 256 + ((uint32_t)quarter << 21);
-      uint32_t* room = (uint32_t*)c.parts + ((int64_t)blockIdx.x * 2 + (b == b0 ? 0 : 1)) * NP * A.nc * 128 + quarter * 32 + lane;
+      uint32_t* room = (uint32_t*)c.parts + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * NP * A.nc * 128 + quarter * 32 + lane;
 #pragma unroll 1
       for (int r = 0; r < rows; r += 16) {
         uint32_t v[NP * 16];
@@ -663,7 +732,7 @@ __global__ void __launch_bounds__(GF_T, 1) k_gemm_few(const __grid_constant__ Ge
           for (int i = 0; i < 16; i++) {
             if (r + i >= rows) break;
             if (mine) {
-              gm_finish<KIND, O>(c, which, m0 + r + i, col, v[i], v[16 * (NP - 1) + i], sb);
+              gm_finish<KIND, O>(c, which, m0 + r + i, col, v[i], v[16 * (NP - 1) + i], OWN ? ownScale[r + i] : I8 ? c.aScale[m0 + r + i] : 0.f, sb);
             } else {
 #pragma unroll
               for (int p = 0; p < NP; p++) room[(p * A.nc + r + i) * 128] = v[16 * p + i];
@@ -710,6 +779,7 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
   const int64_t col = n0 + threadIdx.x;
   if (col >= c.N) return;
   const float sb = I8 ? c.bScale[col] : 0.f;
+  const float* aScale = c.quantize ? gf_scales(A) : c.aScale;
   // the first CTA's range starts in this tile or before it, the others' in it
   const int64_t room = (int64_t)NP * A.nc * 128;
   const int64_t head = (int64_t)first * 2 + (gf_start(first, A.ctas, n, nk, false) < t * nk);
@@ -726,7 +796,7 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
 #pragma unroll
         for (int p = 0; p < NP; p++) f[p] += __uint_as_float(at[q * 2 * room + p * A.nc * 128]);
     }
-    gm_finish<KIND, O>(c, which, m0 + r, col, I8 ? u : __float_as_uint(f[0]), __float_as_uint(f[NP - 1]), sb);
+    gm_finish<KIND, O>(c, which, m0 + r, col, I8 ? u : __float_as_uint(f[0]), __float_as_uint(f[NP - 1]), I8 ? aScale[m0 + r] : 0.f, sb);
   }
 }
 
@@ -793,6 +863,8 @@ static int gemm_blocks(const GemmCall& c) {  // stages of a segment
   const int depth = 128 / type_bytes(c.type);
   return (int)((c.K + depth - 1) / depth);
 }
+bool gemm_quantizes(int64_t M, int64_t K, int type) { return M <= 16 && K > 0 && M * K * type_bytes(type) <= 32 << 10; }
+
 static GemmPlan gemm_plan(const GemmCall& c) {
   GemmPlan best;
   const int nk = gemm_blocks(c) * (c.kind == GK_SUM ? 2 : 1);
@@ -804,7 +876,7 @@ static GemmPlan gemm_plan(const GemmCall& c) {
   // k_gemm_pair: a stage takes 0.17 us (waits and issue) or its products' time, 4 clocks a column that a CTA brings, at 1.85 GHz; a tile's results
   // leave in 12 ns a column while the next tile's come
   // (32 rows and fewer leave its copies of them nearly empty, which take up to twice the time: not for deep products of so few)
-  for (int wide = 256 / np; wide >= 64 && nk > 0 && (c.M > 32 || nk <= 8); wide /= 2) {
+  for (int wide = 256 / np; wide >= 64 && nk > 0 && (c.M > 32 || nk <= 8) && !c.quantize; wide /= 2) {
     const int mine = np == 2 ? wide : wide / 2;
     if (c.b[0].mn && mine < 64) break;
     const int64_t tiles = ceil_div(c.M, 256) * ceil_div(c.N, wide) * products, turns = ceil_div(tiles, GM_SMS / 2);
@@ -827,7 +899,7 @@ static GemmPlan gemm_plan(const GemmCall& c) {
       const int64_t ctas = whole ? std::min<int64_t>(tiles, GM_SMS) : std::min<int64_t>(GM_SMS, tiles * ceil_div(nk, 4));
       const double out = 0.2 + std::min<int64_t>(nc, c.M) * np * (whole ? 0.05 : 0.01);
       const double chain = whole ? ceil_div(tiles, ctas) * std::max(nk * step, out) : ceil_div(n, ctas) * step;
-      const double join = 3.0 + (double)tiles * std::min<int64_t>(nc, c.M) * np * 512 * 2.5 / 4.0e6;
+      const double join = 4.0 + (double)tiles * std::min<int64_t>(nc, c.M) * np * 512 * 2.5 / 4.0e6;
       const double t = 5.5 + std::max({memory, chain, (double)n * stage / 10.0e6}) + out + (whole ? 0.0 : join);
       if (t >= best.us) continue;
       best.large = false, best.nc = nc, best.ctas = (int)ctas, best.whole = whole, best.us = t;
@@ -839,7 +911,7 @@ static GemmPlan gemm_plan(const GemmCall& c) {
 int64_t gemm_workspace(const GemmCall& c) {
   if (c.M == 0 || c.N == 0) return 0;
   const GemmPlan p = gemm_plan(c);
-  return p.large || p.whole ? 0 : (int64_t)p.ctas * 2 * (c.kind == GK_GATE ? 2 : 1) * p.nc * 128 * 4;
+  return p.large || p.whole ? 0 : gf_parts_bytes(p.ctas, c.kind == GK_GATE ? 2 : 1, p.nc) + 64;
 }
 
 template <int KIND, class O>
@@ -854,14 +926,14 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   if (A.kBlocks > 0)
     for (int i = 0; i < 2; i++) {
       const int boxB = !p.large ? 128 : KIND == GK_GATE ? p.wide : p.wide / 2;
-      if (i == 0 || KIND == GK_SUM)
+      if ((i == 0 || KIND == GK_SUM) && !c.quantize)
         if (const int64_t rc = operand_map(A.a[i], c.a[i], c.type, c.M, c.K, p.large ? 128 : p.nc); rc < 0) return rc;
       if (i == 0 || KIND != GK_Q8)
         if (const int64_t rc = operand_map(A.b[i], c.b[i], c.type, c.N, c.K, boxB); rc < 0) return rc;
     }
   const int np = KIND == GK_GATE ? 2 : 1, products = KIND == GK_PAIR ? 2 : 1;
   static OncePerDevice oncePair, onceFew;
-  static int roomPair, roomFew;
+  static int roomPair;
   if (p.large) {
     A.wide = p.wide;
     A.stages = std::min(GP_STAGES, GP_RING / ((int)GM_OPERAND + (KIND == GK_GATE ? p.wide : p.wide / 2) * 128));
@@ -882,11 +954,23 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   A.tilesM = (int)((c.M + A.nc - 1) / A.nc);
   A.tilesN = (int)((c.N + 127) / 128) * products;
   A.idesc = base | (uint32_t)c.b[0].mn << 15 | (uint32_t)c.a[0].mn << 16 | (uint32_t)(A.nc >> 3) << 17 | (128u >> 4) << 24;
-  if (const int64_t e = all_smem(onceFew, &roomFew, c.device, k_gemm_few<KIND, O>); e < 0) return e;
   static_assert(GF_RING + 1024 <= 226 * 1024, "the ring fits");
-  // (all but 5 KB: CTAs of k_gemm_join may wait next to it, none with tensor memory)
-  EarlyLaunch few(p.ctas, GF_T, GF_RING + 1024, s, c.after != AFTER_CALL);
-  CLA_CUDA(cudaLaunchKernelEx(&few.cfg, k_gemm_few<KIND, O>, A));
+  const auto few = [&](auto kernel, OncePerDevice& once) -> int64_t {
+    int room;
+    if (const int64_t e = all_smem(once, &room, c.device, kernel); e < 0) return e;
+    // (all but 5 KB: CTAs of k_gemm_join may wait next to it, none with tensor memory)
+    EarlyLaunch l(p.ctas, GF_T, GF_RING + 1024, s, c.after != AFTER_CALL);
+    CLA_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, A));
+    return CLA_OK;
+  };
+  int64_t rc;
+  if constexpr (KIND == GK_Q8) {
+    static OncePerDevice onceOwn;
+    rc = c.quantize ? few(k_gemm_few<KIND, O, O>, onceOwn) : few(k_gemm_few<KIND, O, void>, onceFew);
+  } else {
+    rc = few(k_gemm_few<KIND, O, void>, onceFew);
+  }
+  if (rc < 0) return rc;
   if (!p.whole) {
     static OncePerDevice onceJoin;
     if (const int64_t e = onceJoin(c.device, [] { return like_products(k_gemm_join<KIND, O>); }); e < 0) return e;

@@ -144,9 +144,11 @@ def test_q8_product(M, N, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("M,N,K", [(1, 64, 4096), (5, 77, 501), (200, 130, 333), (2, 3, 0)])
-def test_q8_linear(M, N, K, dtype):
-    x, w = normal(M, K, dtype, 3), normal(K, N, torch.float32, 4)
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 4096), (5, 77, 501), (200, 130, 333), (2, 3, 0), (1, 20000, 300), (16, 130, 256), (1, 300, 16), (3, 129, 1001),
+                                   (1, 2000, 8192), (17, 40, 200)])
+def test_q8_linear(M, N, K, dtype, pad):
+    x, w = normal(M, K, dtype, 3, pad=pad), normal(K, N, torch.float32, 4)
     b, sb = CLALibQ8.quantizeCols(w)
     qa, sa = ref.quantize(x)
     want = q8_want(qa, sa, b.cpu().numpy(), sb.cpu().numpy())
