@@ -418,14 +418,15 @@ class CLALibDecompress:
         """Rows ``[row0, row0 + rows)`` as a torch tensor on the block's device, rounded once to ``dtype`` (float64, float32, bfloat16,
         float16): what the dense operators take of a compressed block."""
         import torch
-        from .dense import _result, _rows, _stream, _type, _workspace
+        from .dense import _rows, _stream, _type, _workspace
         h, t = cmb.handle(), _type(dtype, "rows of a block")
-        dev = torch.device("cuda", cmb.device)
         if row0 < 0 or rows < 0 or row0 + rows > cmb.rlen:
             raise native.CLAError(-4, "rows of a block: outside the matrix")
-        y = _result(out, (rows, cmb.clen), dtype, dev, "rows of a block, out")
-        py, ldo = _rows(y, "rows of a block, out", dtype, dev)
+        y = torch.empty((rows, cmb.clen), dtype=dtype, device=torch.device("cuda", cmb.device)) if out is None else out
+        if tuple(y.shape) != (rows, cmb.clen):
+            raise native.CLAError(-4, "rows of a block, out: another shape")
+        py, ldo = _rows(y, "rows of a block, out", dtype, cmb.device)
         n = check(native.lib().cla_rows_workspace(h, rows, t))
-        work = _workspace(n, dev)
-        check(native.lib().cla_decompress_rows_dev(h, row0, rows, t, py, ldo, work.data_ptr() if n else None, n, _stream(cmb.device)))
+        work = _workspace(n, y.device)
+        check(native.lib().cla_decompress_rows_dev(h, row0, rows, t, py, ldo, work.data_ptr(), n, _stream(cmb.device)))
         return y

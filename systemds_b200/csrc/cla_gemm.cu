@@ -865,7 +865,7 @@ static int gemm_blocks(const GemmCall& c) {  // stages of a segment
 }
 bool gemm_quantizes(int64_t M, int64_t K, int type) { return M <= 16 && K > 0 && M * K * type_bytes(type) <= 32 << 10; }
 
-static GemmPlan gemm_plan(const GemmCall& c) {
+static GemmPlan find_plan(const GemmCall& c) {
   GemmPlan best;
   const int nk = gemm_blocks(c) * (c.kind == GK_SUM ? 2 : 1);
   const int np = c.kind == GK_GATE ? 2 : 1, products = c.kind == GK_PAIR ? 2 : 1;
@@ -907,6 +907,19 @@ static GemmPlan gemm_plan(const GemmCall& c) {
     }
   }
   return best;
+}
+// A call asks for its plan three times, and programs ask for the same sizes again: the last few are kept, by all that they depend on
+static GemmPlan gemm_plan(const GemmCall& c) {
+  struct Kept {
+    int64_t M = -1, N, K;
+    int how;
+    GemmPlan plan;
+  };
+  static thread_local Kept kept[16];
+  const int how = (int)c.kind * 64 + (c.type == CLA_T_I8) * 32 + c.split * 16 + c.quantize * 8 + c.a[0].mn * 4 + c.b[0].mn * 2;
+  Kept& k = kept[(uint64_t)(c.M * 31 + c.N * 7 + c.K * 3 + how) % 16];
+  if (k.M != c.M || k.N != c.N || k.K != c.K || k.how != how) k = {c.M, c.N, c.K, how, find_plan(c)};
+  return k.plan;
 }
 int64_t gemm_workspace(const GemmCall& c) {
   if (c.M == 0 || c.N == 0) return 0;

@@ -30,18 +30,22 @@ def _fail(code: int, msg: str):
     raise CLAError(code, msg)
 
 
-def _rows(t, what: str, dtype=None, device=None):
+def _rows(t, what: str, dtype=None, device: int = -1):
     """Address and row stride of a device matrix whose rows have adjacent elements."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _fail(-2, f"{what}: a CUDA tensor is needed")
-    if t.dim() != 2:
+    try:
+        dev = t.get_device()
+        rows, cols = t.shape
+        s0, s1 = t.stride()
+    except (AttributeError, ValueError, RuntimeError):
+        if not isinstance(t, torch.Tensor):
+            _fail(-2, f"{what}: a CUDA tensor is needed")
         _fail(-4, f"{what}: two dimensions are needed")
+    if dev < 0:
+        _fail(-2, f"{what}: a CUDA tensor is needed")
     if dtype is not None and t.dtype != dtype:
         _fail(-3, f"{what}: type {t.dtype}, expected {dtype}")
-    if device is not None and t.device != device:
+    if device >= 0 and dev != device:
         _fail(-2, f"{what}: on another device than the first operand")
-    rows, cols = t.shape
-    s0, s1 = t.stride()
     if s1 != 1 and cols > 1:
         _fail(-3, f"{what}: the elements of a row must be adjacent")
     if rows <= 1:
@@ -51,17 +55,18 @@ def _rows(t, what: str, dtype=None, device=None):
     return t.data_ptr(), s0
 
 
-def _vector(t, what: str, n: int, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device:
+def _vector(t, what: str, n: int, device: int):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != device:
         _fail(-2, f"{what}: float32 on the operands' device is needed")
     if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
         _fail(-4, f"{what}: {n} adjacent values are needed")
     return t.data_ptr()
 
 
-def _result(out, shape, dtype, device, what: str):
+def _result(out, shape, dtype, like, what: str):
+    """``out``, or a new tensor on the device of ``like``."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if like.dtype == dtype else torch.empty(shape, dtype=dtype, device=like.device)
     if tuple(out.shape) != tuple(shape):
         _fail(-4, f"{what}: shape {tuple(out.shape)}, expected {tuple(shape)}")
     return out
@@ -75,7 +80,7 @@ def _type(dtype, what: str) -> int:
 
 
 def _workspace(n: int, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _drop(p, seed, step, row0) -> native.cla_drop:
@@ -91,12 +96,14 @@ class CLALibDropout:
         ``seed`` and counter ``(c / 4, row0 + r, step)`` decides about element (r, c): applied to the output's gradient with the same
         ``(seed, step)`` it is the backward pass, and a shard of rows passes its first row as ``row0``. ``out`` may be ``x``."""
         px, ldx = _rows(x, "dropout, x")
-        t = _type(x.dtype, "dropout")
-        y = _result(out, x.shape, x.dtype, x.device, "dropout, out")
-        py, ldy = _rows(y, "dropout, out", x.dtype, x.device)
+        dtype = x.dtype
+        t = _type(dtype, "dropout")
+        dev = x.get_device()
+        rows, cols = shape = x.shape
+        y = _result(out, shape, dtype, x, "dropout, out")
+        py, ldy = (y.data_ptr(), cols) if out is None else _rows(y, "dropout, out", dtype, dev)
         d = _drop(p, seed, step, row0)
-        dev = x.device.index
-        check(native.lib().cla_dropout_dev(t, px, ldx, x.shape[0], x.shape[1], py, ldy, C.byref(d), dev, _stream(dev)))
+        check(native.lib().cla_dropout_dev(t, px, ldx, rows, cols, py, ldy, C.byref(d), dev, _stream(dev)))
         return y
 
 
@@ -109,7 +116,7 @@ class CLALibQ8:
         rows, cols = x.shape
         q = torch.empty((rows, -(-cols // 128) * 128), dtype=torch.int8, device=x.device)[:, :cols]
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-        dev = x.device.index
+        dev = x.get_device()
         check(native.lib().cla_q8_quantize_dev(t, px, ldx, rows, cols, 0, q.data_ptr(), -(-cols // 128) * 128, scale.data_ptr(), dev, _stream(dev)))
         return q, scale
 
@@ -121,30 +128,30 @@ class CLALibQ8:
         rows, cols = w.shape
         q = torch.empty((cols, -(-rows // 128) * 128), dtype=torch.int8, device=w.device)[:, :rows]
         scale = torch.empty(cols, dtype=torch.float32, device=w.device)
-        dev = w.device.index
+        dev = w.get_device()
         check(native.lib().cla_q8_quantize_dev(t, pw, ldw, rows, cols, 1, q.data_ptr(), -(-rows // 128) * 128, scale.data_ptr(), dev, _stream(dev)))
         return q, scale
 
     @staticmethod
     def _mm(a, aType, aScale, b, bScale, dtype, out):
         pa, lda = _rows(a, "8-bit product, a")
-        dev = a.device
+        dev = a.get_device()
         pb, ldb = _rows(b, "8-bit product, b", torch.int8, dev)
         M, K = a.shape
-        N = b.shape[0]
-        if b.shape[1] != K:
+        N, inner = b.shape
+        if inner != K:
             _fail(-4, "8-bit product: inner dimensions do not match")
-        y = _result(out, (M, N), dtype, dev, "8-bit product, out")
-        py, ldo = _rows(y, "8-bit product, out", dtype, dev)
+        y = _result(out, (M, N), dtype, a, "8-bit product, out")
+        py, ldo = (y.data_ptr(), N) if out is None else _rows(y, "8-bit product, out", dtype, dev)
         L = native.lib()
         args = native.cla_q8(M, N, K, pa, lda, None if aScale is None else _vector(aScale, "8-bit product, scales of a", M, dev), pb, ldb,
-                             _vector(bScale, "8-bit product, scales of b", N, dev), py, ldo, None, 0, aType, _type(dtype, "8-bit product"), dev.index)
+                             _vector(bScale, "8-bit product, scales of b", N, dev), py, ldo, None, 0, aType, _type(dtype, "8-bit product"), dev)
         ref = C.byref(args)
         n = check(L.cla_q8_workspace(ref))
         if n:
-            work = _workspace(n, dev)
+            work = _workspace(n, a.device)
             args.work, args.workBytes = work.data_ptr(), n
-        check(L.cla_q8_mm_dev(ref, _stream(dev.index)))
+        check(L.cla_q8_mm_dev(ref, _stream(dev)))
         return y
 
     @staticmethod
@@ -169,19 +176,18 @@ class CLALibQ8:
     def rightMultByMatrix(m1, b, bScale, dtype=torch.float64, out=None):
         """``m1 %*% W`` for a compressed block ``m1`` and W in 8 bits, as ``linear`` of its rows (beside
         ``CLALibRightMultBy.rightMultByMatrix``, in FP64). The result is a tensor on the block's device."""
-        dev = torch.device("cuda", m1.device if m1.device is not None else 0)
+        dev = m1.device if m1.device is not None else 0
         pb, ldb = _rows(b, "8-bit right product, b", torch.int8, dev)
         N = b.shape[0]
         if b.shape[1] != m1.clen:
             _fail(-4, "8-bit right product: inner dimensions do not match")
         ps = _vector(bScale, "8-bit right product, scales", N, dev)
-        y = _result(out, (m1.rlen, N), dtype, dev, "8-bit right product, out")
+        y = _result(out, (m1.rlen, N), dtype, b, "8-bit right product, out")
         py, ldo = _rows(y, "8-bit right product, out", dtype, dev)
         L = native.lib()
         n = check(L.cla_q8_rmm_workspace(m1.handle(), N))
-        work = _workspace(n, dev)
-        check(L.cla_q8_rmm_dev(m1.handle(), pb, ldb, ps, N, _type(dtype, "8-bit right product"), py, ldo, work.data_ptr() if n else None, n,
-                               _stream(dev.index)))
+        work = _workspace(n, b.device)
+        check(L.cla_q8_rmm_dev(m1.handle(), pb, ldb, ps, N, _type(dtype, "8-bit right product"), py, ldo, work.data_ptr(), n, _stream(dev)))
         return y
 
 
@@ -192,6 +198,7 @@ class CLALibGated:
     @staticmethod
     def _args(x, wGate, wUp, act, p, seed, step, row0):
         px, ldx = _rows(x, "gated block, x")
+        dev = x.get_device()
         if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
             _fail(-3, f"gated block: unsupported type {x.dtype} (bfloat16 and float16)")
         a = ACTS.get(act)
@@ -206,11 +213,11 @@ class CLALibGated:
             _fail(-4, "gated block: weights must both be [columns of x, F]")
         if wGate.stride(1) != 1 and wGate.shape[1] > 1:
             wGate, wUp, trans = wGate.t(), wUp.t(), 1
-        pg, ldg = _rows(wGate, "gated block, wGate", x.dtype, x.device)
-        pu, ldu = _rows(wUp, "gated block, wUp", x.dtype, x.device)
+        pg, ldg = _rows(wGate, "gated block, wGate", x.dtype, dev)
+        pu, ldu = _rows(wUp, "gated block, wUp", x.dtype, dev)
         c = native.cla_gated(M, D, wGate.shape[0] if trans else wGate.shape[1], px, pg, pu, ldx, ldg, ldu)
         c.drop = _drop(p, seed, step, row0)
-        c.type, c.act, c.wTrans, c.device = TYPES[x.dtype], a, trans, x.device.index
+        c.type, c.act, c.wTrans, c.device = TYPES[x.dtype], a, trans, dev
         return c
 
     @staticmethod
@@ -227,10 +234,10 @@ class CLALibGated:
         """``H`` [rows of x, F]; with ``save`` also ``X Wg`` and ``X Wu``, which ``backward`` takes. ``p``, ``seed``, ``step``, ``row0``:
         dropout of H, as ``CLALibDropout.apply``."""
         c = CLALibGated._args(x, wGate, wUp, act, p, seed, step, row0)
-        h = _result(out, (c.M, c.F), x.dtype, x.device, "gated block, out")
-        c.h, c.ldh = _rows(h, "gated block, out", x.dtype, x.device)
+        h = _result(out, (c.M, c.F), x.dtype, x, "gated block, out")
+        c.h, c.ldh = _rows(h, "gated block, out", x.dtype, c.device)
         if save:
-            g, u = torch.empty((c.M, c.F), dtype=x.dtype, device=x.device), torch.empty((c.M, c.F), dtype=x.dtype, device=x.device)
+            g, u = x.new_empty((c.M, c.F)), x.new_empty((c.M, c.F))
             c.g, c.u = g.data_ptr(), u.data_ptr()
             c.ldg = c.ldu = c.F
         CLALibGated._run(c, 0, x.device)
@@ -242,7 +249,7 @@ class CLALibGated:
         """``(dX, dWg, dWu)`` from the gradient of H and what ``forward(..., save=True)`` gave, with the same activation and dropout
         arguments; dX or the weights' gradients are None where not needed."""
         c = CLALibGated._args(x, wGate, wUp, act, p, seed, step, row0)
-        dev = x.device
+        dev = c.device
         for t, what in ((dH, "dH"), (g, "g"), (u, "u")):
             if not isinstance(t, torch.Tensor) or tuple(t.shape) != (c.M, c.F):
                 _fail(-4, f"gated block, {what}: expected [{c.M}, {c.F}]")
@@ -251,13 +258,13 @@ class CLALibGated:
         c.u, c.ldu = _rows(u, "gated block, u", x.dtype, dev)
         dx = dwg = dwu = None
         if needX:
-            dx = torch.empty((c.M, c.D), dtype=x.dtype, device=dev)
+            dx = x.new_empty((c.M, c.D))
             c.dx, c.lddx = dx.data_ptr(), c.D
         if needW:
-            dwg, dwu = torch.empty((c.D, c.F), dtype=x.dtype, device=dev), torch.empty((c.D, c.F), dtype=x.dtype, device=dev)
+            dwg, dwu = x.new_empty((c.D, c.F)), x.new_empty((c.D, c.F))
             c.dwg, c.dwu = dwg.data_ptr(), dwu.data_ptr()
             c.lddwg = c.lddwu = c.F
-        CLALibGated._run(c, 1, dev)
+        CLALibGated._run(c, 1, x.device)
         return dx, dwg, dwu
 
 
