@@ -61,9 +61,9 @@ def sum_bound(K, magnitudes):
 ACT_REL, SLOPE_ABS = 2.0 ** -20, 2.0 ** -18
 
 
-def gated(x, wg, wu, name, factors, dtype):
+def gated(x, wg, wu, name, factors, dtype, device="cpu"):
     """h, g, u and the bounds of their errors."""
-    x, wg, wu = x.double().cpu(), wg.double().cpu(), wu.double().cpu()
+    x, wg, wu = (t.double().to(device) for t in (x, wg, wu))
     K = x.shape[1]
     g, u = x @ wg, x @ wu
     eg, eu = sum_bound(K, x.abs() @ wg.abs()), sum_bound(K, x.abs() @ wu.abs())
@@ -75,9 +75,9 @@ def gated(x, wg, wu, name, factors, dtype):
     return (h, g, u), tuple(e + hs * (v.abs() + e) + t for v, e in ((h, eh), (g, eg), (u, eu)))
 
 
-def gated_grads(dh, x, wg, wu, g, u, name, factors, dtype):
+def gated_grads(dh, x, wg, wu, g, u, name, factors, dtype, device="cpu"):
     """dx, dwg, dwu and the bounds of their errors: dg and du are rounded to the type, then summed in FP32 and rounded again."""
-    dh, x, wg, wu, g, u = (t.double().cpu() for t in (dh, x, wg, wu, g, u))
+    dh, x, wg, wu, g, u = (t.double().to(device) for t in (dh, x, wg, wu, g, u))
     hs, t = half_step(dtype), tiny(dtype)
     d = dh * factors
     a, s = act(name, g), act_slope(name, g)
@@ -110,7 +110,7 @@ def quantize(x):
 
 
 def close(got, want, bound, what=""):
-    got = got.double().cpu()
+    got = got.double().to(want.device)
     assert got.shape == want.shape, what
     bad = ~((got - want).abs() <= bound)
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() / bound)[bad].max()):.3g} times the bound"

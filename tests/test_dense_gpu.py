@@ -288,13 +288,83 @@ def test_gated_values_that_are_not_finite_stay_in_their_rows():
     assert torch.equal(CLALibGated.forward(x, wg, wu)[rest], clean[rest])
 
 
+MANY = [(2500, 1100, 3001), (40, 5000, 9000), (300, 6000, 260), (1, 3000, 20000), (700, 2050, 1800), (32, 8200, 520)]
+
+
+@pytest.mark.parametrize("M,D,F", MANY)
+@pytest.mark.parametrize("dtype", HALVES)
+def test_gated_of_many_tiles(M, D, F, dtype):
+    """More tiles than SMs, depths that several CTAs share, and sums over many stages (the 64-bit forms on the GPU)."""
+    x, wg, wu = gated_inputs(M, D, F, dtype)
+    f = ref.drop_factors(M, F, 0.1, 21, 5).cuda()
+    want, bound = ref.gated(x, wg, wu, "silu", f, dtype, "cuda")
+    got = CLALibGated.forward(x, wg, wu, "silu", p=0.1, seed=21, step=5, save=True)
+    for name, y, v, e in zip("hgu", got, want, bound):
+        ref.close(y, v, e, name)
+    dh = normal(M, F, dtype, 13)
+    want, bound = ref.gated_grads(dh, x, wg, wu, got[1], got[2], "silu", f, dtype, "cuda")
+    grads = CLALibGated.backward(dh, x, wg, wu, got[1], got[2], "silu", p=0.1, seed=21, step=5)
+    for name, y, v, e in zip(("dx", "dwg", "dwu"), grads, want, bound):
+        ref.close(y, v, e, name)
+    for _ in range(3):  # bit by bit the same, whatever ran before
+        again = CLALibGated.backward(dh, x, wg, wu, got[1], got[2], "silu", p=0.1, seed=21, step=5)
+        assert all(torch.equal(p, q) for p, q in zip(again, grads))
+
+
+@pytest.mark.parametrize("M,N,K", [(3000, 5001, 700), (16, 9000, 4096), (100, 1000, 20000), (1, 20001, 1024), (5000, 64, 501), (260, 30000, 130)])
+def test_q8_of_many_tiles(M, N, K):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(M + N)
+    a, b = (torch.randint(-128, 128, s, dtype=torch.int8, device="cuda", generator=gen) for s in ((M, K), (N, K)))
+    sa, sb = torch.rand(M, device="cuda", generator=gen) + 0.1, torch.rand(N, device="cuda", generator=gen) + 0.1
+    want = (a.double() @ b.double().T) * sa.double()[:, None] * sb.double()  # (whole sums below 2^53: exact)
+    for dtype in FLOATS:
+        got = CLALibQ8.matrixMult(a, sa, b, sb, dtype)
+        # A rounding to the type gives an infinity from half a step above its largest value on (fp16: 65504 + 16 = 65520): there the definition
+        # has one, and just there, within the FP32 scaling's 2^-22, either
+        top = float(torch.finfo(dtype).max) * (1 + ref.half_step(dtype) / 2)
+        over, under = want.abs() > top * (1 + 2.0 ** -22), want.abs() < top * (1 - 2.0 ** -22)
+        assert torch.equal(got[over].double(), torch.copysign(torch.full_like(want[over], float("inf")), want[over]))
+        ref.close(torch.where(under, got.double(), 0), torch.where(under, want, 0), q8_bound(want, dtype))
+        assert torch.equal(got, CLALibQ8.matrixMult(a, sa, b, sb, dtype))
+
+
+def test_offsets_beyond_32_bits():
+    """Matrices of more than 2^31 elements: their last rows."""
+    M, F = 70_001, 32_000
+    x, wg, wu = gated_inputs(M, 64, F, torch.bfloat16)
+    h = CLALibGated.forward(x, wg, wu, p=0.5, seed=3)
+    f = ref.drop_factors(5, F, 0.5, 3, 0, M - 5)
+    want, bound = ref.gated(x[-5:], wg, wu, "silu", f, torch.bfloat16)
+    ref.close(h[-5:], want[0], bound[0])
+    y = CLALibDropout.apply(h, 0.25, 9)
+    f = ref.drop_factors(3, F, 0.25, 9, 0, M - 3)
+    want = h[-3:].double().cpu() * f
+    ref.close(y[-3:], want, want.abs() * (ref.half_step(torch.bfloat16) + 2.0 ** -22) + ref.tiny(torch.bfloat16))
+    dx, _, _ = CLALibGated.backward(y, x, wg, wu, h, h, needW=False)
+    want, bound = ref.gated_grads(y[-4:], x[-4:], wg, wu, h[-4:], h[-4:], "silu", torch.ones(4, F, dtype=torch.float64), torch.bfloat16)
+    ref.close(dx[-4:], want[0], bound[0])
+    del y, dx
+    q, s = CLALibQ8.quantizeRows(h)
+    wq, ws = ref.quantize(h[-3:])
+    assert np.array_equal(q[-3:].cpu().numpy(), wq) and np.array_equal(s[-3:].cpu().numpy(), ws)
+    del h
+    b = torch.randint(-128, 128, (40, F), dtype=torch.int8, device="cuda")
+    got = CLALibQ8.matrixMult(q, s, b, torch.ones(40, device="cuda"), torch.float64)
+    want = q8_want(wq, ws, b.cpu().numpy(), np.ones(40, np.float32))
+    ref.close(got[-3:], want, q8_bound(want, torch.float64))
+    del q
+    torch.cuda.empty_cache()
+
+
 # ---- beside one another -----------------------------------------------------------------------------------------------
-def test_streams_devices_and_graphs():
+@pytest.mark.parametrize("M,D,F", [(64, 256, 512), (333, 1001, 2731), (3, 2000, 999)])
+def test_streams_and_graphs(M, D, F):
     """Calls on two streams at once, and captured calls replayed in turn with direct ones."""
-    x, wg, wu = gated_inputs(64, 256, 512, torch.bfloat16)
+    x, wg, wu = gated_inputs(M, D, F, torch.bfloat16)
     w8, s8 = CLALibQ8.quantizeCols(normal(501, 64, torch.float32, 2))
-    z = normal(300, 501, torch.float32, 1)
-    dh = normal(64, 512, torch.bfloat16, 4)
+    z = normal(M, 501, torch.float32, 1)
+    dh = normal(M, F, torch.bfloat16, 4)
 
     def step():
         h, g, u = CLALibGated.forward(x, wg, wu, "gelu", p=0.1, seed=1, step=2, save=True)
@@ -306,11 +376,11 @@ def test_streams_devices_and_graphs():
     want, scores = step(), score()
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
-    for _ in range(3):
+    for _ in range(5):
         with torch.cuda.stream(a):
-            got = [step() for _ in range(4)]
+            got = [step() for _ in range(6)]
         with torch.cuda.stream(b):
-            sc = [score() for _ in range(4)]
+            sc = [score() for _ in range(12)]
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for r in got for p, q in zip(r, want))
         assert all(torch.equal(p, q) for r in sc for p, q in zip(r, scores))
