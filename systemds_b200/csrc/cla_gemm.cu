@@ -207,24 +207,44 @@ __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t co
         }
       }
     } else {
-      for (int r = part * (32 / G); r < end; r++) {
-        char* const row = (char*)(out + r * ld + c0);
-        const auto word = [&](int w) {
-          uint32_t v;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(place(r, w >> 2) + (w & 3) * 4) : "memory");
-          return v;
-        };
-        if (sizeof(O) >= 4 || ((uintptr_t)row & 2) == 0) {
-          for (int w = lane; 4 * w < there; w += 32) {
-            if (4 * w + 4 <= there) *(uint32_t*)(row + 4 * w) = word(w);
-            else *(uint16_t*)(row + 4 * w) = (uint16_t)word(w);
+      const auto word = [&](int r, int w) {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(place(r, w >> 2) + (w & 3) * 4) : "memory");
+        return v;
+      };
+      char* row = (char*)(out + part * (32 / G) * ld + c0);
+      if (there == LINE) {  // two words a lane
+#pragma unroll 4
+        for (int r = part * (32 / G); r < end; r++, row += ld * (int)sizeof(O)) {
+          const uint32_t v = word(r, lane), u = word(r, lane + 32);
+          if (sizeof(O) >= 4 || ((uintptr_t)row & 2) == 0) {
+            ((uint32_t*)row)[lane] = v;
+            ((uint32_t*)row)[lane + 32] = u;
+          } else {  // the row starts in the middle of a word: the words are the upper half of one and the lower half of the next
+            const uint32_t mid = __shfl_sync(0xffffffffu, u, 0);
+            uint32_t nv = __shfl_down_sync(0xffffffffu, v, 1), nu = __shfl_down_sync(0xffffffffu, u, 1);
+            if (lane == 31) nv = mid;
+            uint32_t* q = (uint32_t*)(row + 2);
+            q[lane] = __byte_perm(v, nv, 0x5432);
+            if (lane < 31) q[lane + 32] = __byte_perm(u, nu, 0x5432);
+            else *(uint16_t*)(q + 63) = (uint16_t)(u >> 16);
+            if (lane == 0) *(uint16_t*)row = (uint16_t)v;
           }
-        } else {  // the row starts in the middle of a word: the words are the upper half of one and the lower half of the next
-          if (lane == 0 && there > 0) *(uint16_t*)row = (uint16_t)word(0);
-          for (int w = lane; 4 * w + 2 < there; w += 32) {
-            const uint32_t v = word(w);
-            if (4 * w + 6 <= there) *(uint32_t*)(row + 4 * w + 2) = __byte_perm(v, word(w + 1), 0x5432);
-            else *(uint16_t*)(row + 4 * w + 2) = (uint16_t)(v >> 16);
+        }
+      } else {
+        for (int r = part * (32 / G); r < end; r++, row += ld * (int)sizeof(O)) {
+          if (sizeof(O) >= 4 || ((uintptr_t)row & 2) == 0) {
+            for (int w = lane; 4 * w < there; w += 32) {
+              if (4 * w + 4 <= there) *(uint32_t*)(row + 4 * w) = word(r, w);
+              else *(uint16_t*)(row + 4 * w) = (uint16_t)word(r, w);
+            }
+          } else {
+            if (lane == 0 && there > 0) *(uint16_t*)row = (uint16_t)word(r, 0);
+            for (int w = lane; 4 * w + 2 < there; w += 32) {
+              const uint32_t v = word(r, w);
+              if (4 * w + 6 <= there) *(uint32_t*)(row + 4 * w + 2) = __byte_perm(v, word(r, w + 1), 0x5432);
+              else *(uint16_t*)(row + 4 * w + 2) = (uint16_t)(v >> 16);
+            }
           }
         }
       }
@@ -246,8 +266,8 @@ __device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa,
 constexpr int GP_STAGES = 10, GP_RING = 6 * 2 * GM_OPERAND, GP_GROUP = 8;
 
 // Warps that take the sums out. GATE: 16, for the activation and the dropout of a tile keep eight busy for twice as long as its products take at a
-// depth of 2048 (18 against 9 us: few instructions of a warp at a time are independent).
-__host__ __device__ constexpr int gp_out(int kind) { return kind == GK_GATE ? 16 : 8; }
+// depth of 2048 (18 against 9 us: few instructions of a warp at a time are independent). FP64 results: 16 as well, for the conversions.
+__host__ __device__ constexpr int gp_out(int kind, int bytes) { return kind == GK_GATE || bytes == 8 ? 16 : 8; }
 
 __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& tn) {
   const int per = GP_GROUP * A.tilesN, g = t / per, first = g * GP_GROUP, n = min(GP_GROUP, A.tilesM - first), r = t - g * per;
@@ -256,9 +276,9 @@ __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& 
 }
 
 template <int KIND, class O>
-__global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
+__global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
   constexpr bool I8 = KIND == GK_Q8;
-  constexpr int OUT = gp_out(KIND), G = OUT / 4;  // warps that write results, and of each 32 rows of a tile
+  constexpr int OUT = gp_out(KIND, sizeof(O)), G = OUT / 4;  // warps that write results, and of each 32 rows of a tile
   extern __shared__ __align__(1024) unsigned char gmsm[];
   __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
@@ -413,15 +433,19 @@ __global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2
         const int halfN = A.tilesN / 2, which = KIND == GK_PAIR && tn >= halfN;
         const int64_t n0 = (int64_t)(which ? tn - halfN : tn) * A.wide;
         const float sa = I8 && m < c.M ? c.aScale[m] : 0.f;
-        gm_rows<O, 16, G>((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, A.wide, aligned(which), room, part, 1 + quarter,
-                          [&](int j, O(&o)[16]) {
-                            uint32_t v[16];
-                            gm_tmem16(at + j, v);
+        constexpr int CH = OUT == 16 ? 8 : 16;
+        gm_rows<O, CH, G>((O*)c.out[which] + m0 * c.ldo[which] + n0, c.ldo[which], rows, c.N - n0, A.wide, aligned(which), room, part, 1 + quarter,
+                          [&](int j, O(&o)[CH]) {
+                            uint32_t v[CH];
+                            if constexpr (CH == 8) gm_tmem8(at + j, v);
+                            else gm_tmem16(at + j, v);
                             gm_loaded(v);
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
+                            for (int i = 0; i < CH; i++) {
                               if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
-                              else o[i] = gm_cast<O>(__uint_as_float(v[i]));
+                              else if constexpr (sizeof(O) == 2) {
+                                if (i % 2 == 0) *(uint32_t*)(o + i) = to_word<O>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                              } else o[i] = gm_cast<O>(__uint_as_float(v[i]));
                             }
                           });
       }
@@ -956,7 +980,7 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
     if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
     static_assert(GP_RING + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
     const unsigned ctas = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
-    EarlyLaunch pair(ctas, 128 + gp_out(KIND) * 32, roomPair, s, c.after != AFTER_CALL);
+    EarlyLaunch pair(ctas, 128 + gp_out(KIND, sizeof(O)) * 32, roomPair, s, c.after != AFTER_CALL);
     CLA_CUDA(cudaLaunchKernelEx(&pair.cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
   }
