@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__
   __shared__ Bits part[DN_T / 32];
   const int lane = threadIdx.x % G, warp = threadIdx.x / 32;
   const int64_t r = (int64_t)blockIdx.x * (DN_T / G) + threadIdx.x / G;
-  if (G == 32 && r >= rows) return;
+  if (G < DN_T && r >= rows) return;  // (with all of its group)
   gm_let_next();  // (the product's weights may come meanwhile)
   const T* p = x + r * ldx + (VEC ? lane * V : lane);
   int8_t* to = q + r * ldq + (VEC ? lane * V : lane);
@@ -150,21 +150,32 @@ __global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__
     }
   };
   Bits most = 0;
+  uint32_t most2 = 0;  // of 16-bit values two at a time: their bits have their order too
   for (int first = 0; first < cols; first += ROUND) {
     load(first);
 #pragma unroll
-    for (int j = 0; j < C; j++)
+    for (int j = 0; j < C; j++) {
+      if (sizeof(T) < 8 && first + j * G * V >= cols) break;
 #pragma unroll
-      for (int i = 0; i < V; i++) most = max(most, magnitude(widen(v[j][i])));
+      for (int i = 0; i < V; i += sizeof(T) == 2 ? 2 : 1) {
+        if constexpr (sizeof(T) == 2) most2 = __vmaxu2(most2, *(const uint32_t*)&v[j][i] & 0x7fff7fffu);
+        else most = max(most, magnitude(widen(v[j][i])));
+      }
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t larger = (uint16_t)max(most2 & 0xffffu, most2 >> 16);
+    most = magnitude(widen(*(const T*)&larger));
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
   if (G > 32) {
+    const int group = threadIdx.x / G;
     if (threadIdx.x % 32 == 0) part[warp] = most;
-    __syncthreads();
-    most = part[0];
+    gm_group_sync(1 + group, G);
+    most = part[group * (G / 32)];
 #pragma unroll
-    for (int i = 1; i < DN_T / 32; i++) most = max(most, part[i]);
+    for (int i = 1; i < G / 32; i++) most = max(most, part[group * (G / 32) + i]);
   }
   const float s = q8_scale(most);
   const Q8Row<W> q8(s);
@@ -442,18 +453,17 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
     }
     constexpr int V = DN_V<T>, C = sizeof(T) == 8 ? 8 : 4;
     const bool vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
-    // a warp per row, without a barrier, where it holds the row and there are rows enough
-    const bool warps = cols <= 32 * C * V && rows >= 148;
-    auto go = [&](auto kernel, OncePerDevice& once, unsigned grid) {
+    // the fewest threads that hold the row, where there are rows enough for all SMs: a warp (no barrier), half a CTA, a CTA
+    const int group = rows < 148 ? DN_T : cols <= 32 * C * V ? 32 : cols <= 128 * C * V ? 128 : DN_T;
+    auto go = [&](auto kernel, OncePerDevice& once) {
       rc = once(device, [&] { return like_products(kernel); });
-      if (rc >= 0) kernel<<<grid, DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale);
+      const int down = DN_T / group;
+      if (rc >= 0) kernel<<<(unsigned)((rows + down - 1) / down), DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale);
     };
-    const unsigned grid = (unsigned)(warps ? (rows + DN_T / 32 - 1) / (DN_T / 32) : rows);
-    static OncePerDevice once[4];
-    if (warps && vec) go(k_quantize_rows<T, 32, C, true>, once[0], grid);
-    else if (warps) go(k_quantize_rows<T, 32, C, false>, once[1], grid);
-    else if (vec) go(k_quantize_rows<T, DN_T, C, true>, once[2], grid);
-    else go(k_quantize_rows<T, DN_T, C, false>, once[3], grid);
+    static OncePerDevice once[6];
+    if (group == 32) vec ? go(k_quantize_rows<T, 32, C, true>, once[0]) : go(k_quantize_rows<T, 32, C, false>, once[1]);
+    else if (group == 128) vec ? go(k_quantize_rows<T, 128, C, true>, once[2]) : go(k_quantize_rows<T, 128, C, false>, once[3]);
+    else vec ? go(k_quantize_rows<T, DN_T, C, true>, once[4]) : go(k_quantize_rows<T, DN_T, C, false>, once[5]);
   });
   if (rc < 0) return rc;
   CLA_CUDA(cudaGetLastError());

@@ -137,7 +137,7 @@ __device__ __forceinline__ unsigned long long magnitude(double v) { return (unsi
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ float q8_scale(unsigned long long most) { return (float)(__longlong_as_double((long long)most) / 127.0); }
 __device__ __forceinline__ float q8_scale(uint32_t most) { return __uint_as_float(most) / 127.f; }
-// The nearest whole number of x / scale, as the low byte of the result. The product with the reciprocal is off by three roundings of a value
+// The nearest whole number of x / scale, as the low byte of the result. The product with the reciprocal is off by roundings of a value
 // below 128: unless it comes that near to a half, where the quotient itself decides, both have the same nearest whole number. So the product
 // is taken first, rounded by adding 1.5 times the power of two whose unit is 1, and whether some value came near is asked once
 // for many of them: the quotients are then taken for all.
@@ -148,9 +148,9 @@ template <class W> struct Q8Row {
       : scale((W)s), inv((W)1 / (W)s), some(s > 0.f && s < INFINITY), quick(s >= 0x1p-126f && s < INFINITY) {}
   __device__ __forceinline__ uint32_t product(W x, bool& near) const {
     constexpr W MAGIC = sizeof(W) == 8 ? (W)0x1.8p52 : (W)0x1.8p23;
-    constexpr W FAR = (W)0.5 - (sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-15);  // above 3/2 of 127 roundings of 2^-52, 2^-23
-    const W t = x * inv, r = t + MAGIC;
-    near |= !(fabs(t - (r - MAGIC)) <= FAR);
+    constexpr W FAR = (W)0.5 - (sizeof(W) == 8 ? (W)0x1p-43 : (W)0x1p-15);  // above 127 times two roundings of 2^-53, 2^-24 (of the reciprocal, of the quotient) and the last one
+    const W r = fma(x, inv, MAGIC);
+    near |= !(fabs(fma(x, inv, MAGIC - r)) <= FAR);
     if constexpr (sizeof(W) == 8) return (uint32_t)__double2loint(r);
     else return __float_as_uint(r);
   }
@@ -246,6 +246,8 @@ enum After {
   AFTER_NONE   // the two read and write nothing that the other writes: at the end, so that who waits for this one has waited for both. The one
                // before has let this one by only after its own wait, so that what came before both is over when this one starts
 };
+// A barrier of some of a CTA's warps
+__device__ __forceinline__ void gm_group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void gm_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void gm_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // A launch configuration with the kernel before still running, or not (After)

@@ -160,7 +160,6 @@ template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f
 // of up to LINE bytes go out, 32 / G rows a warp: in pieces of 16 bytes where rows start on 16-byte boundaries (vec), else a word a
 // lane. (Long pieces count where rows do not start on sectors: each piece then writes parts of two sectors.) The pieces of shared
 // memory are swizzled over the rows.
-__device__ __forceinline__ void gm_group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // Whether all of them say so
 __device__ __forceinline__ bool gm_group_all(int id, int threads, bool ok) {
   uint32_t r;
