@@ -310,8 +310,8 @@ int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t ro
                             float* scale, int32_t device, void* stream);
 
 /* out[m, n] = aScale[m] * bScale[n] * sum over k of a[m, k] * b[n, k], the sum exact in 32-bit integers, K <= 131071. aType CLA_T_I8, or a
- * floating type: a's rows are then quantised in the call as cla_q8_quantize_dev does (aScale unused). Scaled in FP64 for
- * outType F64, else in FP32, and rounded once to outType. */
+ * floating type: a's rows are then quantised in the call as cla_q8_quantize_dev does (aScale unused). Scaled as (sum * aScale) * bScale in
+ * FP64 for outType F64, else in FP32, and rounded once to outType. */
 typedef struct cla_q8 {
   int64_t M, N, K;
   const void* a;

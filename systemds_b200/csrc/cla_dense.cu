@@ -329,7 +329,7 @@ struct Copies {
   const void* from[3];
   void* to[3];
   int64_t ldFrom[3], ldTo[3];
-  int bytes[3];  // of a row
+  int64_t bytes[3];  // of a row
   Walk walk[3];
   int ctas[4];   // the first CTA of each, down the rows
 };
@@ -342,14 +342,15 @@ __global__ void __launch_bounds__(DN_T) k_repitch(const __grid_constant__ Copies
   const int tx = threadIdx.x & ((1 << w.log) - 1), down = DN_T >> w.log, ctas = c.ctas[k + 1] - c.ctas[k];
   const int64_t step = (int64_t)ctas * down, ldx = c.ldFrom[k], ldy = c.ldTo[k];
   for (int piece = blockIdx.x * (1 << w.log) + tx; piece < w.per; piece += gridDim.x << w.log) {
-    const int left = c.bytes[k] - piece * 16;
+    const int64_t at = (int64_t)piece * 16;
+    const int left = (int)min((int64_t)16, c.bytes[k] - at);
     for (int64_t r = (int64_t)(blockIdx.y - c.ctas[k]) * down + (threadIdx.x >> w.log); r < w.rows; r += 2 * step) {
       alignas(16) uint8_t v[2][16];
       const bool two = r + step < w.rows;
-      load_vec(x + r * ldx + piece * 16, left, false, v[0]);
-      if (two) load_vec(x + (r + step) * ldx + piece * 16, left, false, v[1]);
-      store_vec(y + r * ldy + piece * 16, left, true, v[0]);
-      if (two) store_vec(y + (r + step) * ldy + piece * 16, left, true, v[1]);
+      load_vec(x + r * ldx + at, left, false, v[0]);
+      if (two) load_vec(x + (r + step) * ldx + at, left, false, v[1]);
+      store_vec(y + r * ldy + at, left, true, v[0]);
+      if (two) store_vec(y + (r + step) * ldy + at, left, true, v[1]);
     }
   }
 }
@@ -383,7 +384,9 @@ struct OnDevice {
       e = cudaSetDevice(device);
       if (e == cudaSuccess) before = now;
     }
-    if (e != cudaSuccess) rc = fail(CLA_ERR_CUDA, std::string("device of a dense call: ") + cudaGetErrorString(e));
+    if (e == cudaSuccess) return;
+    rc = fail(CLA_ERR_CUDA, std::string("device of a dense call: ") + cudaGetErrorString(e));
+    cudaGetLastError();  // (or the next launch would be taken for the one that failed)
   }
   ~OnDevice() {
     if (before >= 0) cudaSetDevice(before);
@@ -500,7 +503,7 @@ struct Aligned {
     if (rows && cols) {
       c.from[n] = o.p, c.to[n] = to;
       c.ldFrom[n] = o.ld * bytes, c.ldTo[n] = ld * bytes;
-      c.bytes[n] = (int)(cols * bytes);
+      c.bytes[n] = cols * bytes;
       c.walk[n].rows = rows;
       n++;
     }

@@ -195,7 +195,7 @@ __device__ __forceinline__ float act_slope(int act, float g, float& value) {
     default: {
       const float s = sigmoid_of(gelu_arg(g));
       value = g * s;
-      return s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
+      return s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * fminf(g * g, 1e4f));  // (beyond, 1 - s or s is 0, and the square may be infinite)
     }
   }
 }

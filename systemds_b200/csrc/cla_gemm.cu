@@ -155,12 +155,7 @@ struct alignas(64) GemmArgs {
 // ---- epilogues ----------------------------------------------------------------------------------------------------------
 template <class O> __device__ __forceinline__ O gm_cast(float v) { return from_f32<O>(v); }
 
-// The warps that hold the same 32 rows of a tile (a lane each), G of them, write `width` columns of these rows. f(j, o): columns j .. j + CH - 1 of
-// the lane's row, all lanes together. The warps take LINE / G bytes of a row in turn into the shared memory of the group; from there whole rows
-// of up to LINE bytes go out, 32 / G rows a warp: in pieces of 16 bytes where rows start on 16-byte boundaries (vec), else a word a
-// lane. (Long pieces count where rows do not start on sectors: each piece then writes parts of two sectors.) The pieces of shared
-// memory are swizzled over the rows.
-// Whether all of them say so
+// Whether all of some of a CTA's warps say so
 __device__ __forceinline__ bool gm_group_all(int id, int threads, bool ok) {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
@@ -169,6 +164,11 @@ __device__ __forceinline__ bool gm_group_all(int id, int threads, bool ok) {
                : "memory");
   return r != 0;
 }
+// The warps that hold the same 32 rows of a tile (a lane each), G of them, write `width` columns of these rows. f(j, o): columns j .. j + CH - 1 of
+// the lane's row, all lanes together. The warps take LINE / G bytes of a row in turn into the shared memory of the group; from there whole rows
+// of up to LINE bytes go out, 32 / G rows a warp: in pieces of 16 bytes where rows start on 16-byte boundaries (vec), else a word a
+// lane. (Long pieces count where rows do not start on sectors: each piece then writes parts of two sectors.) The pieces of shared
+// memory are swizzled over the rows.
 template <class O, int CH, int G, class F>
 __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t cols, int width, bool vec, uint32_t buf, int part, int id, F&& f) {
   constexpr int LINE = 256, PIECES = CH * (int)sizeof(O) / 16;
@@ -259,8 +259,8 @@ __device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa,
 
 // ---- large results --------------------------------------------------------------------------------------------------------
 // Tile 256 x 256 per pair of CTAs (GATE: 256 x 128 of both products; narrower for few columns): each CTA holds the sums of its 128 rows and
-// brings 128 rows and 128 columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight take the sums out of one half of
-// tensor memory while the other fills. A launch's pairs take tiles in turn, along the rows within groups of GP_GROUP row tiles, so that what
+// brings 128 rows and 128 columns of the operands, 32 KB a stage. One warp copies, one multiplies (the first CTA's, for both), eight or sixteen (gp_out) take the
+// sums out of one half of tensor memory while the other fills. A launch's pairs take tiles in turn, along the rows within groups of GP_GROUP row tiles, so that what
 // runs at once shares operands in L2.
 constexpr int GP_STAGES = 10, GP_RING = 6 * 2 * GM_OPERAND, GP_GROUP = 8;
 
@@ -827,6 +827,7 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
 int64_t dense_status(int device) {
   (void)device;
   int32_t e = 0, zero = 0;
+  CLA_CUDA(cudaDeviceSynchronize());  // (the copy itself waits for no stream that was made not to)
   CLA_CUDA(cudaMemcpyFromSymbol(&e, denseErr, sizeof(e)));
   if (!e) return CLA_OK;
   CLA_CUDA(cudaMemcpyToSymbol(denseErr, &zero, sizeof(zero)));

@@ -6,7 +6,7 @@
 
 They have no counterpart in the reference. Operands are torch CUDA tensors with rows of adjacent elements (any row stride; weights may also be
 transposed views). Each call is enqueued on the current stream of its tensors' device, takes results and workspaces from torch's
-allocator, and may be captured into a graph. A ``CompressedMatrixBlock`` takes part through ``CLALibQ8.rightMultByMatrix`` and
+allocator, and may be captured into a graph. Nothing is recorded for autograd: gradients are the ``backward`` calls' and the dropout's own. A ``CompressedMatrixBlock`` takes part through ``CLALibQ8.rightMultByMatrix`` and
 ``CLALibDecompress.rows``. Failures raise ``CLAError``.
 """
 from __future__ import annotations
@@ -67,6 +67,8 @@ def _result(out, shape, dtype, like, what: str):
     """``out``, or a new tensor on the device of ``like``."""
     if out is None:
         return like.new_empty(shape) if like.dtype == dtype else torch.empty(shape, dtype=dtype, device=like.device)
+    if not isinstance(out, torch.Tensor):
+        _fail(-2, f"{what}: a CUDA tensor is needed")
     if tuple(out.shape) != tuple(shape):
         _fail(-4, f"{what}: shape {tuple(out.shape)}, expected {tuple(shape)}")
     return out
@@ -86,6 +88,8 @@ def _workspace(n: int, device):
 def _drop(p, seed, step, row0) -> native.cla_drop:
     if not 0 <= seed < 1 << 64 or not 0 <= step < 1 << 64:
         _fail(-2, "dropout: seed and step are unsigned 64-bit numbers")
+    if not 0 <= row0 <= 1 << 32:
+        _fail(-2, "dropout: rows beyond 2^32")
     return native.cla_drop(p, seed, step, row0)
 
 

@@ -1,9 +1,11 @@
 """The dense operators on the GPU against their plain 64-bit forms (tests/dense_ref.py, where the bounds are derived)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
-from systemds_b200 import CLAError, CLALibDecompress, CLALibDropout, CLALibGated, CLALibQ8, datagen
+from systemds_b200 import CLAError, CLALibDecompress, CLALibDropout, CLALibGated, CLALibQ8, datagen, native
 from systemds_b200.dense import status
 from tests import dense_ref as ref
 from tests.util import dense_of
@@ -288,6 +290,18 @@ def test_gated_values_that_are_not_finite_stay_in_their_rows():
     assert torch.equal(CLALibGated.forward(x, wg, wu)[rest], clean[rest])
 
 
+@pytest.mark.parametrize("act", ref.ACTS)
+def test_gated_slopes_of_large_gates(act):
+    """Where the square or the cube of a gate leaves FP32 the slope is that of the line: 1 or 0."""
+    g = torch.tensor([[1e38, -1e38, 1e20, -1e20, 1e13, -1e13, 200.0, -200.0]], dtype=torch.bfloat16, device="cuda")
+    one = torch.ones_like(g)
+    w = torch.ones((8, 8), dtype=torch.bfloat16, device="cuda")
+    _, dwg, dwu = CLALibGated.backward(one, one, w, w, g, one, act, needX=False)
+    up = (g > 0).to(g.dtype)
+    assert torch.equal(dwg, (torch.zeros_like(up) if act == "sigmoid" else up).expand(8, 8))
+    assert torch.equal(dwu, (up if act == "sigmoid" else up * g).expand(8, 8))
+
+
 MANY = [(2500, 1100, 3001), (40, 5000, 9000), (300, 6000, 260), (1, 3000, 20000), (700, 2050, 1800), (32, 8200, 520)]
 
 
@@ -354,6 +368,20 @@ def test_offsets_beyond_32_bits():
     want = q8_want(wq, ws, b.cpu().numpy(), np.ones(40, np.float32))
     ref.close(got[-3:], want, q8_bound(want, torch.float64))
     del q
+    torch.cuda.empty_cache()
+
+
+def test_a_row_of_two_gigabytes_off_its_boundary():
+    D = 1 << 30
+    x = torch.zeros(D + 1, dtype=torch.bfloat16, device="cuda")[1:].reshape(1, D)
+    w = [torch.zeros((2, D), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for k, at in enumerate((0, 7, 12345, D // 2, D - 9, D - 1)):
+        x[0, at] = 1
+        w[0][:, at] = 1 << k
+        w[1][1, at] = 1
+    h = CLALibGated.forward(x, w[0].t(), w[1].t(), "relu")
+    assert h.tolist() == [[0.0, 63 * 6.0]]
+    del x, w, h
     torch.cuda.empty_cache()
 
 
@@ -450,3 +478,28 @@ def test_refusals_on_the_device():
               lambda: CLALibDropout.apply(x, 0.5, 1, out=torch.empty_like(x).half()), lambda: CLALibDropout.apply(x[:1].expand(8, 16), 0.5, 1, out=x)):
         with pytest.raises(CLAError):
             f()
+
+
+def test_a_refused_device_leaves_the_next_call_as_it_was():
+    x = normal(8, 16, torch.float32, 1)
+    y, d = torch.empty_like(x), native.cla_drop(0.5, 1, 2, 0)
+    with pytest.raises(CLAError):
+        native.check(native.lib().cla_dropout_dev(1, x.data_ptr(), 16, 8, 16, y.data_ptr(), 16, C.byref(d), 99, None))
+    assert torch.equal(CLALibDropout.apply(x, 0.5, 1, 2, out=y), CLALibDropout.apply(x, 0.5, 1, 2))
+    for f in (lambda: CLALibDropout.apply(x, 0.5, 1, row0=(1 << 64) + 5), lambda: CLALibDropout.apply(x, 0.5, 1, out=[1]),
+              lambda: CLALibDropout.apply(x, 0.5, 1, out=y.cpu().numpy())):
+        with pytest.raises(CLAError):
+            f()
+
+
+def test_status_waits_for_every_stream():
+    x = torch.ones((8192, 8192), device="cuda")
+    y = torch.empty_like(x)
+    CLALibDropout.apply(x, 0.5, 1, out=y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for step in range(100):
+            CLALibDropout.apply(x, 0.5, 1, step, out=y)
+    status()
+    assert side.query()
