@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__
   for (int first = 0; first < cols; first += ROUND) {
     if (cols > ROUND) load(first);
     const int left = cols - first - (VEC ? lane * V : lane);
-    // how many pieces are asked about together: FP64 values hardly ever come near, the others' in one of a hundred pieces of a warp
+    // how many pieces are asked about together: FP64 values hardly ever come near, FP32 ones in one of a hundred pieces of a warp
     constexpr int ASK = sizeof(T) == 8 ? C : 1;
 #pragma unroll
     for (int j0 = 0; j0 < C; j0 += ASK) {
@@ -196,9 +196,12 @@ __global__ void __launch_bounds__(DN_T, 3) k_quantize_rows(const T* __restrict__
         for (int i = 0; i < V; i++) o[j][i] = (uint8_t)q8.product(widen(v[j0 + j][i]), near);
       if (near) {  // (calls, which are not made before it is known whether they are wanted)
 #pragma unroll
-        for (int j = 0; j < ASK; j++)
+        for (int j = 0; j < ASK; j++) {
+          W x[V];
 #pragma unroll
-          for (int i = 0; i < V; i++) o[j][i] = (uint8_t)q8_quotient(widen(v[j0 + j][i]), q8.scale, q8.some);
+          for (int i = 0; i < V; i++) x[i] = widen(v[j0 + j][i]);
+          q8_quotients<T>(q8, x, o[j]);
+        }
       }
 #pragma unroll
       for (int j = 0; j < ASK; j++) {
@@ -563,6 +566,8 @@ int64_t q8_run(const cla_q8& c, bool run, Work& w, cudaStream_t s, bool split = 
   if (aligned.n) g.after = AFTER_ALL;
   if (split && c.aType == c.outType && gemm_quantizes(c.M, c.K, c.aType)) {
     g.quantize = true;
+  } else if (c.aType == c.outType && gemm_scores(c.M, c.N, c.K, c.aType)) {
+    g.scores = true;
   } else if (c.aType != CLA_T_I8) {
     const int64_t ld = round_up(c.K, PITCH);
     int8_t* q = (int8_t*)w.take(c.M * ld);

@@ -159,6 +159,18 @@ template <class W> __device__ __noinline__ uint32_t q8_quotient(W x, W scale, bo
   return some ? (uint32_t)(int)fmin((W)127, fmax((W)-127, rint(x / scale))) : 0u;
 }
 
+// The quotients of values of which some product came near. Of 16-bit values one in 200 does (quotients of two of 256 numbers, times 127): then only those
+// are divided that a lane of the warp asks for (16384 x 4096 BF16 values: 53 us, all of a piece divided 70).
+template <class T, int N, class O>
+__device__ __forceinline__ void q8_quotients(const Q8Row<typename WideOf<T>::type>& q8, const typename WideOf<T>::type (&v)[N], O (&o)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j++) {
+    bool near = !q8.quick;
+    if (sizeof(T) == 2) q8.product(v[j], near);
+    if (sizeof(T) > 2 || near) o[j] = (O)q8_quotient(v[j], q8.scale, q8.some);
+  }
+}
+
 // ---- the activation, in FP32 ------------------------------------------------------------------------------------------
 // With the fast exponential and quotient: off by some units of 2^-23, under 2^-20 of the value where |g| < 10 (beyond, a unit more for each
 // of g's), next to the 2^-11 or 2^-8 of the rounding that follows.
@@ -236,6 +248,7 @@ struct GemmCall {
   void* parts = nullptr;  // gemm_workspace() bytes, 256-byte aligned
   int after = 0;          // AFTER_*
   bool quantize = false;  // Q8: a holds rows of outType, which the product quantises itself (gemm_quantizes())
+  bool scores = false;    // the same, for few columns (gemm_scores()); the rows of a need no alignment
 };
 // What a kernel has to do with the one that the same call has launched just before it (which itself came after all that the stream held). The kernel may
 // then start while that one still runs, and waits for its end where it says; the one before lets it by gm_let_next().
@@ -265,6 +278,7 @@ struct EarlyLaunch {
 };
 // Whether a product quantises so many rows itself, of the type that the results have
 bool gemm_quantizes(int64_t M, int64_t K, int type);
+bool gemm_scores(int64_t M, int64_t N, int64_t K, int type);  // so many rows for so few columns
 int64_t gemm_workspace(const GemmCall& c);  // goes by the sizes, the types and which index is contiguous
 int64_t launch_gemm(const GemmCall& c, cudaStream_t s);
 int64_t dense_status(int device);  // the self-check word of the product kernels, cleared

@@ -3,7 +3,8 @@
 //  * k_gemm_pair: two CTAs share a 256 x 256 tile. For large results.
 //  * k_gemm_few: tiles of 128 columns of the result and 16 to 128 of its rows, whose depth the CTAs share evenly; k_gemm_join adds up the
 //    parts of tiles that several CTAs share. For few rows.
-// Both are launched with at most one CTA an SM, which takes all of the SM's shared and tensor memory and loops: no CTA waits for tensor memory.
+//  * k_gemm_rows: 8-bit products of many rows with few columns, which quantises the rows on the way.
+// All are launched with at most one CTA an SM, which takes all of the SM's shared and tensor memory and loops: no CTA waits for tensor memory.
 #include <cuda.h>
 #include <algorithm>
 #include "cla_dense.cuh"
@@ -251,9 +252,10 @@ __device__ __forceinline__ void gm_rows(O* out, int64_t ld, int rows, int64_t co
     gm_group_sync(id, G * 32);
   }
 }
-template <int KIND, class O>
-__device__ __forceinline__ O gm_scaled(const GemmCall& c, int32_t sum, float sa, float sb) {
-  if constexpr (sizeof(O) == 8) return (double)sum * sa * sb;
+// (sums as doubles: below the 32 bits that a number of 2^52 leaves, shifted to be positive; a conversion takes four times as long)
+template <class O, class W>
+__device__ __forceinline__ O gm_scaled(int32_t sum, W sa, W sb) {
+  if constexpr (sizeof(O) == 8) return (__hiloint2double(0x43300000, sum ^ (int32_t)0x80000000) - (0x1p52 + 0x1p31)) * (double)sa * (double)sb;
   else return gm_cast<O>((float)sum * sa * sb);
 }
 
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
                             gm_loaded(v);
 #pragma unroll
                             for (int i = 0; i < CH; i++) {
-                              if constexpr (I8) o[i] = gm_scaled<KIND, O>(c, (int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
+                              if constexpr (I8) o[i] = gm_scaled<O>((int32_t)v[i], sa, n0 + j + i < c.N ? __ldg(c.bScale + n0 + j + i) : 0.f);
                               else if constexpr (sizeof(O) == 2) {
                                 if (i % 2 == 0) *(uint32_t*)(o + i) = to_word<O>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                               } else o[i] = gm_cast<O>(__uint_as_float(v[i]));
@@ -484,7 +486,7 @@ __host__ __device__ inline int gf_start(int i, int ctas, int n, int nk, bool who
 template <int KIND, class O>
 __device__ __forceinline__ void gm_finish(const GemmCall& c, int which, int64_t m, int64_t n, uint32_t v0, uint32_t v1, float sa, float sb) {
   if constexpr (KIND == GK_Q8) {
-    ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<KIND, O>(c, (int32_t)v0, sa, sb);
+    ((O*)c.out[0])[m * c.ldo[0] + n] = gm_scaled<O>((int32_t)v0, sa, sb);
   } else if constexpr (KIND == GK_GATE) {
     const float g = __uint_as_float(v0), u = __uint_as_float(v1);
     float h = act_value(c.act, g) * u;
@@ -823,6 +825,232 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
   }
 }
 
+// ---- few columns ----------------------------------------------------------------------------------------------------------
+// Products of rows that are quantised on the way, for so few columns that a CTA holds all of the weights: the rows come from memory once and in
+// nothing but their own type, with no copy of them in 8 bits. A CTA takes an even range of the rows, its sixteen warps one row after another each: a
+// warp brings its next rows to its own places of shared memory, by copies of the 16-byte pieces that hold a row (it may start anywhere; copying them for all
+// warps, one lane was busy for 200 clocks a row and took longest), finds the scale, and puts the 8-bit values where the products read them, 128 rows a
+// tile. Then come the tile's products, which take a twentieth of the time, and all warps write the results while the next rows are on their way.
+// Bound: memory next to the instructions of the quantisation (100,003 rows of 501 values, 64 columns: FP64 85 us, 5.3 TB/s; FP32 57 us, BF16 66 us, where
+// the issue slots are 55 % busy).
+constexpr int GR_WARPS = 16, GR_T = GR_WARPS * 32, GR_SLOTS = 128, GR_ROOM = 223 * 1024;
+struct RowsPlan {
+  int kb, wide, slot, slots;  // blocks of the depth; columns with those that are not there; bytes of a row in the ring, rows
+  bool fits = false;
+};
+static RowsPlan rows_plan(int64_t N, int64_t K, int type) {
+  RowsPlan p;
+  if (N > 256 || K <= 0 || K > 2048) return p;
+  p.kb = (int)(K + 127) / 128;
+  p.wide = 32;
+  while (p.wide < N) p.wide *= 2;
+  p.slot = (int)round_up(K * type_bytes(type), 16) + 16;
+  const int left = GR_ROOM - 1024 - std::max(p.kb * (int)GM_OPERAND, 4 * 8192) - p.kb * p.wide * 128;
+  p.slots = left > 0 ? std::min(GR_SLOTS, left / p.slot / GR_WARPS * GR_WARPS) : 0;
+  p.fits = p.slots == GR_SLOTS || (p.slots >= 2 * GR_WARPS && p.slots * p.slot >= 24 << 10);  // (two rows a warp)
+  return p;
+}
+
+__device__ __forceinline__ uint32_t gr_most(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ unsigned long long gr_most(unsigned long long v) {
+  const uint32_t hi = (uint32_t)(v >> 32), most = __reduce_max_sync(0xffffffffu, hi);
+  return (unsigned long long)most << 32 | __reduce_max_sync(0xffffffffu, hi == most ? (uint32_t)v : 0u);
+}
+
+// ROWS: how many rows a warp takes at once (of a row alone one operation waits for another most of the time: 100,003 FP64 rows of 100 values, 64
+// columns: 49 us, one at a time 55; longer ones of FP64 leave the memory less to do meanwhile). KEPT: blocks of a row that stay in registers, all of
+// them or none (the row is then read a second time).
+template <class X, int ROWS, int KEPT>
+__global__ void __launch_bounds__(GR_T, 1) k_gemm_rows(const __grid_constant__ GemmArgs A) {
+  using W = typename WideOf<X>::type;
+  extern __shared__ __align__(1024) unsigned char gmsm[];
+  __shared__ __align__(8) uint64_t full[GR_SLOTS], bFull, sumFull;
+  __shared__ float scale[128];
+  __shared__ W columns[256];  // the columns' scales
+  __shared__ uint32_t tmemAt;
+  const GemmCall& c = A.c;
+  const int lane = threadIdx.x & 31, warp = gm_warp(), kbs = A.kBlocks, wide = A.wide, slots = A.stages, slot = A.nc;
+  const uint32_t smem = (gm_smem(gmsm) + 1023u) & ~1023u, atB = smem + max(kbs * (int)GM_OPERAND, 4 * 8192), ring = atB + kbs * wide * 128;
+  const int64_t r0 = c.M * blockIdx.x / gridDim.x;
+  const int rows = (int)(c.M * (blockIdx.x + 1) / gridDim.x - r0);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(gm_smem(&tmemAt)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < slots; i++) gm_init(gm_smem(full + i), 1);
+    gm_init(gm_smem(&bFull), 1);
+    gm_init(gm_smem(&sumFull), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmemAt, fullAt = gm_smem(full);
+  bool ok = true;
+  const auto row = [&](int i) { return (const X*)c.a[0].p + (r0 + i) * c.a[0].ld; };
+  const auto bring = [&](int i, int s) {  // (all lanes)
+    if (i < rows && gm_elect()) {
+      const uintptr_t first = (uintptr_t)row(i), from = first & ~(uintptr_t)15;
+      const uint32_t bytes = (uint32_t)(((first + c.K * sizeof(X) + 15) & ~(uintptr_t)15) - from);
+      gm_expect(fullAt + s * 8, bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + s * slot), "l"(from), "r"(bytes),
+                   "r"(fullAt + s * 8)
+                   : "memory");
+    }
+    __syncwarp();
+  };
+  for (int i = warp; i < slots; i += GR_WARPS) bring(i, i);
+  if (warp == 0) {
+    if (gm_elect()) {
+      gm_expect(gm_smem(&bFull), kbs * wide * 128);
+      for (int kb = 0; kb < kbs; kb++) gm_load<false>(atB + kb * wide * 128, A.b, kb * 128, 0, gm_smem(&bFull));
+    }
+    __syncwarp();
+  }
+  if (threadIdx.x < wide) columns[threadIdx.x] = threadIdx.x < c.N ? (W)c.bScale[threadIdx.x] : (W)0;
+  const unsigned char* ringAt = gmsm + (ring - gm_smem(gmsm));
+  int at = warp, place = warp;  // the warp's row, and where it is
+  uint32_t turn = 0;
+  const int left = (int)c.K - lane;
+  // The warp's next R rows, side by side
+  const auto take = [&](auto count, int t0) {
+    constexpr int R = decltype(count)::value;
+    const X* x[R];
+    int from[R];
+    uint32_t to[R], swizzle[R];
+    decltype(magnitude(W())) most[R];
+    const uint32_t half = lane >> 4;
+    int p = place;
+    uint32_t parity = turn;
+#pragma unroll
+    for (int q = 0; q < R; q++) {
+      if (!gm_wait_all(fullAt + p * 8, parity)) return false;
+      const int i = at + q * GR_WARPS, r = i - t0;
+      x[q] = (const X*)(ringAt + p * slot + ((uintptr_t)row(i) & 15)) + lane;
+      from[q] = p;
+      to[q] = smem + r * 128 + (lane & 15), swizzle[q] = r & 7;
+      most[q] = 0;
+      p += GR_WARPS;
+      if (p >= slots) p = warp, parity ^= 1;
+    }
+    const auto load = [&](int q, int kb, W(&v)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[j] = kb * 128 + j * 32 < left ? widen(x[q][kb * 128 + j * 32]) : (W)0;
+        most[q] = max(most[q], magnitude(v[j]));
+      }
+    };
+    const auto store = [&](int q, const Q8Row<W>& q8, int kb, const W(&v)[4]) {
+      uint32_t o[4];
+      bool near = !q8.quick;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = q8.product(v[j], near);
+      if (near) q8_quotients<X>(q8, v, o);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        asm volatile("st.shared.u8 [%0], %1;" ::"r"(to[q] + kb * GM_OPERAND + ((2 * j + half) ^ swizzle[q]) * 16), "r"(o[j]) : "memory");
+    };
+    W v[R][KEPT ? KEPT : 1][4];
+    if constexpr (KEPT > 0) {
+#pragma unroll
+      for (int kb = 0; kb < KEPT; kb++)
+#pragma unroll
+        for (int q = 0; q < R; q++)
+          if (kb < kbs) load(q, kb, v[q][kb]);
+    } else {
+#pragma unroll 2
+      for (int kb = 0; kb < kbs; kb++) load(0, kb, v[0][0]);
+    }
+#pragma unroll
+    for (int q = 0; q < R; q++) most[q] = gr_most(most[q]);  // (of values that all lanes have read)
+    if constexpr (KEPT > 0)
+#pragma unroll
+      for (int q = 0; q < R; q++) bring(at + q * GR_WARPS + slots, from[q]);
+    float sc[R];
+#pragma unroll
+    for (int q = 0; q < R; q++) sc[q] = q8_scale(most[q]);
+#pragma unroll
+    for (int q = 0; q < R; q++) {
+      if (lane == 0) scale[at + q * GR_WARPS - t0] = sc[q];
+      const Q8Row<W> q8(sc[q]);
+      if constexpr (KEPT > 0) {
+#pragma unroll
+        for (int kb = 0; kb < KEPT; kb++)
+          if (kb < kbs) store(q, q8, kb, v[q][kb]);
+      } else {
+#pragma unroll 2
+        for (int kb = 0; kb < kbs; kb++) {
+          load(0, kb, v[0][0]);
+          store(0, q8, kb, v[0][0]);
+        }
+        __syncwarp();
+        bring(at + slots, from[0]);
+      }
+    }
+    at += R * GR_WARPS, place = p, turn = parity;
+    return true;
+  };
+  {
+    const int quarter = warp & 3;
+    const uint64_t da = gm_desc(smem, false), db = gm_desc(atB, false);
+    uint32_t ph = 0;
+    for (int t0 = 0; t0 < rows; t0 += 128, ph ^= 1) {
+      const int n = min(128, rows - t0);
+      while (ok && at < t0 + n) {
+        if (ROWS == 2 && at + GR_WARPS < t0 + n) ok = take(std::integral_constant<int, ROWS>(), t0);
+        else ok = take(std::integral_constant<int, 1>(), t0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      ok = gm_group_all(1, GR_T, ok);
+      if (!ok) break;
+      if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        ok = gm_wait_all(gm_smem(&bFull), 0);
+        if (ok && gm_elect()) {
+          for (int kb = 0; kb < kbs; kb++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              gm_mma<false, true>(tmem, da + (kb * GM_OPERAND >> 4) + i * gm_step(false), db + (kb * wide * 128 >> 4) + i * gm_step(false), A.idesc, kb > 0 || i > 0);
+          gm_commit<false>(gm_smem(&sumFull));
+        }
+        __syncwarp();
+      }
+      ok = gm_wait_all(gm_smem(&sumFull), ph) && ok;
+      ok = gm_group_all(1, GR_T, ok);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int64_t m0 = r0 + t0 + quarter * 32;
+      const W sa = scale[quarter * 32 + lane];
+      const bool aligned = ((uintptr_t)c.out[0] | (uintptr_t)(c.ldo[0] * sizeof(X))) % 16 == 0;
+      gm_rows<X, 8, GR_WARPS / 4>((X*)c.out[0] + m0 * c.ldo[0], c.ldo[0], max(0, min(32, n - quarter * 32)), c.N, wide, aligned, smem + quarter * 8192, warp >> 2,
+                                  2 + quarter, [&](int j, X(&o)[8]) {
+                                    uint32_t v[8];
+                                    gm_tmem8(tmem + ((uint32_t)quarter << 21) + j, v);
+                                    gm_loaded(v);
+#pragma unroll
+                                    for (int i = 0; i < 8; i++) o[i] = gm_scaled<X>((int32_t)v[i], sa, columns[j + i]);
+                                  });
+      gm_group_sync(1, GR_T);  // (the results passed through the tile's place)
+    }
+  }
+  if (!ok) {  // the copies that are on their way
+    for (int i = at; i < min(rows, at + slots); i += GR_WARPS) gm_wait_all(fullAt + i % slots * 8, i / slots & 1);
+    gm_wait_all(gm_smem(&bFull), 0);
+  }
+  if (!ok) atomicExch(&denseErr, 203);
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------------
 int64_t dense_status(int device) {
   (void)device;
@@ -889,6 +1117,11 @@ static int gemm_blocks(const GemmCall& c) {  // stages of a segment
 }
 bool gemm_quantizes(int64_t M, int64_t K, int type) { return M <= 16 && K > 0 && M * K * type_bytes(type) <= 32 << 10; }
 
+// (16 rows and fewer: k_gemm_few, with the columns over all SMs. FP32, 300 values a row, 128 columns: 1000 rows in 10.7 us a call and 7.7 us of the
+// device's, quantised by a kernel of their own 15.4 and 6.6; 6000 rows 9.5 and 9.6 us of the device's; FP64, 200 values, 256 columns: 1000 rows 12.4 and
+// 6.6 us, 6000 rows 14.5 and 15.9. 100,003 FP64 rows of 501 values, 64 columns: 85 and 130 us.)
+bool gemm_scores(int64_t M, int64_t N, int64_t K, int type) { return M > 16 && (N <= 128 || M >= 4096) && rows_plan(N, K, type).fits; }
+
 static GemmPlan find_plan(const GemmCall& c) {
   GemmPlan best;
   const int nk = gemm_blocks(c) * (c.kind == GK_SUM ? 2 : 1);
@@ -946,7 +1179,7 @@ static GemmPlan gemm_plan(const GemmCall& c) {
   return k.plan;
 }
 int64_t gemm_workspace(const GemmCall& c) {
-  if (c.M == 0 || c.N == 0) return 0;
+  if (c.M == 0 || c.N == 0 || c.scores) return 0;
   const GemmPlan p = gemm_plan(c);
   return p.large || p.whole ? 0 : gf_parts_bytes(p.ctas, c.kind == GK_GATE ? 2 : 1, p.nc) + 64;
 }
@@ -1017,10 +1250,36 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   return CLA_OK;
 }
 
+template <class X>
+static int64_t launch_rows(GemmArgs& A, cudaStream_t s) {
+  const GemmCall& c = A.c;
+  const RowsPlan p = rows_plan(c.N, c.K, c.outType);
+  A.kBlocks = p.kb, A.wide = p.wide, A.nc = p.slot, A.stages = p.slots;
+  A.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.wide >> 3) << 17 | (128u >> 4) << 24;
+  if (const int64_t rc = operand_map(A.b[0], c.b[0], CLA_T_I8, c.N, c.K, p.wide); rc < 0) return rc;
+  const auto go = [&](auto kernel, OncePerDevice& once) -> int64_t {
+    int room;
+    if (const int64_t e = all_smem(once, &room, c.device, kernel); e < 0) return e;
+    EarlyLaunch l((unsigned)std::min<int64_t>(GM_SMS, (c.M + GR_WARPS - 1) / GR_WARPS), GR_T, GR_ROOM, s, false);
+    CLA_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, A));
+    return CLA_OK;
+  };
+  static OncePerDevice once[3];
+  if (p.kb <= 2) return go(k_gemm_rows<X, 2, 2>, once[0]);
+  if (p.kb <= 4) return go(k_gemm_rows<X, sizeof(X) == 8 ? 1 : 2, 4>, once[1]);
+  return go(k_gemm_rows<X, 1, 0>, once[2]);
+}
+
 int64_t launch_gemm(const GemmCall& c, cudaStream_t s) {
   if (c.M == 0 || c.N == 0) return CLA_OK;
   GemmArgs A = {};
   A.c = c;
+  if (c.scores) {
+    if (c.outType == CLA_T_F64) return launch_rows<double>(A, s);
+    if (c.outType == CLA_T_F32) return launch_rows<float>(A, s);
+    if (c.outType == CLA_T_BF16) return launch_rows<__nv_bfloat16>(A, s);
+    return launch_rows<__half>(A, s);
+  }
   if (c.kind == GK_Q8) {
     if (c.outType == CLA_T_F64) return launch_kind<GK_Q8, double>(A, s);
     if (c.outType == CLA_T_F32) return launch_kind<GK_Q8, float>(A, s);

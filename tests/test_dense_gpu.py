@@ -161,6 +161,29 @@ def test_q8_linear(M, N, K, dtype, pad):
         assert bool(torch.isnan(y[0]).all()) and not bool(torch.isnan(y[1:]).any())
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("pad", [0, 3, 16])
+@pytest.mark.parametrize("M,N,K", [(17, 1, 1), (300, 32, 100), (2500, 64, 501), (5000, 33, 128), (20011, 10, 20), (150, 256, 500), (1999, 200, 129),
+                                   (700, 64, 1024), (40, 256, 1100)])
+def test_q8_scores(M, N, K, dtype, pad):
+    """Many rows against few columns, rows of zeros, of an infinity, of a NaN and of tiny values among them."""
+    x, w = normal(M, K, dtype, 3, pad=pad), normal(K, N, torch.float32, 4)
+    x[M // 3], x[M // 2, K // 2], x[M - 2, K - 1] = 0, float("inf"), float("nan")
+    x[M - 1] *= 1e-6
+    b, sb = CLALibQ8.quantizeCols(w)
+    qa, sa = ref.quantize(x)
+    out, intact = framed(M, N, dtype)
+    CLALibQ8.linear(x, b, sb, out=out)
+    bad = torch.tensor([M // 2, M - 2])
+    good = torch.ones(M, dtype=torch.bool)
+    good[bad] = False
+    want = q8_want(qa[good], sa[good], b.cpu().numpy(), sb.cpu().numpy())
+    ref.close(out[good.cuda()], want, q8_bound(want, dtype))
+    assert intact() and bool(torch.isnan(out[bad.cuda()]).all())
+    whole = CLALibQ8.linear(x, b, sb)
+    assert torch.equal(whole[good.cuda()], out[good.cuda()])
+
+
 def test_q8_largest_sums():
     """The longest sums that are taken, every term at its largest: -128 * -128 * 131071 = 2^31 - 2^14."""
     K = 131071
