@@ -403,6 +403,11 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
           uint32_t v[16];
           gm_tmem8(at + j, v);
           gm_tmem8(at + A.wide + j, v + 8);
+          uint4 words[2];  // (while the sums come)
+          if (c.drop.on) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) words[q] = drop_words(c.drop, (uint32_t)m, (uint32_t)((n0 + j) / 4 + q));
+          }
           gm_loaded(v);
           float h[8];
           with_act(c.act, [&](auto act) {
@@ -412,9 +417,8 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
           if (c.drop.on) {
 #pragma unroll
             for (int q = 0; q < 8; q += 4) {
-              const uint4 w = drop_words(c.drop, (uint32_t)m, (uint32_t)((n0 + j + q) / 4));
 #pragma unroll
-              for (int i = 0; i < 4; i++) h[q + i] = word_of(w, i) >= c.drop.cut ? h[q + i] * c.drop.scale : 0.f;
+              for (int i = 0; i < 4; i++) h[q + i] = word_of(words[q / 4], i) >= c.drop.cut ? h[q + i] * c.drop.scale : 0.f;
             }
           }
 #pragma unroll
