@@ -69,7 +69,7 @@ def _result(out, shape, dtype, like, what: str):
         return like.new_empty(shape) if like.dtype == dtype else torch.empty(shape, dtype=dtype, device=like.device)
     if not isinstance(out, torch.Tensor):
         _fail(-2, f"{what}: a CUDA tensor is needed")
-    if tuple(out.shape) != tuple(shape):
+    if out.shape != shape:
         _fail(-4, f"{what}: shape {tuple(out.shape)}, expected {tuple(shape)}")
     return out
 
@@ -83,6 +83,11 @@ def _type(dtype, what: str) -> int:
 
 def _workspace(n: int, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _workspace_like(n: int, t):
+    """The same, by the quicker way where a tensor is at hand."""
+    return t.new_empty(-(-n // t.element_size()))
 
 
 def _drop(p, seed, step, row0) -> native.cla_drop:
@@ -153,7 +158,7 @@ class CLALibQ8:
         ref = C.byref(args)
         n = check(L.cla_q8_workspace(ref))
         if n:
-            work = _workspace(n, a.device)
+            work = _workspace_like(n, a)
             args.work, args.workBytes = work.data_ptr(), n
         check(L.cla_q8_mm_dev(ref, _stream(dev)))
         return y
@@ -225,11 +230,11 @@ class CLALibGated:
         return c
 
     @staticmethod
-    def _run(c, backward, device):
+    def _run(c, backward, x):
         L, ref = native.lib(), C.byref(c)
         n = check(L.cla_gated_workspace(ref, backward))
         if n:
-            work = _workspace(n, device)
+            work = _workspace_like(n, x)
             c.work, c.workBytes = work.data_ptr(), n
         check((L.cla_gated_bwd_dev if backward else L.cla_gated_fwd_dev)(ref, _stream(c.device)))
 
@@ -239,12 +244,12 @@ class CLALibGated:
         dropout of H, as ``CLALibDropout.apply``."""
         c = CLALibGated._args(x, wGate, wUp, act, p, seed, step, row0)
         h = _result(out, (c.M, c.F), x.dtype, x, "gated block, out")
-        c.h, c.ldh = _rows(h, "gated block, out", x.dtype, c.device)
+        c.h, c.ldh = (h.data_ptr(), c.F) if out is None else _rows(h, "gated block, out", x.dtype, c.device)
         if save:
             g, u = x.new_empty((c.M, c.F)), x.new_empty((c.M, c.F))
             c.g, c.u = g.data_ptr(), u.data_ptr()
             c.ldg = c.ldu = c.F
-        CLALibGated._run(c, 0, x.device)
+        CLALibGated._run(c, 0, x)
         return (h, g, u) if save else h
 
     @staticmethod
@@ -253,10 +258,10 @@ class CLALibGated:
         """``(dX, dWg, dWu)`` from the gradient of H and what ``forward(..., save=True)`` gave, with the same activation and dropout
         arguments; dX or the weights' gradients are None where not needed."""
         c = CLALibGated._args(x, wGate, wUp, act, p, seed, step, row0)
-        dev = c.device
+        dev, M, F = c.device, c.M, c.F
         for t, what in ((dH, "dH"), (g, "g"), (u, "u")):
-            if not isinstance(t, torch.Tensor) or tuple(t.shape) != (c.M, c.F):
-                _fail(-4, f"gated block, {what}: expected [{c.M}, {c.F}]")
+            if not isinstance(t, torch.Tensor) or t.shape != (M, F):
+                _fail(-4, f"gated block, {what}: expected [{M}, {F}]")
         c.dh, c.lddh = _rows(dH, "gated block, dH", x.dtype, dev)
         c.g, c.ldg = _rows(g, "gated block, g", x.dtype, dev)
         c.u, c.ldu = _rows(u, "gated block, u", x.dtype, dev)
@@ -268,7 +273,7 @@ class CLALibGated:
             dwg, dwu = x.new_empty((c.D, c.F)), x.new_empty((c.D, c.F))
             c.dwg, c.dwu = dwg.data_ptr(), dwu.data_ptr()
             c.lddwg = c.lddwu = c.F
-        CLALibGated._run(c, 1, x.device)
+        CLALibGated._run(c, 1, x)
         return dx, dwg, dwu
 
 
