@@ -394,6 +394,22 @@ def test_offsets_beyond_32_bits():
     torch.cuda.empty_cache()
 
 
+def test_scores_of_more_than_32_bits_of_values():
+    M, K, N = 4_400_003, 500, 33
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, M // 2, M - 700, M - 1]
+    x[at] = normal(5, K, torch.bfloat16, 1)
+    b, sb = CLALibQ8.quantizeCols(normal(K, N, torch.float32, 2))
+    got = CLALibQ8.linear(x, b, sb)
+    qa, sa = ref.quantize(x[at])
+    want = q8_want(qa, sa, b.cpu().numpy(), sb.cpu().numpy())
+    ref.close(got[at], want, q8_bound(want, torch.bfloat16))
+    got[at] = 0
+    assert not bool(got.any())
+    del x, got
+    torch.cuda.empty_cache()
+
+
 def test_a_row_of_two_gigabytes_off_its_boundary():
     D = 1 << 30
     x = torch.zeros(D + 1, dtype=torch.bfloat16, device="cuda")[1:].reshape(1, D)
@@ -485,6 +501,29 @@ def test_compressed_block_through_the_layers():
         CLALibDecompress.rows(cmb, 4000, 1001, torch.float32)
     with pytest.raises(CLAError):
         CLALibQ8.rightMultByMatrix(cmb, b[:, 1:], sb)
+    cmb.free()
+
+
+@pytest.mark.parametrize("N", [5, 140, 300])
+def test_scores_of_a_block_in_the_smallest_chunks(N):
+    """Chunks of 1024 rows, the last of nine: the same results as in one, in every type."""
+    cmb = datagen.random_cmb(4, 2 * 1024 + 9, datagen.KINDS).to_device(0)
+    n, m = 2 * 1024 + 9, cmb.clen
+    b, sb = CLALibQ8.quantizeCols(normal(m, N, torch.float64, 9))
+    rows = CLALibDecompress.rows(cmb, 0, n, torch.float64)
+    up = lambda v: -(-v // 256) * 256  # noqa: E731
+    pitch = -(-m // 128) * 128
+    size = up(1024 * pitch) + up(1024 * 4) + up(1024 * m * 8) + up(N * pitch)
+    L = native.lib()
+    for code, dtype in enumerate(FLOATS):
+        out, intact = framed(n, N, dtype)
+        work = torch.empty(size, dtype=torch.uint8, device="cuda")
+        call = lambda bytes: L.cla_q8_rmm_dev(cmb.handle(), b.data_ptr(), b.stride(0), sb.data_ptr(), N, code, out.data_ptr(), out.stride(0),  # noqa: E731
+                                              work.data_ptr(), bytes, torch.cuda.current_stream().cuda_stream)
+        with pytest.raises(CLAError):
+            native.check(call(size // 2))
+        native.check(call(size))
+        assert torch.equal(out, CLALibQ8.linear(rows, b, sb, dtype=dtype)) and intact()
     cmb.free()
 
 
