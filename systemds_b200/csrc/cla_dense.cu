@@ -459,15 +459,19 @@ int64_t quantize(int type, const void* x, int64_t ldx, int64_t rows, int64_t col
     }
     constexpr int V = DN_V<T>, C = sizeof(T) == 8 ? 8 : 4;
     const bool vec = rows_aligned(x, ldx, rows, sizeof(T)) && rows_aligned(q, ldq, rows, 1, V);
-    // the fewest threads that hold the row, where there are rows enough for all SMs: a warp (no barrier), half a CTA, a CTA
-    const int group = rows < 148 ? DN_T : cols <= 32 * C * V ? 32 : cols <= 128 * C * V ? 128 : DN_T;
+    // the fewest threads that hold the row: a warp (no barrier), two, half a CTA, a CTA (50,000 rows of 520 FP64 values: by two warps 69 us, by four 128,
+    // most of them idle). More where rows are too few for that to matter: a CTA where there is not one for every SM, 16 values of 16 bits a thread
+    // while there are not two for every SM (they are divided more often: 500 x 2000 by two warps 6.8 us, by a CTA 4.0)
+    int group = 32;
+    while (group < DN_T && (cols > group * C * V || rows < 148 || (sizeof(T) == 2 && cols > group * 16 && rows * group < 148 * 2 * DN_T))) group *= 2;
     auto go = [&](auto kernel, OncePerDevice& once) {
       rc = once(device, [&] { return like_products(kernel); });
       const int down = DN_T / group;
       if (rc >= 0) kernel<<<(unsigned)((rows + down - 1) / down), DN_T, 0, s>>>((const T*)x, ldx, rows, (int)cols, q, ldq, scale);
     };
-    static OncePerDevice once[6];
+    static OncePerDevice once[8];
     if (group == 32) vec ? go(k_quantize_rows<T, 32, C, true>, once[0]) : go(k_quantize_rows<T, 32, C, false>, once[1]);
+    else if (group == 64) vec ? go(k_quantize_rows<T, 64, C, true>, once[6]) : go(k_quantize_rows<T, 64, C, false>, once[7]);
     else if (group == 128) vec ? go(k_quantize_rows<T, 128, C, true>, once[2]) : go(k_quantize_rows<T, 128, C, false>, once[3]);
     else vec ? go(k_quantize_rows<T, DN_T, C, true>, once[4]) : go(k_quantize_rows<T, DN_T, C, false>, once[5]);
   });
