@@ -838,6 +838,8 @@ __global__ void __launch_bounds__(128) k_gemm_join(const __grid_constant__ GemmA
 // Bound: memory next to the instructions of the quantisation (100,003 rows of 501 values, 64 columns: FP64 85 us, 5.3 TB/s; FP32 57 us, BF16 66 us, where
 // the issue slots are 55 % busy).
 constexpr int GR_WARPS = 16, GR_T = GR_WARPS * 32, GR_SLOTS = 128, GR_ROOM = 223 * 1024;
+// Blocks of a row's depth up to which a warp takes two rows at once
+constexpr int gr_pairs(int bytes) { return bytes == 8 ? 2 : 4; }
 struct RowsPlan {
   int kb, wide, slot, slots;  // blocks of the depth; columns with those that are not there; bytes of a row in the ring, rows
   bool fits = false;
@@ -851,7 +853,10 @@ static RowsPlan rows_plan(int64_t N, int64_t K, int type) {
   p.slot = (int)round_up(K * type_bytes(type), 16) + 16;
   const int left = GR_ROOM - 1024 - std::max(p.kb * (int)GM_OPERAND, 4 * 8192) - p.kb * p.wide * 128;
   p.slots = left > 0 ? std::min(GR_SLOTS, left / p.slot / GR_WARPS * GR_WARPS) : 0;
-  p.fits = p.slots == GR_SLOTS || (p.slots >= 2 * GR_WARPS && p.slots * p.slot >= 24 << 10);  // (two rows a warp)
+  // one place a warp is enough where a row takes long to come: 100,003 x 640 FP64, 64 columns 119 us, by two kernels 174, FP32 x 700 99 and 117; 16 bits x 1000,
+  // 16 columns 130 and 117
+  const int least = type_bytes(type) > 2 && p.kb > gr_pairs(type_bytes(type)) ? 1 : 2;
+  p.fits = p.slots == GR_SLOTS || (p.slots >= least * GR_WARPS && p.slots * p.slot >= 24 << 10);
   return p;
 }
 
@@ -1270,7 +1275,7 @@ static int64_t launch_rows(GemmArgs& A, cudaStream_t s) {
   };
   static OncePerDevice once[3];
   if (p.kb <= 2) return go(k_gemm_rows<X, 2, 2>, once[0]);
-  if (p.kb <= 4) return go(k_gemm_rows<X, sizeof(X) == 8 ? 1 : 2, 4>, once[1]);
+  if (p.kb <= 4) return go(k_gemm_rows<X, gr_pairs(sizeof(X)) == 4 ? 2 : 1, 4>, once[1]);
   return go(k_gemm_rows<X, 1, 0>, once[2]);
 }
 

@@ -164,7 +164,7 @@ def test_q8_linear(M, N, K, dtype, pad):
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("pad", [0, 3, 16])
 @pytest.mark.parametrize("M,N,K", [(17, 1, 1), (300, 32, 100), (2500, 64, 501), (5000, 33, 128), (20011, 10, 20), (150, 256, 500), (1999, 200, 129),
-                                   (700, 64, 1024), (40, 256, 1100)])
+                                   (700, 64, 1024), (40, 256, 1100), (2300, 64, 640), (333, 100, 700), (5000, 16, 1000)])
 def test_q8_scores(M, N, K, dtype, pad):
     """Many rows against few columns, rows of zeros, of an infinity, of a NaN and of tiny values among them."""
     x, w = normal(M, K, dtype, 3, pad=pad), normal(K, N, torch.float32, 4)
