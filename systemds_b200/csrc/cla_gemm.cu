@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
   constexpr bool I8 = KIND == GK_Q8;
   constexpr int OUT = gp_out(KIND, sizeof(O)), G = OUT / 4;  // warps that write results, and of each 32 rows of a tile
   extern __shared__ __align__(1024) unsigned char gmsm[];
-  __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumEmpty[2];
+  __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumRead[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
   const GemmCall& c = A.c;
   const int lane = threadIdx.x & 31, warp = gm_warp();
@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
     }
     for (int i = 0; i < 2; i++) {
       gm_init(gm_smem(sumFull + i), 1);
-      gm_init(gm_smem(sumEmpty + i), 2 * OUT);  // the warps of both CTAs
+      gm_init(gm_smem(sumRead + i), OUT);
+      gm_init(gm_smem(sumEmpty + i), 2);  // both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -383,6 +384,19 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
         }
       }
     }
+  } else if (warp == 3) {
+    // Tells the first CTA that this one's sums have been read. Not a matter for the warps that read them: an arrival at another CTA waits for all that a
+    // warp has written, which for their results took 2000 clocks a tile.
+    int n = 0;
+    for (int t = pair; t + 2 * pairs < tiles; t += pairs, n++) {  // (somebody waits for it: no arrival on its way when the CTAs end)
+      const int buf = n & 1;
+      ok = gm_wait_all(gm_smem(sumRead + buf), (n >> 1) & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gm_peer(gm_smem(sumEmpty + buf), 0)) : "memory");
+      __syncwarp();
+    }
   } else if (warp >= 4) {
     const int quarter = warp & 3, part = (warp - 4) >> 2;  // of the rows, of the columns
     int n = 0;
@@ -456,8 +470,7 @@ __global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __clust
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0 && t + 2 * pairs < tiles)  // (somebody waits for it: no arrival on its way when the CTAs end)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gm_peer(gm_smem(sumEmpty + buf), 0)) : "memory");
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(gm_smem(sumRead + buf)) : "memory");
     }
   }
   if (c.after == AFTER_NONE) gm_after_previous();
