@@ -268,10 +268,29 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
                                                        int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w) {
   constexpr int V = DN_V<T>, N = V / 4;
   const int64_t r0 = walk_first(w), step = walk_step(w);
+  // Rows that start anywhere: the words that hold the values, put in place when they are used (before, whoever asked for them waited)
+  struct Words {
+    uint32_t w[VEC ? 4 : 5];
+    __device__ __forceinline__ void load(const T* p, int left) {
+      if constexpr (VEC) {
+        T v[V];
+        load_vec(p, left, true, v);
+        memcpy(w, v, 16);
+      } else {
+        const uint32_t off = (uint32_t)(uintptr_t)p & 2, end = off + 2 * min(left, V);
+        const uint32_t* from = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+#pragma unroll
+        for (int k = 0; k < 5; k++) w[k] = 4 * k < end ? __ldg(from + k) : 0u;
+      }
+    }
+    __device__ __forceinline__ void place(const T* p) {
+      if constexpr (!VEC)
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(w[k], w[k + 1], ((uint32_t)(uintptr_t)p & 2) * 8);
+    }
+  };
   struct Values {
-    alignas(16) T h[V];
-    alignas(16) T g[V];
-    alignas(16) T u[V];
+    Words h, g, u;
   };
   struct Kept {
     int64_t c;
@@ -281,9 +300,9 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
   };
   gm_let_next();
   auto load = [&](int64_t r, int64_t c, int left, Values& v) {
-    load_vec(dh + r * lddh + c, left, VEC, v.h);
-    load_vec(g + r * ldg + c, left, VEC, v.g);
-    load_vec(u + r * ldu + c, left, VEC, v.u);
+    v.h.load(dh + r * lddh + c, left);
+    v.g.load(g + r * ldg + c, left);
+    v.u.load(u + r * ldu + c, left);
   };
   with_act(act, [&](auto name) {
     walk<1>(
@@ -297,6 +316,10 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
         [&](Kept& k, int64_t r, int64_t, int) {
           Values v = k.next;
           if (r + step < w.rows) load(r + step, k.c, k.left, k.next);
+          v.h.place(dh + r * lddh);
+          v.g.place(g + r * ldg);
+          v.u.place(u + r * ldu);
+          alignas(16) uint32_t toG[V / 2], toU[V / 2];
 #pragma unroll
           for (int q = 0; q < V; q += 4) {
             uint4 words;
@@ -304,9 +327,9 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
 #pragma unroll
             for (int j = 0; j < 4; j += 2) {
               float h[2], gate[2], up[2];
-              from_word<T>(*(const uint32_t*)(v.h + q + j), h[0], h[1]);
-              from_word<T>(*(const uint32_t*)(v.g + q + j), gate[0], gate[1]);
-              from_word<T>(*(const uint32_t*)(v.u + q + j), up[0], up[1]);
+              from_word<T>(v.h.w[(q + j) / 2], h[0], h[1]);
+              from_word<T>(v.g.w[(q + j) / 2], gate[0], gate[1]);
+              from_word<T>(v.u.w[(q + j) / 2], up[0], up[1]);
 #pragma unroll
               for (int i = 0; i < 2; i++) {
                 float a;
@@ -315,12 +338,12 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
                 gate[i] = h[i] * up[i] * slope;
                 up[i] = h[i] * a;
               }
-              *(uint32_t*)(v.g + q + j) = to_word<T>(gate[0], gate[1]);
-              *(uint32_t*)(v.u + q + j) = to_word<T>(up[0], up[1]);
+              toG[(q + j) / 2] = to_word<T>(gate[0], gate[1]);
+              toU[(q + j) / 2] = to_word<T>(up[0], up[1]);
             }
           }
-          store_vec(dg + r * ldo + k.c, k.left, true, v.g);
-          store_vec(du + r * ldo + k.c, k.left, true, v.u);
+          store_vec(dg + r * ldo + k.c, k.left, true, (const T(&)[V])toG);
+          store_vec(du + r * ldo + k.c, k.left, true, (const T(&)[V])toU);
         });
   });
   gm_after_previous();  // (the copies next to this: who waits for this kernel has waited for both)
