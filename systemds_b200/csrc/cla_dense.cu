@@ -54,24 +54,83 @@ __device__ __forceinline__ DropPieces<N> drop_pieces(const DropDev& d, int64_t c
   else return {{DropColumns(d, (uint32_t)(c / 4)), DropColumns(d, (uint32_t)(c / 4) + 1)}};
 }
 
+// V values of a row, on their way until they are used. VEC: from a 16-byte boundary; else 16-bit values come as the words that hold them, which are put
+// in place when they are used (before, whoever asked for them waited: the gradients of 4069 x 8315 gates took 131 us, and 78 so).
+// (not through the read-only path: dropout's result may go where its operand is)
+template <class T, bool VEC, int V, bool SHIFTED = !VEC && sizeof(T) == 2>
+struct Words {
+  alignas(16) T v[V];
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if constexpr (sizeof(T) == 8 && !VEC) {
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = i < left ? p[i] : T(0);
+    } else {
+#pragma unroll
+      for (int h = 0; h < V; h += DN_V<T>) load_vec(p + h, left - h, VEC, (T(&)[DN_V<T>])v[h]);
+    }
+  }
+  __device__ __forceinline__ void place(const T*, T (&to)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; i++) to[i] = v[i];
+  }
+};
+template <class T, bool VEC, int V>
+struct Words<T, VEC, V, true> {
+  uint32_t w[V / 2 + 1];
+  __device__ __forceinline__ void load(const T* p, int left) {
+    const uint32_t off = (uint32_t)(uintptr_t)p & 2, end = off + 2 * min(left, V);
+    const uint32_t* from = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+#pragma unroll
+    for (int k = 0; k <= V / 2; k++) w[k] = 4 * k < end ? from[k] : 0u;
+  }
+  __device__ __forceinline__ void place(const T* p, T (&to)[V]) const {
+#pragma unroll
+    for (int k = 0; k < V / 2; k++) ((uint32_t*)to)[k] = __funnelshift_r(w[k], w[k + 1], ((uint32_t)(uintptr_t)p & 2) * 8);
+  }
+};
+// The same for a warp's results, V a lane, side by side in a row that starts anywhere: through the warp's place in shared memory (32 lanes' values
+// and a word), so that a store's words lie together. lanes: how many of the warp are there, the first ones; count: values.
+template <class T, int V>
+__device__ __forceinline__ void store_across(T* to, int64_t count, const T (&v)[V], uint32_t* place, int lanes) {
+  constexpr int N = V * (int)sizeof(T) / 4;
+  const uint32_t lane = threadIdx.x & 31, mask = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1;
+  const int off = (int)((uintptr_t)to & 2), end = off + (int)count * (int)sizeof(T);
+  char* base = (char*)to - off;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) *(uint4*)(place + 4 + lane * N + i) = ((const uint4*)v)[i / 4];
+  __syncwarp(mask);
+  const auto word = [&](int k) { return off ? __funnelshift_r(place[3 + k], place[4 + k], 16) : place[4 + k]; };
+  const auto put = [&](int k) {
+    if ((k > 0 || off == 0) && 4 * k + 4 <= end) *(uint32_t*)(base + 4 * k) = word(k);
+    else if (k == 0 && off) *(uint16_t*)(base + 2) = (uint16_t)(word(0) >> 16);
+    else *(uint16_t*)(base + 4 * k) = (uint16_t)word(k);
+  };
+  if (count == 32 * V) {
+    put(lane);
+#pragma unroll
+    for (int i = 1; i < N; i++) *(uint32_t*)(base + 4 * (lane + 32 * i)) = word(lane + 32 * i);
+    if (off && lane == 0) *(uint16_t*)(base + 128 * N) = (uint16_t)word(32 * N);
+  } else {
+    for (int k = lane; 4 * k < end; k += lanes) put(k);
+  }
+  __syncwarp(mask);
+}
+
 // ---- dropout --------------------------------------------------------------------------------------------------------
 // Pieces of 16 bytes (F64: 32, the four columns of a counter). Bound: the words (sixteen 64-bit products and as many three-way logic
 // operations for four columns) next to memory.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, int64_t cols, T* y, int64_t ldy, const __grid_constant__ DropDev d,
-                                                     const __grid_constant__ Walk w) {
+__global__ void __launch_bounds__(DN_T, VEC ? 5 : 4) k_dropout(const T* x, int64_t ldx, int64_t cols, T* y, int64_t ldy, const __grid_constant__ DropDev d,
+                                                               const __grid_constant__ Walk w) {
   constexpr int P = DN_V<T>, V = P < 4 ? 4 : P, N = V / 4;
+  __shared__ __align__(16) uint32_t places[VEC ? 1 : DN_T / 32][VEC ? 1 : 32 * V * sizeof(T) / 4 + 4 + 4];
   struct Kept {
     const T* x;
     T* y;
     int64_t stepX, stepY;
     int left;
     DropPieces<N> drop;
-    alignas(16) T next[V];  // the next row's values: on their way while a row's are worked on
-  };
-  auto load = [&](Kept& k) {
-#pragma unroll
-    for (int h = 0; h < V; h += P) load_vec(k.x + h, k.left - h, VEC, (T(&)[P])k.next[h]);
+    Words<T, VEC, V> next;  // the next row's values: on their way while a row's are worked on
   };
   const int64_t r0 = walk_first(w), step = walk_step(w);
   walk<1>(
@@ -79,15 +138,16 @@ __global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, in
       [&](int piece) {
         const int64_t c = (int64_t)piece * V;
         Kept k{x + r0 * ldx + c, y + r0 * ldy + c, step * ldx, step * ldy, (int)min((int64_t)V, cols - c), drop_pieces<N>(d, c), {}};
-        if (r0 < w.rows) load(k);
+        if (r0 < w.rows) k.next.load(k.x, k.left);
         return k;
       },
       [&](Kept& k, int64_t r, int64_t, int) {
-        alignas(16) T v[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = k.next[i];
+        const Words<T, VEC, V> here = k.next;
+        const T* from = k.x;
         k.x += k.stepX;
-        if (r + step < w.rows) load(k);
+        if (r + step < w.rows) k.next.load(k.x, k.left);
+        alignas(16) T v[V];
+        here.place(from, v);
         if (d.on) {
 #pragma unroll
           for (int q = 0; q < V; q += 4) {
@@ -110,8 +170,17 @@ __global__ void __launch_bounds__(DN_T, 5) k_dropout(const T* x, int64_t ldx, in
             }
           }
         }
+        if constexpr (VEC) {
 #pragma unroll
-        for (int h = 0; h < V; h += P) store_vec(k.y + h, k.left - h, VEC, (const T(&)[P])v[h]);
+          for (int h = 0; h < V; h += P) store_vec(k.y + h, k.left - h, true, (const T(&)[P])v[h]);
+        } else if (sizeof(T) != 4 && w.log >= 5) {  // (a warp is in one row; FP32 values are words already: 252 us for 16384 x 8191, through shared memory 304)
+          const int lane = threadIdx.x & 31;
+          const int64_t there = cols - (k.y - y - r * ldy) + (int64_t)lane * V;  // from the warp's first value on
+          store_across<T, V>(k.y - lane * V, min((int64_t)32 * V, there), v, places[threadIdx.x / 32], (int)min((int64_t)32, (there + V - 1) / V));
+        } else {
+#pragma unroll
+          for (int h = 0; h < V; h += P) store_vec(k.y + h, k.left - h, false, (const T(&)[P])v[h]);
+        }
         k.y += k.stepY;
       });
 }
@@ -268,29 +337,8 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
                                                        int64_t ldo, const __grid_constant__ DropDev d, int act, const __grid_constant__ Walk w) {
   constexpr int V = DN_V<T>, N = V / 4;
   const int64_t r0 = walk_first(w), step = walk_step(w);
-  // Rows that start anywhere: the words that hold the values, put in place when they are used (before, whoever asked for them waited)
-  struct Words {
-    uint32_t w[VEC ? 4 : 5];
-    __device__ __forceinline__ void load(const T* p, int left) {
-      if constexpr (VEC) {
-        T v[V];
-        load_vec(p, left, true, v);
-        memcpy(w, v, 16);
-      } else {
-        const uint32_t off = (uint32_t)(uintptr_t)p & 2, end = off + 2 * min(left, V);
-        const uint32_t* from = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
-#pragma unroll
-        for (int k = 0; k < 5; k++) w[k] = 4 * k < end ? __ldg(from + k) : 0u;
-      }
-    }
-    __device__ __forceinline__ void place(const T* p) {
-      if constexpr (!VEC)
-#pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(w[k], w[k + 1], ((uint32_t)(uintptr_t)p & 2) * 8);
-    }
-  };
   struct Values {
-    Words h, g, u;
+    Words<T, VEC, V> h, g, u;
   };
   struct Kept {
     int64_t c;
@@ -316,10 +364,10 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
         [&](Kept& k, int64_t r, int64_t, int) {
           Values v = k.next;
           if (r + step < w.rows) load(r + step, k.c, k.left, k.next);
-          v.h.place(dh + r * lddh);
-          v.g.place(g + r * ldg);
-          v.u.place(u + r * ldu);
-          alignas(16) uint32_t toG[V / 2], toU[V / 2];
+          alignas(16) T inH[V], inG[V], inU[V], toG[V], toU[V];
+          v.h.place(dh + r * lddh, inH);
+          v.g.place(g + r * ldg, inG);
+          v.u.place(u + r * ldu, inU);
 #pragma unroll
           for (int q = 0; q < V; q += 4) {
             uint4 words;
@@ -327,9 +375,9 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
 #pragma unroll
             for (int j = 0; j < 4; j += 2) {
               float h[2], gate[2], up[2];
-              from_word<T>(v.h.w[(q + j) / 2], h[0], h[1]);
-              from_word<T>(v.g.w[(q + j) / 2], gate[0], gate[1]);
-              from_word<T>(v.u.w[(q + j) / 2], up[0], up[1]);
+              from_word<T>(*(const uint32_t*)(inH + q + j), h[0], h[1]);
+              from_word<T>(*(const uint32_t*)(inG + q + j), gate[0], gate[1]);
+              from_word<T>(*(const uint32_t*)(inU + q + j), up[0], up[1]);
 #pragma unroll
               for (int i = 0; i < 2; i++) {
                 float a;
@@ -338,12 +386,12 @@ __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh,
                 gate[i] = h[i] * up[i] * slope;
                 up[i] = h[i] * a;
               }
-              toG[(q + j) / 2] = to_word<T>(gate[0], gate[1]);
-              toU[(q + j) / 2] = to_word<T>(up[0], up[1]);
+              *(uint32_t*)(toG + q + j) = to_word<T>(gate[0], gate[1]);
+              *(uint32_t*)(toU + q + j) = to_word<T>(up[0], up[1]);
             }
           }
-          store_vec(dg + r * ldo + k.c, k.left, true, (const T(&)[V])toG);
-          store_vec(du + r * ldo + k.c, k.left, true, (const T(&)[V])toU);
+          store_vec(dg + r * ldo + k.c, k.left, true, toG);
+          store_vec(du + r * ldo + k.c, k.left, true, toU);
         });
   });
   gm_after_previous();  // (the copies next to this: who waits for this kernel has waited for both)
