@@ -267,8 +267,9 @@ __device__ __forceinline__ O gm_scaled(int32_t sum, W sa, W sb) {
 constexpr int GP_STAGES = 10, GP_RING = 6 * 2 * GM_OPERAND, GP_GROUP = 8;
 
 // Warps that take the sums out. GATE: 16, for the activation and the dropout of a tile keep eight busy for twice as long as its products take at a
-// depth of 2048 (18 against 9 us: few instructions of a warp at a time are independent). FP64 results: 16 as well, for the conversions.
-__host__ __device__ constexpr int gp_out(int kind, int bytes) { return kind == GK_GATE || bytes == 8 ? 16 : 8; }
+// depth of 2048 (18 against 9 us: few instructions of a warp at a time are independent). 8 bits: 16 as well, for the conversions (8192 x 256 x 4097 to
+// BF16 56 to 60 us, by eight 65; FP32 61 and 69). The others: eight (64 x 1024 x 4096: 11.3 us, by 16 12.6).
+__host__ __device__ constexpr int gp_out(int kind) { return kind == GK_GATE || kind == GK_Q8 ? 16 : 8; }
 
 __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& tn) {
   const int per = GP_GROUP * A.tilesN, g = t / per, first = g * GP_GROUP, n = min(GP_GROUP, A.tilesM - first), r = t - g * per;
@@ -277,9 +278,9 @@ __device__ __forceinline__ void gp_tile(const GemmArgs& A, int t, int& tm, int& 
 }
 
 template <int KIND, class O>
-__global__ void __launch_bounds__(128 + gp_out(KIND, sizeof(O)) * 32, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
+__global__ void __launch_bounds__(128 + gp_out(KIND) * 32, 1) __cluster_dims__(2) k_gemm_pair(const __grid_constant__ GemmArgs A) {
   constexpr bool I8 = KIND == GK_Q8;
-  constexpr int OUT = gp_out(KIND, sizeof(O)), G = OUT / 4;  // warps that write results, and of each 32 rows of a tile
+  constexpr int OUT = gp_out(KIND), G = OUT / 4;  // warps that write results, and of each 32 rows of a tile
   extern __shared__ __align__(1024) unsigned char gmsm[];
   __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], sumFull[2], sumRead[2], sumEmpty[2];
   __shared__ uint32_t tmemAt;
@@ -1235,7 +1236,7 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
     if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
     static_assert(GP_RING + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
     const unsigned ctas = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
-    EarlyLaunch pair(ctas, 128 + gp_out(KIND, sizeof(O)) * 32, roomPair, s, c.after != AFTER_CALL);
+    EarlyLaunch pair(ctas, 128 + gp_out(KIND) * 32, roomPair, s, c.after != AFTER_CALL);
     CLA_CUDA(cudaLaunchKernelEx(&pair.cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
   }
