@@ -63,6 +63,28 @@ def test_dropout(dtype, rows, cols, pad):
         assert intact()
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,cols", [(7, 1101), (9, 301), (4, 259), (40, 5003), (1300, 257)])
+def test_dropout_of_rows_that_start_anywhere(dtype, rows, cols):
+    """Rows at every offset from a 16-byte boundary, into other rows at other offsets and onto themselves."""
+    f = ref.drop_factors(rows, cols, 0.25, 11, 3)
+    for start, ld in ((1, cols), (2, cols + 2), (3, cols + 5)):
+        flat = torch.full((start + rows * ld + 8,), float("nan"), device="cuda", dtype=dtype)
+        x = flat[start:start + rows * ld].view(rows, ld)[:, :cols]
+        x.copy_(normal(rows, cols, dtype, start))
+        keep = x.clone()
+        want = keep.double().cpu() * f
+        bound = want.abs() * (2.0 ** -52 if dtype == torch.float64 else ref.half_step(dtype) + 2.0 ** -22) + ref.tiny(dtype)
+        y, intact = framed(rows, cols, dtype)
+        CLALibDropout.apply(x, 0.25, 11, 3, out=y)
+        ref.close(y, want, bound)
+        assert intact() and torch.equal(x, keep)
+        CLALibDropout.apply(x, 0.25, 11, 3, out=x)
+        assert torch.equal(x, y)
+        x.fill_(float("nan"))
+        assert bool(torch.isnan(flat).all())
+
+
 def test_dropout_shards_draw_the_whole_mask_and_dropped_values_are_zero():
     x = normal(100, 333, torch.float32, 1)
     x[::3, ::2] = float("nan")
