@@ -172,42 +172,74 @@ __device__ __forceinline__ void q8_quotients(const Q8Row<typename WideOf<T>::typ
 }
 
 // ---- the activation, in FP32 ------------------------------------------------------------------------------------------
-// With the fast exponential and quotient: off by some units of 2^-23, under 2^-20 of the value where |g| < 10 (beyond, a unit more for each
-// of g's), next to the 2^-11 or 2^-8 of the rounding that follows.
-__device__ __forceinline__ float sigmoid_of(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+// Nothing here subtracts from 1 what has come near it: sigmoid(g) and sigmoid(-g) are both quotients of e = exp(-|g|), whose denominator is between 1 and
+// 2, and the normal distribution's share below -|g| is exp(-g^2 / 2) times a smooth function. So the tails keep their relative error, in units of 2^-23
+// (the fast exponential of x: 2 + 1.2 |x|, the fast quotient 2, the roundings of an argument x: |x|): SiLU and sigmoid 6 + 1.2 |g|, GELU 10 + 1.2 g^2,
+// its tanh form 6 + 3.2 |y| for sigmoid(y). Slopes two to three times that, of their terms' magnitudes. A rounding to 16 bits of 2^-8 or 2^-11 follows.
+struct Sigmoids {
+  float s, r;  // of g and of -g
+};
+__device__ __forceinline__ Sigmoids sigmoids_of(float g) {
+  const float e = __expf(-fabsf(g)), q = __fdividef(1.f, 1.f + e), t = e * q;
+  return g < 0.f ? Sigmoids{t, q} : Sigmoids{q, t};
+}
+__device__ __forceinline__ float sigmoid_of(float g) {
+  const float e = __expf(-fabsf(g));
+  return __fdividef(g < 0.f ? e : 1.f, 1.f + e);
+}
 // (1 + tanh(y)) / 2 is sigmoid(2 y)
 __device__ __forceinline__ float gelu_arg(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
+// The normal distribution's share below g, (1 + erf(g / sqrt 2)) / 2, and exp(-g^2 / 2). Below -a it is exp(-a^2 / 2) t R(t) with t = 1 / (1 + 0.28 a): R is a
+// polynomial fitted for the least relative error over all a >= 0 (1.7e-7; in FP32 4.4 units of 2^-23). One exponential serves value and
+// slope (forward of 4095 x 2048 x 5461 with dropout, saved: 190 us with erfcf, 179 so).
+struct Normal {
+  float share, e;
+};
+__device__ __forceinline__ Normal normal_of(float g) {
+  const float e = __expf(-0.5f * g * g), t = __fdividef(1.f, fmaf(0.28f, fabsf(g), 1.f));
+  float r = 0.0247199624f;
+  r = fmaf(r, t, -0.0935930849f);
+  r = fmaf(r, t, 0.0924280604f);
+  r = fmaf(r, t, -0.00644913645f);
+  r = fmaf(r, t, 0.0727749934f);
+  r = fmaf(r, t, 0.0836307955f);
+  r = fmaf(r, t, 0.103084664f);
+  r = fmaf(r, t, 0.111699803f);
+  r = fmaf(r, t, 0.111703858f);
+  const float tail = e * (t * r);
+  return {g < 0.f ? tail : 1.f - tail, e};
+}
 __device__ __forceinline__ float act_value(int act, float g) {
   switch (act) {
     case CLA_ACT_SILU: return g * sigmoid_of(g);
     case CLA_ACT_SIGMOID: return sigmoid_of(g);
     case CLA_ACT_RELU: return g < 0.f ? 0.f : g;
-    case CLA_ACT_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+    case CLA_ACT_GELU: return g * normal_of(g).share;
     default: return g * sigmoid_of(gelu_arg(g));
   }
 }
 __device__ __forceinline__ float act_slope(int act, float g, float& value) {
   switch (act) {
     case CLA_ACT_SILU: {
-      const float s = sigmoid_of(g);
-      value = g * s;
-      return s * (1.f + g * (1.f - s));
+      const Sigmoids v = sigmoids_of(g);
+      value = g * v.s;
+      return v.s * (1.f + g * v.r);
     }
     case CLA_ACT_SIGMOID: {
-      const float s = sigmoid_of(g);
-      value = s;
-      return s * (1.f - s);
+      const Sigmoids v = sigmoids_of(g);
+      value = v.s;
+      return v.s * v.r;
     }
     case CLA_ACT_RELU: value = g < 0.f ? 0.f : g; return g > 0.f ? 1.f : 0.f;
     case CLA_ACT_GELU: {
-      const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-      value = g * c;
-      return c + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
+      const Normal v = normal_of(g);
+      value = g * v.share;
+      return v.share + g * v.e * 0.39894228040143268f;
     }
     default: {
-      const float s = sigmoid_of(gelu_arg(g));
-      value = g * s;
-      return s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * fminf(g * g, 1e4f));  // (beyond, 1 - s or s is 0, and the square may be infinite)
+      const Sigmoids v = sigmoids_of(gelu_arg(g));
+      value = g * v.s;
+      return v.s + g * v.s * v.r * 1.5957691216057308f * (1.f + 0.134145f * fminf(g * g, 1e4f));  // (beyond, s or r is 0, and the square may be infinite)
     }
   }
 }

@@ -1,0 +1,75 @@
+"""The dense operators on the GPU where a tail, another caller or an odd argument shows what the bounds of test_dense_gpu.py do not."""
+import math
+
+import pytest
+import torch
+
+from systemds_b200 import CLALibGated
+from systemds_b200.dense import status
+from tests import dense_ref as ref
+
+pytestmark = pytest.mark.gpu
+HALVES = (torch.bfloat16, torch.float16)
+
+
+@pytest.fixture(autouse=True)
+def no_check_trips():
+    yield
+    status()
+
+
+# ---- activations in their tails -----------------------------------------------------------------------------------------
+def gates_of(dtype, most):
+    """Every value of a 16-bit type from 2^-6 to `most` in magnitude, and zero."""
+    v = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    m = v.double().abs()
+    return torch.cat([v[(m >= 2.0 ** -6) & (m <= most)], torch.zeros(1, dtype=dtype)])
+
+
+def tail_forms(act, g):
+    """act(g), act'(g) without a cancelling sum, and the magnitudes that its relative error counts from (their sum may pass through zero), both with the
+    error of a float32 evaluation in units of 2^-23: a documented 2 + 1.173 |x| for the exponential of x, 2 for the quotient, what a rounding of the
+    argument x is worth, |x| / 2 each, 1/2 for each other rounding, and 4.4 for a polynomial of degree 8 in GELU's tail (2 + 1.173 g^2 / 2 + g^2 / 2 + 4.4 + 1 for that)."""
+    s, r = torch.sigmoid(g), torch.sigmoid(-g)
+    a = g.abs()
+    if act == "relu":
+        return g.clamp(min=0), (g > 0).double(), (g > 0).double(), 0 * a, 0 * a
+    if act == "sigmoid":
+        return s, s * r, s * r, 6 + 1.2 * a, 20 + 3.6 * a
+    if act == "silu":
+        return g * s, s + g * s * r, s + a * s * r, 6 + 1.2 * a, 20 + 3.6 * a
+    if act == "gelu":
+        c = 0.5 * torch.special.erfc(-g / math.sqrt(2))
+        p = g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+        return g * c, c + p, c + p.abs(), 10 + 1.2 * g * g, 12 + 1.2 * g * g
+    k = math.sqrt(8 / math.pi)  # (1 + tanh(y)) / 2 = sigmoid(2 y)
+    y = k * (g + 0.044715 * g ** 3)
+    s, r, d = torch.sigmoid(y), torch.sigmoid(-y), k * (1 + 3 * 0.044715 * g * g)
+    return g * s, s + g * s * r * d, s + a * s * r * d, 6 + 3.2 * y.abs(), 20 + 9.6 * y.abs()
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("dtype,most,scale", [(torch.bfloat16, 110.0, 1.0), (torch.float16, 20.0, 512.0)])
+@pytest.mark.parametrize("act", ref.ACTS)
+def test_activations_hold_their_relative_error_in_the_tails(act, dtype, most, scale, rows):
+    """One column of ones times the gates: the products are the gates themselves, and the weights' gradients dG and dU of a single row."""
+    gate = gates_of(dtype, most).cuda()
+    F, g = len(gate), gate.double().cpu()
+    up = torch.full((1, F), scale, dtype=dtype, device="cuda")
+    x = torch.ones((rows, 1), dtype=dtype, device="cuda")
+    value, slope, mags, ulps, slope_ulps = tail_forms(act, g)
+    half, tiny, unit = ref.half_step(dtype), ref.tiny(dtype), 2.0 ** -23
+
+    def holds(got, want, ulps, mags, what):
+        # (the float32 error, the scaling's rounding, then the type's; below 2^-126 float32 has steps of 2^-149)
+        e = scale * mags.abs() * (ulps + 2) * unit + scale * (1 + g.abs()) * 2.0 ** -147
+        ref.close(got, want * scale, e + half * ((want * scale).abs() + e) + tiny, what)
+
+    h = CLALibGated.forward(x, gate[None], up, act)
+    assert torch.equal(h, h[:1].expand_as(h))
+    holds(h[0], value, ulps, value, "value")
+    if rows == 1:
+        one = torch.ones((1, F), dtype=dtype, device="cuda")
+        _, dwg, dwu = CLALibGated.backward(up, x, gate[None], one, gate[None], one, act, needX=False)
+        holds(dwg[0], slope, slope_ulps, mags, "slope")
+        holds(dwu[0], value, ulps, value, "value in the gradient")
