@@ -275,8 +275,9 @@ int64_t cla_group_counts(cla_handle h, int32_t g, int64_t* counts);
  * on `stream` of `device` and return CLA_OK without waiting or allocating; the current device stays what it was. Calls share nothing:
  * any number may run at once on any streams, captured or not, as long as their buffers differ. `work` is the caller's, 256-byte aligned,
  * of the size that the *_workspace function gives for the same arguments (0: none needed, work may be NULL); a call uses it until its
- * kernels are done. Outputs may not overlap inputs, but for dropout onto its own input. Every result repeats bit for bit. Elements of a row behind its length, and rows behind
- * the last, are neither read for a result nor written. A kernel's self-check that trips (a wait that ran out) is reported by cla_dense_status. */
+ * kernels are done. Outputs and workspaces that share a byte with an input or with one another are refused (CLA_ERR_BAD_ARG), but for dropout
+ * onto its own input; parts of the same rows that lie side by side share none. Every result repeats bit for bit. Elements of a row behind its
+ * length, and rows behind the last, are neither read for a result nor written. A kernel's self-check that trips (a wait that ran out) is reported by cla_dense_status. */
 #define CLA_T_F64 0
 #define CLA_T_F32 1
 #define CLA_T_BF16 2

@@ -4,6 +4,7 @@
 #include "cla_dense.cuh"
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 namespace cla {
 
@@ -493,6 +494,45 @@ int64_t check_matrix(const char* what, const void* p, int64_t rows, int64_t cols
     if (const int64_t rc_ = (__VA_ARGS__); rc_ < 0) return rc_; \
   } while (0)
 
+// A matrix as the bytes that a call reads or writes of it; ld in bytes
+struct Area {
+  const void* p;
+  int64_t rows, bytes, ld;
+};
+Area area(const void* p, int64_t rows, int64_t cols, int64_t ld, int bytes) { return {p, p ? rows : 0, cols * bytes, ld * bytes}; }
+Area area(const void* p, int64_t bytes) { return {p, p ? 1 : 0, bytes, bytes}; }
+// Whether two of them share a byte. Matrices side by side in the rows of a larger one do not, though their addresses are mixed.
+bool share(Area a, Area b) {
+  using Wide = __int128;  // (rows times strides pass 64 bits before anybody has such memory)
+  if (a.rows <= 0 || b.rows <= 0 || a.bytes <= 0 || b.bytes <= 0) return false;
+  const Wide d = (Wide)(uintptr_t)a.p - (Wide)(uintptr_t)b.p;
+  if (d >= (Wide)(b.rows - 1) * b.ld + b.bytes || -d >= (Wide)(a.rows - 1) * a.ld + a.bytes) return false;
+  const auto floor_div = [](Wide n, Wide by) { return n / by - (n % by < 0); };
+  // rows of a stride s: the first of b's rows -most .. most from a's that ends behind its start
+  const auto meets = [&](Wide off, int64_t s, int64_t least, int64_t most) {
+    const Wide k = std::max<Wide>(floor_div(-a.bytes - off, s) + 1, least);
+    return k <= most && off + k * s < b.bytes;
+  };
+  if (a.rows == 1) a.ld = b.ld;
+  if (b.rows == 1) b.ld = a.ld;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.ld == b.ld) return meets(d, a.ld, -(b.rows - 1), a.rows - 1);
+  if (a.rows < b.rows) return share(b, a);
+  for (int64_t j = 0; j < b.rows; j++)  // (a's rows against row j of b)
+    if (meets(d - (Wide)j * b.ld, a.ld, 0, a.rows - 1)) return true;
+  return false;
+}
+// Outputs that share a byte with an input or with one another: CTAs would read what others have written already
+int64_t check_apart(const char* what, std::initializer_list<Area> outs, std::initializer_list<Area> ins) {
+  for (const Area* o = outs.begin(); o != outs.end(); o++) {
+    for (const Area& i : ins)
+      if (share(*o, i)) return fail(CLA_ERR_BAD_ARG, std::string(what) + ": a result or the workspace overlaps an operand");
+    for (const Area* q = outs.begin(); q != o; q++)
+      if (share(*o, *q)) return fail(CLA_ERR_BAD_ARG, std::string(what) + ": results or the workspace overlap one another");
+  }
+  return CLA_OK;
+}
+
 int64_t drop_device(const cla_drop& d, int64_t rows, DropDev& o) {
   if (!(d.p >= 0.0 && d.p < 1.0)) return fail(CLA_ERR_BAD_ARG, "dropout: p must be at least 0 and below 1");
   if (d.row0 < 0 || d.row0 + rows > (int64_t)1 << 32) return fail(CLA_ERR_BAD_ARG, "dropout: rows beyond 2^32");
@@ -758,6 +798,22 @@ int64_t check_work(const Work& need, const void* work, int64_t bytes) {
   return CLA_OK;
 }
 
+int64_t check_q8_apart(const cla_q8& c, int64_t used) {
+  const bool i8 = c.aType == CLA_T_I8;
+  return check_apart("8-bit product", {area(c.out, c.M, c.N, c.ldo, type_bytes(c.outType)), area(c.work, used)},
+                     {area(c.a, c.M, c.K, c.lda, type_bytes(c.aType)), area(c.b, c.N, c.K, c.ldb, 1), area(i8 ? c.aScale : nullptr, c.M * 4),
+                      area(c.bScale, c.N * 4)});
+}
+int64_t check_gated_apart(const cla_gated& c, bool backward, int64_t used) {
+  const int64_t wr = c.wTrans ? c.F : c.D, wc = c.wTrans ? c.D : c.F;
+  const Area x = area(c.x, c.M, c.D, c.ldx, 2), wg = area(c.wg, wr, wc, c.ldwg, 2), wu = area(c.wu, wr, wc, c.ldwu, 2), work = area(c.work, used);
+  const Area g = area(c.g, c.M, c.F, c.ldg, 2), u = area(c.u, c.M, c.F, c.ldu, 2);
+  if (!backward) return check_apart("gated block", {area(c.h, c.M, c.F, c.ldh, 2), g, u, work}, {x, wg, wu});
+  return check_apart("gated block",
+                     {area(c.dx, c.M, c.D, c.lddx, 2), area(c.dwg, c.D, c.F, c.lddwg, 2), area(c.dwu, c.D, c.F, c.lddwu, 2), work},
+                     {x, wg, wu, g, u, area(c.dh, c.M, c.F, c.lddh, 2)});
+}
+
 // ---- rows of a compressed block ---------------------------------------------------------------------------------------
 constexpr int64_t ROWS_CHUNK = 64ll << 20;  // bytes of FP64 rows at a time that the workspace functions ask for: half the L2
 // Rows [row0, row0 + rows) through an FP64 buffer of `cap` rows: use(first row, rows, their cells). Decompression starts where the skip
@@ -803,6 +859,8 @@ int64_t cla_dropout_dev(int32_t type, const void* x, int64_t ldx, int64_t rows, 
   DN_CHECK(check_matrix("dropout, y", y, rows, cols, ldy, type_bytes(type)));
   DropDev d;
   DN_CHECK(drop_device(*drop, rows, d));
+  if (x != y || (rows > 1 && ldx != ldy))  // (onto its own input: every thread reads an element before it writes it)
+    DN_CHECK(check_apart("dropout", {area(y, rows, cols, ldy, type_bytes(type))}, {area(x, rows, cols, ldx, type_bytes(type))}));
   OnDevice on(device);
   if (on.rc < 0) return on.rc;
   if (rows == 0 || cols == 0) return CLA_OK;
@@ -825,6 +883,8 @@ int64_t cla_q8_quantize_dev(int32_t type, const void* x, int64_t ldx, int64_t ro
   DN_CHECK(check_matrix("quantize, x", x, rows, cols, ldx, type_bytes(type)));
   DN_CHECK(check_matrix("quantize, q", q, byCols ? cols : rows, byCols ? rows : cols, ldq, 1));
   if ((byCols ? cols : rows) && !scale) return fail(CLA_ERR_BAD_ARG, "quantize: null scales");
+  DN_CHECK(check_apart("quantize", {area(q, byCols ? cols : rows, byCols ? rows : cols, ldq, 1), area(scale, (byCols ? cols : rows) * 4)},
+                       {area(x, rows, cols, ldx, type_bytes(type))}));
   OnDevice on(device);
   if (on.rc < 0) return on.rc;
   return quantize(type, x, ldx, rows, cols, byCols, q, ldq, scale, device, (cudaStream_t)stream);
@@ -841,6 +901,7 @@ int64_t cla_q8_mm_dev(const cla_q8* c, void* stream) {
   Work need{nullptr}, w{(char*)c->work};
   DN_CHECK(q8_run(*c, false, need, nullptr));
   DN_CHECK(check_work(need, c->work, c->workBytes));
+  DN_CHECK(check_q8_apart(*c, need.used));
   OnDevice on(c->device);
   if (on.rc < 0) return on.rc;
   return q8_run(*c, true, w, (cudaStream_t)stream);
@@ -859,6 +920,7 @@ static int64_t gated_dev(const cla_gated* c, bool backward, void* stream) {
   Work need{nullptr}, w{(char*)c->work};
   DN_CHECK(backward ? gated_bwd(*c, d, false, need, nullptr) : gated_fwd(*c, d, false, need, nullptr));
   DN_CHECK(check_work(need, c->work, c->workBytes));
+  DN_CHECK(check_gated_apart(*c, backward, need.used));
   OnDevice on(c->device);
   if (on.rc < 0) return on.rc;
   return backward ? gated_bwd(*c, d, true, w, (cudaStream_t)stream) : gated_fwd(*c, d, true, w, (cudaStream_t)stream);
@@ -882,6 +944,7 @@ int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_
   const int64_t cap = workBytes / 8 / m->nCols / SKIP_ROWS * SKIP_ROWS;
   if (!work || cap < SKIP_ROWS) return fail(CLA_ERR_BAD_ARG, "rows of a block: workspace below 1024 rows of FP64");
   if ((uintptr_t)work % 256) return fail(CLA_ERR_BAD_ARG, "workspace not 256-byte aligned");
+  DN_CHECK(check_apart("rows of a block", {area(out, rows, m->nCols, ldo, type_bytes(type)), area(work, std::min(cap, round_up(rows, SKIP_ROWS) + SKIP_ROWS) * m->nCols * 8)}, {}));
   OnDevice on(m->device);
   if (on.rc < 0) return on.rc;
   cudaStream_t s = (cudaStream_t)stream;
@@ -925,6 +988,9 @@ int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* 
   int64_t cap = room / std::max<int64_t>(1, q8_chunk_bytes(m, SKIP_ROWS)) * SKIP_ROWS;
   if (!work || cap < SKIP_ROWS) return fail(CLA_ERR_BAD_ARG, "8-bit right product: workspace below 1024 rows");
   cap = std::min(cap, round_up(c.M, SKIP_ROWS));
+  cla_q8 apart = c;
+  apart.a = nullptr, apart.work = work;
+  DN_CHECK(check_q8_apart(apart, q8_chunk_bytes(m, cap) + round_up(N * round_up(m->nCols, PITCH), 256)));
   OnDevice on(m->device);
   if (on.rc < 0) return on.rc;
   cudaStream_t s = (cudaStream_t)stream;

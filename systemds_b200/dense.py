@@ -6,8 +6,9 @@
 
 They have no counterpart in the reference. Operands are torch CUDA tensors with rows of adjacent elements (any row stride; weights may also be
 transposed views). Each call is enqueued on the current stream of its tensors' device, takes results and workspaces from torch's
-allocator, and may be captured into a graph. Nothing is recorded for autograd: gradients are the ``backward`` calls' and the dropout's own. A ``CompressedMatrixBlock`` takes part through ``CLALibQ8.rightMultByMatrix`` and
-``CLALibDecompress.rows``. Failures raise ``CLAError``.
+allocator, and may be captured into a graph. Nothing is recorded for autograd: gradients are the ``backward`` calls' and the dropout's own. An ``out`` that
+shares memory with an operand is refused, but for dropout onto its own input. A ``CompressedMatrixBlock`` takes part through
+``CLALibQ8.rightMultByMatrix`` and ``CLALibDecompress.rows``. Failures raise ``CLAError``.
 """
 from __future__ import annotations
 
@@ -103,7 +104,7 @@ class CLALibDropout:
     def apply(x, p: float, seed: int, step: int = 0, row0: int = 0, out=None):
         """``x`` with each element zero with probability ``p``, else times ``1 / (1 - p)``. Word ``c % 4`` of Philox4x32-10 with key
         ``seed`` and counter ``(c / 4, row0 + r, step)`` decides about element (r, c): applied to the output's gradient with the same
-        ``(seed, step)`` it is the backward pass, and a shard of rows passes its first row as ``row0``. ``out`` may be ``x``."""
+        ``(seed, step)`` it is the backward pass, and a shard of rows passes its first row as ``row0``. ``out`` may be ``x`` itself."""
         px, ldx = _rows(x, "dropout, x")
         dtype = x.dtype
         t = _type(dtype, "dropout")
@@ -166,7 +167,7 @@ class CLALibQ8:
     @staticmethod
     def matrixMult(a, aScale, b, bScale, dtype=torch.float32, out=None):
         """``out[m, n] = aScale[m] * bScale[n] * sum_k a[m, k] * b[n, k]`` for int8 ``a`` [M x K] and ``b`` [N x K] (a row per output
-        column, as ``quantizeCols`` gives), exact up to the scaling and one rounding to ``dtype``."""
+        column, as ``quantizeCols`` gives), exact up to the scaling and one rounding to ``dtype``. ``out`` shares no memory with an operand."""
         if not isinstance(a, torch.Tensor) or a.dtype != torch.int8:
             _fail(-3, "8-bit product: a must be int8")
         if aScale is None:
@@ -176,7 +177,7 @@ class CLALibQ8:
     @staticmethod
     def linear(x, b, bScale, dtype=None, out=None):
         """``x %*% W`` with W in 8 bits (``b``, ``bScale`` of ``quantizeCols(W)``): the rows of ``x`` are quantised in the call.
-        The result has the type of ``x`` unless ``dtype`` says otherwise."""
+        The result has the type of ``x`` unless ``dtype`` says otherwise; ``out`` shares no memory with an operand."""
         if not isinstance(x, torch.Tensor):
             _fail(-2, "8-bit product, x: a CUDA tensor is needed")
         return CLALibQ8._mm(x, _type(x.dtype, "8-bit product"), None, b, bScale, dtype or x.dtype, out)
@@ -241,7 +242,7 @@ class CLALibGated:
     @staticmethod
     def forward(x, wGate, wUp, act: str = "silu", p: float = 0.0, seed: int = 0, step: int = 0, row0: int = 0, save: bool = False, out=None):
         """``H`` [rows of x, F]; with ``save`` also ``X Wg`` and ``X Wu``, which ``backward`` takes. ``p``, ``seed``, ``step``, ``row0``:
-        dropout of H, as ``CLALibDropout.apply``."""
+        dropout of H, as ``CLALibDropout.apply``. ``out`` shares no memory with an operand."""
         c = CLALibGated._args(x, wGate, wUp, act, p, seed, step, row0)
         h = _result(out, (c.M, c.F), x.dtype, x, "gated block, out")
         c.h, c.ldh = (h.data_ptr(), c.F) if out is None else _rows(h, "gated block, out", x.dtype, c.device)

@@ -1,0 +1,67 @@
+"""What the dense operators refuse on the host, beyond test_dense.py, and how they are imported."""
+import ctypes as C
+
+import pytest
+
+from systemds_b200 import CLAError, native
+from systemds_b200.native import check
+
+M, K, N = 6, 48, 48
+A, B, SA, SB, OUT, WORK, MORE = ((i + 1) << 24 for i in range(7))  # addresses that nothing reads: the calls below are refused on the host
+
+
+def refused(code, f):
+    with pytest.raises(CLAError) as e:
+        check(f())
+    assert e.value.code == code, str(e.value)
+
+
+def test_8_bit_products_onto_their_operands():
+    L = native.lib()
+
+    def mm(**kw):
+        c = native.cla_q8(M=M, N=N, K=K, a=A, lda=K, aScale=SA, b=B, ldb=K, bScale=SB, out=OUT, ldo=N, work=WORK, workBytes=1 << 20, aType=4, outType=1, device=0)
+        for k, v in kw.items():
+            setattr(c, k, v)
+        return L.cla_q8_mm_dev(C.byref(c), None)
+
+    for at in (A, A + 4, A + (M - 1) * K, A - (M - 1) * N * 4, B, B + N * K - 4, SA, SA + 4 * M - 4, SB, SB + 4 * N - 4):
+        refused(-2, lambda: mm(out=at))
+    refused(-2, lambda: mm(lda=240, ldo=60, out=A + 40))  # (240 bytes a row each, side by side but for 8 bytes)
+    refused(-2, lambda: mm(lda=401, ldo=50, out=A + 48 + 12))  # (the rows' distances differ: they meet in some later row)
+    refused(-2, lambda: mm(b=B + 1, work=B))  # (copied to the workspace, off its boundary)
+    refused(-2, lambda: mm(b=B + 1, work=OUT))
+    for at in (A, A + 16):
+        refused(-2, lambda: L.cla_q8_quantize_dev(1, A, 8, 4, 8, 0, at, 8, SA, 0, None))
+        refused(-2, lambda: L.cla_q8_quantize_dev(1, A, 8, 4, 8, 1, OUT, 8, at, 0, None))
+    refused(-2, lambda: L.cla_q8_quantize_dev(1, A, 8, 4, 8, 0, OUT, 8, OUT + 12, 0, None))
+
+
+def test_gated_blocks_onto_their_operands():
+    L = native.lib()
+
+    def call(backward, **kw):
+        c = native.cla_gated(M=M, D=K, F=K, x=A, wg=B, wu=SA, ldx=K, ldwg=K, ldwu=K, h=OUT, g=MORE, u=MORE << 1, ldh=K, ldg=K, ldu=K, dh=SB, lddh=K,
+                             dx=OUT, dwg=OUT << 1, dwu=OUT << 2, lddx=K, lddwg=K, lddwu=K, work=WORK, workBytes=1 << 20, type=2, act=0, wTrans=0, device=0)
+        for k, v in kw.items():
+            setattr(c, k, v)
+        return (L.cla_gated_bwd_dev if backward else L.cla_gated_fwd_dev)(C.byref(c), None)
+
+    last = 2 * (M * K - 1)
+    for kw in ({"h": A}, {"h": A + last}, {"h": B}, {"h": SA + 2 * (K * K - 1)}, {"g": A}, {"u": B}, {"h": MORE}, {"u": MORE + 2}):
+        refused(-2, lambda: call(False, **kw))
+    for kw in ({"dx": A}, {"dx": SB + last}, {"dx": MORE}, {"dwg": B}, {"dwu": SA}, {"dwg": MORE << 1}, {"dwu": OUT << 1}, {"work": A}, {"work": OUT}):
+        refused(-2, lambda: call(True, **kw))
+
+
+def test_dropout_partly_onto_its_operand():
+    L = native.lib()
+
+    def call(x, ldx, y, ldy, rows=4, cols=8):
+        return L.cla_dropout_dev(1, x, ldx, rows, cols, y, ldy, C.byref(native.cla_drop(0.5, 1, 2, 0)), 0, None)
+
+    for at in (A + 4, A + 32, A + 96 + 28, A - 4, A - 96 - 28):
+        refused(-2, lambda: call(A, 8, at, 8))
+    refused(-2, lambda: call(A, 8, A, 16))
+    refused(-2, lambda: call(A, 20, A + 28, 20))
+    refused(-2, lambda: call(A, 20, A + 32, 21, rows=8))  # (the sixth row has moved on to the next one's place)

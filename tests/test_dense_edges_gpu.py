@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from systemds_b200 import CLALibGated
+from systemds_b200 import CLAError, CLALibDropout, CLALibGated, CLALibQ8
 from systemds_b200.dense import status
 from tests import dense_ref as ref
 
@@ -73,3 +73,33 @@ def test_activations_hold_their_relative_error_in_the_tails(act, dtype, most, sc
         _, dwg, dwu = CLALibGated.backward(up, x, gate[None], one, gate[None], one, act, needX=False)
         holds(dwg[0], slope, slope_ulps, mags, "slope")
         holds(dwu[0], value, ulps, value, "value in the gradient")
+
+
+# ---- results next to operands -------------------------------------------------------------------------------------------
+def test_results_onto_operands_are_refused():
+    """Shapes that fit: it is the shared memory that refuses the call, and nothing has been written."""
+    x = torch.randn(40, 64, device="cuda").to(torch.bfloat16)
+    w = torch.randn(64, 64, device="cuda").to(torch.bfloat16)
+    keep, keepW = x.clone(), w.clone()
+    q, s = CLALibQ8.quantizeCols(w)
+    for f in (lambda: CLALibGated.forward(x, w, w, out=x), lambda: CLALibGated.forward(w, w, keepW, out=w), lambda: CLALibQ8.linear(x, q, s, out=x),
+              lambda: CLALibDropout.apply(x[:39], 0.5, 1, out=x[1:])):
+        with pytest.raises(CLAError):
+            f()
+    assert torch.equal(x, keep) and torch.equal(w, keepW)
+
+
+def test_results_beside_operands_in_the_same_rows_are_taken():
+    w = torch.randn(64, 64, device="cuda").to(torch.bfloat16)
+    q, s = CLALibQ8.quantizeCols(w)
+    wide = torch.randn(50, 200, device="cuda").to(torch.bfloat16)
+    x, out = wide[:, 3:67], wide[:, 67:131]
+    want = CLALibGated.forward(x.clone(), w, w), CLALibQ8.linear(x.clone(), q, s), CLALibDropout.apply(x.clone(), 0.5, 1)
+    for f, v in zip((lambda: CLALibGated.forward(x, w, w, out=out), lambda: CLALibQ8.linear(x, q, s, out=out),
+                     lambda: CLALibDropout.apply(x, 0.5, 1, out=out)), want):
+        assert torch.equal(f(), v) and torch.equal(out, v)
+    x, out = wide[:25, 3:67], wide.view(25, 400)[:, 270:334]  # rows twice as far apart as the operand's
+    want = CLALibDropout.apply(x.clone(), 0.5, 1)
+    assert torch.equal(CLALibDropout.apply(x, 0.5, 1, out=out), want)
+    with pytest.raises(CLAError):
+        CLALibDropout.apply(x, 0.5, 1, out=wide.view(25, 400)[:, 266:330])
