@@ -23,7 +23,9 @@
  * Device-buffer calls (cla_*_dev) return once their work is enqueued on the caller's stream; all
  * calls on a handle share that handle's scratch buffers, so the library orders them on the device
  * as well: a call that arrives on another stream than the handle's previous call waits (event
- * wait on the device, not on the host) until that call's kernels have finished. A kernel's
+ * wait on the device, not on the host) until that call's kernels have finished. Calls that are captured into a graph
+ * are ordered in that way among those of the same capture; a replay runs where its stream has come to, and a program
+ * that replays on one stream and calls on another orders the two itself. A kernel's
  * self-check that trips in a device-buffer call is reported by the next cla_stats_get or
  * host-buffer call on the handle (CLA_ERR_DEVICE_CHECK); callers that never make one should poll
  * cla_stats_get. The right products (X %*% v, X %*% V), the specialised left vector product and
@@ -272,7 +274,8 @@ int64_t cla_group_counts(cla_handle h, int32_t g, int64_t* counts);
  * What follows a compressed product in a model's training and scoring: the hidden layer of a gated feed-forward block with its
  * gradients, dropout, and products in 8-bit integers. They have no counterpart in the reference. Matrices are device memory in rows
  * of `ld` elements (ld >= the row's length; rows need no alignment), of at most 2^30 rows and columns, types CLA_T_*; sums are 32 bits or wider. Calls enqueue
- * on `stream` of `device` and return CLA_OK without waiting or allocating; the current device stays what it was. Calls share nothing:
+ * on `stream` of `device` and return CLA_OK without waiting or allocating (but for the two calls on a compressed block, which build at the
+ * block's first calls what its decompression needs, and wait for that, unless they are being captured); the current device stays what it was. Calls share nothing:
  * any number may run at once on any streams, captured or not, as long as their buffers differ. `work` is the caller's, 256-byte aligned,
  * of the size that the *_workspace function gives for the same arguments (0: none needed, work may be NULL); a call uses it until its
  * kernels are done. Outputs and workspaces that share a byte with an input or with one another are refused (CLA_ERR_BAD_ARG), but for dropout

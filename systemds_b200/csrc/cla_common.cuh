@@ -285,6 +285,10 @@ struct Matrix {
   cudaEvent_t lastDone = nullptr;
   cudaStream_t lastStream = nullptr;
   bool lastValid = false;
+  // The same among the calls of one capture: an event recorded in a capture means nothing outside it, nor one of before inside
+  cudaEvent_t captureDone = nullptr;
+  cudaStream_t captureStream = nullptr;
+  unsigned long long lastCapture = 0;
   FastPlan* fast = nullptr;
   // listed rows of the SDC groups, group by group in element order: row in its 1024-row block | tuple << 10
   uint32_t* sdcItems = nullptr;

@@ -99,7 +99,23 @@ static int64_t grow(Matrix* m, void** p, size_t* cur, size_t bytes) {
   *cur = want;
   return CLA_OK;
 }
+// The capture that a stream takes part in, 0 if none
+static unsigned long long capture_of(cudaStream_t s) {
+  if (s == nullptr) return 0;  // (the legacy default stream cannot be captured)
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
 int64_t order_begin(Matrix* m, cudaStream_t s) {
+  if (const unsigned long long id = capture_of(s)) {
+    // Nothing runs now, and a graph cannot wait for what is outside it: ordered among the calls of the same capture alone
+    if (m->lastCapture == id && m->captureStream != s) CLA_CUDA(cudaStreamWaitEvent(s, m->captureDone, 0));
+    return CLA_OK;
+  }
   if (m->lastValid && m->lastStream != s) {
     if (m->lastStream == nullptr) CLA_CUDA(cudaEventRecord(m->lastDone, nullptr));  // not recorded by order_end, see there
     CLA_CUDA(cudaStreamWaitEvent(s, m->lastDone, 0));
@@ -107,6 +123,12 @@ int64_t order_begin(Matrix* m, cudaStream_t s) {
   return CLA_OK;
 }
 int64_t order_end(Matrix* m, cudaStream_t s) {
+  if (const unsigned long long id = capture_of(s)) {
+    CLA_CUDA(cudaEventRecord(m->captureDone, s));
+    m->lastCapture = id;
+    m->captureStream = s;
+    return CLA_OK;
+  }
   // The legacy default stream always exists, so the event behind a call on it is recorded only when a call on another
   // stream needs it (everything enqueued there by then is waited for); other streams may be destroyed by their owner.
   if (s != nullptr) CLA_CUDA(cudaEventRecord(m->lastDone, s));
@@ -542,6 +564,7 @@ int64_t init_device_state(Matrix* m) {
   CLA_CUDA(cudaEventCreate(&m->ev0));
   CLA_CUDA(cudaEventCreate(&m->ev1));
   CLA_CUDA(cudaEventCreateWithFlags(&m->lastDone, cudaEventDisableTiming));
+  CLA_CUDA(cudaEventCreateWithFlags(&m->captureDone, cudaEventDisableTiming));
   void* errp = nullptr;
   CLA_CUDA(dev_malloc(m, &errp, 64));
   // (on the handle's own stream: a clear on the default stream could run after the first checks have reported)
@@ -873,6 +896,8 @@ void release(Matrix* m) {
   m->ev0 = m->ev1 = nullptr;
   if (m->lastDone) cudaEventDestroy(m->lastDone);
   m->lastDone = nullptr;
+  if (m->captureDone) cudaEventDestroy(m->captureDone);
+  m->captureDone = nullptr;
   m->lastValid = false;
   for (auto& e : m->copyDone)
     if (e) {

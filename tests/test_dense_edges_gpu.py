@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from systemds_b200 import CLAError, CLALibDropout, CLALibGated, CLALibQ8
+from systemds_b200 import CLAError, CLALibDecompress, CLALibDropout, CLALibGated, CLALibQ8, datagen, native
 from systemds_b200.dense import status
 from tests import dense_ref as ref
 
@@ -103,3 +103,48 @@ def test_results_beside_operands_in_the_same_rows_are_taken():
     assert torch.equal(CLALibDropout.apply(x, 0.5, 1, out=out), want)
     with pytest.raises(CLAError):
         CLALibDropout.apply(x, 0.5, 1, out=wide.view(25, 400)[:, 266:330])
+
+
+# ---- a compressed block's calls, captured -------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [3000, 700_000])  # (the larger one in chunks, the second of which finds a plan worth building)
+def test_block_calls_captured_between_direct_ones(rows):
+    """Direct calls on the default stream, captured ones on another, replays, and direct calls on a third stream and again on the first."""
+    cmb = datagen.random_cmb(3, rows, datagen.KINDS).to_device(0)
+    w, scale = CLALibQ8.quantizeCols(torch.randn(cmb.clen, 33, device="cuda"))
+    V = torch.randn(cmb.clen, 2, device="cuda", dtype=torch.float64)
+
+    def calls():
+        product = torch.empty((rows, 2), device="cuda", dtype=torch.float64)
+        native.check(native.lib().cla_rmm_dev(cmb.handle(), V.data_ptr(), cmb.clen, 2, product.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        return CLALibDecompress.rows(cmb, 5, rows - 7, torch.float32), CLALibQ8.rightMultByMatrix(cmb, w, scale), product
+
+    def same(got):
+        torch.cuda.synchronize()
+        return all(torch.equal(p, q) for p, q in zip(got, want))
+
+    want = calls()
+    torch.cuda.synchronize()
+    side, other, third = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream()
+    graphs = []
+    for fork in (False, True):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = calls()
+            if fork:  # the handle's calls on two streams of one capture
+                other.wait_stream(side)
+                with torch.cuda.stream(other):
+                    out += calls()
+                side.wait_stream(other)
+                out += calls()
+        graphs.append((graph, out))
+        assert same(calls())
+    for graph, out in graphs * 2:
+        for t in out:
+            t.zero_()
+        graph.replay()
+        assert same(out[:3]) and same(out[-3:]) and same(out[len(out) // 3:][:3] if len(out) > 3 else out)
+        with torch.cuda.stream(third):
+            got = calls()
+        assert same(got) and same(calls())
+    del graphs, graph
+    cmb.free()
