@@ -535,7 +535,7 @@ int64_t check_apart(const char* what, std::initializer_list<Area> outs, std::ini
 
 int64_t drop_device(const cla_drop& d, int64_t rows, DropDev& o) {
   if (!(d.p >= 0.0 && d.p < 1.0)) return fail(CLA_ERR_BAD_ARG, "dropout: p must be at least 0 and below 1");
-  if (d.row0 < 0 || d.row0 + rows > (int64_t)1 << 32) return fail(CLA_ERR_BAD_ARG, "dropout: rows beyond 2^32");
+  if (d.row0 < 0 || d.row0 > ((int64_t)1 << 32) - rows) return fail(CLA_ERR_BAD_ARG, "dropout: rows beyond 2^32");
   o.on = d.p > 0.0;
   o.cut = (uint32_t)std::floor(d.p * 4294967296.0);
   o.row0 = (uint32_t)d.row0;
@@ -938,7 +938,7 @@ int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_
                                 void* stream) {
   DN_MATRIX(h);
   if (!is_float_type(type)) return fail(CLA_ERR_UNSUPPORTED, "rows of a block: unknown type");
-  if (row0 < 0 || rows < 0 || row0 + rows > m->nRows) return fail(CLA_ERR_SHAPE, "rows of a block: outside the matrix");
+  if (row0 < 0 || rows < 0 || rows > m->nRows || row0 > m->nRows - rows) return fail(CLA_ERR_SHAPE, "rows of a block: outside the matrix");
   DN_CHECK(check_matrix("rows of a block, result", out, rows, m->nCols, ldo, type_bytes(type)));
   if (rows == 0 || m->nCols == 0) return CLA_OK;
   const int64_t cap = workBytes / 8 / m->nCols / SKIP_ROWS * SKIP_ROWS;
@@ -968,6 +968,7 @@ int64_t cla_decompress_rows_dev(cla_handle h, int64_t row0, int64_t rows, int32_
 int64_t cla_q8_rmm_workspace(cla_handle h, int64_t N) {
   DN_MATRIX(h);
   if (N < 0) return fail(CLA_ERR_SHAPE, "8-bit right product: negative size");
+  if (N > 1 << 30) return fail(CLA_ERR_UNSUPPORTED, "8-bit right product: more than 2^30 columns");
   return q8_chunk_bytes(m, chunk_rows(m, m->nRows)) + round_up(N * round_up(m->nCols, PITCH), 256);
 }
 int64_t cla_q8_rmm_dev(cla_handle h, const int8_t* b, int64_t ldb, const float* bScale, int64_t N, int32_t outType, void* out, int64_t ldo,

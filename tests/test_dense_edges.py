@@ -65,3 +65,13 @@ def test_dropout_partly_onto_its_operand():
     refused(-2, lambda: call(A, 8, A, 16))
     refused(-2, lambda: call(A, 20, A + 28, 20))
     refused(-2, lambda: call(A, 20, A + 32, 21, rows=8))  # (the sixth row has moved on to the next one's place)
+
+
+def test_rows_whose_end_leaves_64_bits():
+    L = native.lib()
+    for row0 in ((1 << 63) - 1, (1 << 63) - 4, (1 << 63) - 6):
+        d = native.cla_drop(0.5, 1, 2, row0)
+        refused(-2, lambda: L.cla_dropout_dev(1, A, 8, M, 8, B, 8, C.byref(d), 0, None))
+        c = native.cla_gated(M=M, D=K, F=K, x=A, wg=B, wu=SA, ldx=K, ldwg=K, ldwu=K, h=OUT, ldh=K, drop=d, type=2)
+        refused(-2, lambda: L.cla_gated_fwd_dev(C.byref(c), None))
+        refused(-2, lambda: L.cla_gated_workspace(C.byref(c), 0))

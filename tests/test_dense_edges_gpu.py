@@ -148,3 +148,21 @@ def test_block_calls_captured_between_direct_ones(rows):
         assert same(got) and same(calls())
     del graphs, graph
     cmb.free()
+
+
+def test_rows_of_a_block_whose_end_leaves_64_bits():
+    cmb = datagen.random_cmb(3, 3000, datagen.KINDS).to_device(0)
+    L, h = native.lib(), cmb.handle()
+    out = torch.full((8, cmb.clen), 7.0, device="cuda")
+    n = native.check(L.cla_rows_workspace(h, 8, 1))
+    work = torch.empty(n, dtype=torch.uint8, device="cuda")
+    for row0, rows in (((1 << 63) - 1, 8), ((1 << 63) - 8, 8), (2993, 8), (-1, 8), (0, (1 << 63) - 1), (1, (1 << 63) - 1)):
+        with pytest.raises(CLAError) as e:
+            native.check(L.cla_decompress_rows_dev(h, row0, rows, 1, out.data_ptr(), cmb.clen, work.data_ptr(), n, None))
+        assert e.value.code == -4
+    for N in (1 << 31, 1 << 56, (1 << 63) - 1):
+        with pytest.raises(CLAError) as e:
+            native.check(L.cla_q8_rmm_workspace(h, N))
+        assert e.value.code == -3
+    assert bool((out == 7).all())
+    cmb.free()
