@@ -15,6 +15,7 @@ raise ``CLAError`` (the reference wraps its failures in DMLCompressionException 
 from __future__ import annotations
 
 import ctypes as C
+from operator import index
 
 import numpy as np
 
@@ -418,13 +419,20 @@ class CLALibDecompress:
         """Rows ``[row0, row0 + rows)`` as a torch tensor on the block's device, rounded once to ``dtype`` (float64, float32, bfloat16,
         float16): what the dense operators take of a compressed block."""
         import torch
-        from .dense import _rows, _stream, _type, _workspace
+        from .dense import _result, _rows, _stream, _type, _workspace
+        if not isinstance(cmb, CompressedMatrixBlock):
+            raise native.CLAError(-2, "rows of a block: a compressed block is needed")
         h, t = cmb.handle(), _type(dtype, "rows of a block")
+        try:
+            row0, rows = index(row0), index(rows)
+        except TypeError:
+            raise native.CLAError(-2, "rows of a block: row0 and rows are whole numbers") from None
         if row0 < 0 or rows < 0 or row0 + rows > cmb.rlen:
             raise native.CLAError(-4, "rows of a block: outside the matrix")
-        y = torch.empty((rows, cmb.clen), dtype=dtype, device=torch.device("cuda", cmb.device)) if out is None else out
-        if tuple(y.shape) != (rows, cmb.clen):
-            raise native.CLAError(-4, "rows of a block, out: another shape")
+        if out is None:
+            y = torch.empty((rows, cmb.clen), dtype=dtype, device=torch.device("cuda", cmb.device))
+        else:
+            y = _result(out, (rows, cmb.clen), dtype, None, "rows of a block, out")
         py, ldo = _rows(y, "rows of a block, out", dtype, cmb.device)
         n = check(native.lib().cla_rows_workspace(h, rows, t))
         work = _workspace(n, y.device)

@@ -13,10 +13,12 @@ shares memory with an operand is refused, but for dropout onto its own input. A 
 from __future__ import annotations
 
 import ctypes as C
+from operator import index
 
 import torch
 
 from . import native
+from .cmb import CompressedMatrixBlock
 from .native import CLAError, check
 
 TYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
@@ -76,7 +78,7 @@ def _result(out, shape, dtype, like, what: str):
 
 
 def _type(dtype, what: str) -> int:
-    t = TYPES.get(dtype)
+    t = TYPES.get(dtype) if isinstance(dtype, torch.dtype) else None
     if t is None:
         _fail(-3, f"{what}: unsupported type {dtype}")
     return t
@@ -92,6 +94,18 @@ def _workspace_like(n: int, t):
 
 
 def _drop(p, seed, step, row0) -> native.cla_drop:
+    try:
+        return _drop_of(p, seed, step, row0)
+    except (TypeError, OverflowError):  # (numbers of other kinds than Python's own)
+        pass
+    try:
+        p, seed, step, row0 = float(p * 1.0), index(seed), index(step), index(row0)
+    except (TypeError, ValueError):
+        _fail(-2, "dropout: p is a number, seed, step and row0 are whole numbers")
+    return _drop_of(p, seed, step, row0)
+
+
+def _drop_of(p, seed, step, row0) -> native.cla_drop:
     if not 0 <= seed < 1 << 64 or not 0 <= step < 1 << 64:
         _fail(-2, "dropout: seed and step are unsigned 64-bit numbers")
     if not 0 <= row0 <= 1 << 32:
@@ -151,11 +165,12 @@ class CLALibQ8:
         N, inner = b.shape
         if inner != K:
             _fail(-4, "8-bit product: inner dimensions do not match")
+        outType = _type(dtype, "8-bit product")
         y = _result(out, (M, N), dtype, a, "8-bit product, out")
         py, ldo = (y.data_ptr(), N) if out is None else _rows(y, "8-bit product, out", dtype, dev)
         L = native.lib()
         args = native.cla_q8(M, N, K, pa, lda, None if aScale is None else _vector(aScale, "8-bit product, scales of a", M, dev), pb, ldb,
-                             _vector(bScale, "8-bit product, scales of b", N, dev), py, ldo, None, 0, aType, _type(dtype, "8-bit product"), dev)
+                             _vector(bScale, "8-bit product, scales of b", N, dev), py, ldo, None, 0, aType, outType, dev)
         ref = C.byref(args)
         n = check(L.cla_q8_workspace(ref))
         if n:
@@ -180,24 +195,27 @@ class CLALibQ8:
         The result has the type of ``x`` unless ``dtype`` says otherwise; ``out`` shares no memory with an operand."""
         if not isinstance(x, torch.Tensor):
             _fail(-2, "8-bit product, x: a CUDA tensor is needed")
-        return CLALibQ8._mm(x, _type(x.dtype, "8-bit product"), None, b, bScale, dtype or x.dtype, out)
+        return CLALibQ8._mm(x, _type(x.dtype, "8-bit product"), None, b, bScale, x.dtype if dtype is None else dtype, out)
 
     @staticmethod
     def rightMultByMatrix(m1, b, bScale, dtype=torch.float64, out=None):
         """``m1 %*% W`` for a compressed block ``m1`` and W in 8 bits, as ``linear`` of its rows (beside
         ``CLALibRightMultBy.rightMultByMatrix``, in FP64). The result is a tensor on the block's device."""
+        if not isinstance(m1, CompressedMatrixBlock):
+            _fail(-2, "8-bit right product, m1: a compressed block is needed")
         dev = m1.device if m1.device is not None else 0
         pb, ldb = _rows(b, "8-bit right product, b", torch.int8, dev)
         N = b.shape[0]
         if b.shape[1] != m1.clen:
             _fail(-4, "8-bit right product: inner dimensions do not match")
         ps = _vector(bScale, "8-bit right product, scales", N, dev)
+        outType = _type(dtype, "8-bit right product")
         y = _result(out, (m1.rlen, N), dtype, b, "8-bit right product, out")
         py, ldo = _rows(y, "8-bit right product, out", dtype, dev)
         L = native.lib()
         n = check(L.cla_q8_rmm_workspace(m1.handle(), N))
         work = _workspace(n, b.device)
-        check(L.cla_q8_rmm_dev(m1.handle(), pb, ldb, ps, N, _type(dtype, "8-bit right product"), py, ldo, work.data_ptr(), n, _stream(dev)))
+        check(L.cla_q8_rmm_dev(m1.handle(), pb, ldb, ps, N, outType, py, ldo, work.data_ptr(), n, _stream(dev)))
         return y
 
 
@@ -211,7 +229,7 @@ class CLALibGated:
         dev = x.get_device()
         if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
             _fail(-3, f"gated block: unsupported type {x.dtype} (bfloat16 and float16)")
-        a = ACTS.get(act)
+        a = ACTS.get(act) if isinstance(act, str) else None
         if a is None:
             _fail(-3, f"gated block: unknown activation {act!r}")
         M, D = x.shape

@@ -2,8 +2,10 @@
 import ctypes as C
 
 import pytest
+import torch
 
-from systemds_b200 import CLAError, native
+from systemds_b200 import CLAError, CLALibDecompress, CLALibQ8, CompressedMatrixBlock, native
+from systemds_b200.dense import _drop, _type
 from systemds_b200.native import check
 
 M, K, N = 6, 48, 48
@@ -75,3 +77,22 @@ def test_rows_whose_end_leaves_64_bits():
         c = native.cla_gated(M=M, D=K, F=K, x=A, wg=B, wu=SA, ldx=K, ldwg=K, ldwu=K, h=OUT, ldh=K, drop=d, type=2)
         refused(-2, lambda: L.cla_gated_fwd_dev(C.byref(c), None))
         refused(-2, lambda: L.cla_gated_workspace(C.byref(c), 0))
+
+
+def test_arguments_of_other_kinds():
+    """Failures are CLAError also where an argument is nothing that the call knows."""
+    for args in ((None, 1, 0, 0), ("0.5", "1", 0, 0), (0.5, 1.5, 0, 0), (0.5, "1", 0, 0), (0.5, 1, None, 0), (0.5, 1, 0, [0]), (0.5, -1, 0, 0), (0.5, 1, 1 << 64, 0)):
+        refused(-2, lambda: _drop(*args))
+    d = _drop(torch.tensor(0.5), torch.tensor(3), torch.tensor(1 << 40), torch.tensor(7))
+    assert (d.p, d.seed, d.step, d.row0) == (0.5, 3, 1 << 40, 7)
+    for dtype in (torch.int32, "bf16", None, [torch.float32], float):
+        refused(-3, lambda: _type(dtype, "type"))
+    block, x = CompressedMatrixBlock(4, 2, []), torch.ones(4, 2)
+    block._handle = 1  # (refused before anybody asks for it)
+    for args in ((x, 0, 2, torch.float32), (block, "0", 2, torch.float32), (block, 0, 1.5, torch.float32), (block, 0, 2, torch.float32, [1]),
+                 (block, 0, 2, torch.float32, x[:2].numpy())):
+        refused(-2, lambda: CLALibDecompress.rows(*args))
+    refused(-3, lambda: CLALibDecompress.rows(block, 0, 2, "bf16"))
+    refused(-4, lambda: CLALibDecompress.rows(block, 0, 2, torch.float32, x))
+    refused(-2, lambda: CLALibQ8.rightMultByMatrix(x, x, x))
+    block._handle = 0

@@ -166,3 +166,15 @@ def test_rows_of_a_block_whose_end_leaves_64_bits():
         assert e.value.code == -3
     assert bool((out == 7).all())
     cmb.free()
+
+
+def test_arguments_of_other_kinds_on_the_device():
+    x = torch.ones((8, 16), device="cuda", dtype=torch.bfloat16)
+    w, q, s = x.t().contiguous(), *CLALibQ8.quantizeRows(x)
+    for f in (lambda: CLALibQ8.linear(x, q, s, dtype="bf16"), lambda: CLALibQ8.linear(x, q, s, dtype=0), lambda: CLALibQ8.matrixMult(q, s, q, s, None),
+              lambda: CLALibGated.forward(x, w, w, ["silu"]), lambda: CLALibGated.forward(x, w, w, p="0.1"), lambda: CLALibGated.forward(x, w, w, seed=0.5),
+              lambda: CLALibDropout.apply(x, None, 1), lambda: CLALibQ8.linear(x, [q], s), lambda: CLALibQ8.linear(x, q, [s])):
+        with pytest.raises(CLAError):
+            f()
+    seed = torch.tensor(5)
+    assert torch.equal(CLALibDropout.apply(x, torch.tensor(0.5), seed), CLALibDropout.apply(x, 0.5, 5))
