@@ -1,5 +1,8 @@
 """What the dense operators refuse on the host, beyond test_dense.py, and how they are imported."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -96,3 +99,16 @@ def test_arguments_of_other_kinds():
     refused(-4, lambda: CLALibDecompress.rows(block, 0, 2, torch.float32, x))
     refused(-2, lambda: CLALibQ8.rightMultByMatrix(x, x, x))
     block._handle = 0
+
+
+@pytest.mark.parametrize("torch_is_there", [True, False])
+def test_star_import(torch_is_there):
+    """Without torch the compressed products are imported alone; torch waits until it is asked for."""
+    code = ("import sys\n" + ("" if torch_is_there else "sys.modules['torch'] = None\n") + "import systemds_b200\n"
+            "assert sys.modules.get('torch') is None\nfrom systemds_b200 import *\nCompressedMatrixBlock, CLALibRightMultBy, CLAError\n"
+            f"assert ('CLALibQ8' in globals()) == {torch_is_there}\n"
+            "try:\n    from systemds_b200 import CLALibDropout\n    there = True\nexcept ImportError:\n    there = False\n"
+            f"assert there == {torch_is_there}\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr
