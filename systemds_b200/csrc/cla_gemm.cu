@@ -7,6 +7,7 @@
 // All are launched with at most one CTA an SM, which takes all of the SM's shared and tensor memory and loops: no CTA waits for tensor memory.
 #include <cuda.h>
 #include <algorithm>
+#include <atomic>
 #include "cla_dense.cuh"
 
 namespace cla {
@@ -1112,15 +1113,15 @@ static int64_t operand_map(CUtensorMap& map, const GemmOperand& o, int type, int
 }
 
 // All of an SM's shared memory for a CTA, as it takes all of its tensor memory: CTAs that wait for tensor memory while others wait for
-// them could hold up one another
+// them could hold up one another. room: how much it is, where the caller wants to know (threads that meet write the same)
 template <class K>
-static int64_t all_smem(OncePerDevice& once, int* room, int device, K kernel) {
+static int64_t all_smem(OncePerDevice& once, std::atomic<int>* room, int device, K kernel) {
   return once(device, [&]() -> int64_t {
     cudaFuncAttributes a;
     CLA_CUDA(cudaFuncGetAttributes(&a, kernel));
     const int most = 227 * 1024 - (int)a.sharedSizeBytes;  // of a CTA; 1 KB more is kept for it
     CLA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    *room = most;
+    if (room) room->store(most, std::memory_order_relaxed);
     return CLA_OK;
   });
 }
@@ -1226,7 +1227,7 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
     }
   const int np = KIND == GK_GATE ? 2 : 1, products = KIND == GK_PAIR ? 2 : 1;
   static OncePerDevice oncePair, onceFew;
-  static int roomPair;
+  static std::atomic<int> roomPair;
   if (p.large) {
     A.wide = p.wide;
     A.stages = std::min(GP_STAGES, GP_RING / ((int)GM_OPERAND + (KIND == GK_GATE ? p.wide : p.wide / 2) * 128));
@@ -1236,7 +1237,7 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
     if (const int64_t e = all_smem(oncePair, &roomPair, c.device, k_gemm_pair<KIND, O>); e < 0) return e;
     static_assert(GP_RING + 1024 + 8 * 4096 <= 226 * 1024, "the ring and the warps' rooms fit");
     const unsigned ctas = 2 * (unsigned)std::min<int64_t>((int64_t)A.tilesM * A.tilesN, GM_SMS / 2);
-    EarlyLaunch pair(ctas, 128 + gp_out(KIND) * 32, roomPair, s, c.after != AFTER_CALL);
+    EarlyLaunch pair(ctas, 128 + gp_out(KIND) * 32, roomPair.load(std::memory_order_relaxed), s, c.after != AFTER_CALL);
     CLA_CUDA(cudaLaunchKernelEx(&pair.cfg, k_gemm_pair<KIND, O>, A));
     return CLA_OK;
   }
@@ -1249,8 +1250,7 @@ static int64_t launch_kind(GemmArgs& A, cudaStream_t s) {
   A.idesc = base | (uint32_t)c.b[0].mn << 15 | (uint32_t)c.a[0].mn << 16 | (uint32_t)(A.nc >> 3) << 17 | (128u >> 4) << 24;
   static_assert(GF_RING + 1024 <= 226 * 1024, "the ring fits");
   const auto few = [&](auto kernel, OncePerDevice& once) -> int64_t {
-    int room;
-    if (const int64_t e = all_smem(once, &room, c.device, kernel); e < 0) return e;
+    if (const int64_t e = all_smem(once, nullptr, c.device, kernel); e < 0) return e;
     // (all but 5 KB: CTAs of k_gemm_join may wait next to it, none with tensor memory)
     EarlyLaunch l(p.ctas, GF_T, GF_RING + 1024, s, c.after != AFTER_CALL);
     CLA_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, A));
@@ -1281,8 +1281,7 @@ static int64_t launch_rows(GemmArgs& A, cudaStream_t s) {
   A.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.wide >> 3) << 17 | (128u >> 4) << 24;
   if (const int64_t rc = operand_map(A.b[0], c.b[0], CLA_T_I8, c.N, c.K, p.wide); rc < 0) return rc;
   const auto go = [&](auto kernel, OncePerDevice& once) -> int64_t {
-    int room;
-    if (const int64_t e = all_smem(once, &room, c.device, kernel); e < 0) return e;
+    if (const int64_t e = all_smem(once, nullptr, c.device, kernel); e < 0) return e;
     EarlyLaunch l((unsigned)std::min<int64_t>(GM_SMS, (c.M + GR_WARPS - 1) / GR_WARPS), GR_T, GR_ROOM, s, false);
     CLA_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, A));
     return CLA_OK;

@@ -1,6 +1,7 @@
 """What the dense operators refuse on the host, beyond test_dense.py, and how they are imported."""
 import ctypes as C
 import os
+import re
 import subprocess
 import sys
 
@@ -11,6 +12,7 @@ from systemds_b200 import CLAError, CLALibDecompress, CLALibQ8, CompressedMatrix
 from systemds_b200.dense import _drop, _type
 from systemds_b200.native import check
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 M, K, N = 6, 48, 48
 A, B, SA, SB, OUT, WORK, MORE = ((i + 1) << 24 for i in range(7))  # addresses that nothing reads: the calls below are refused on the host
 
@@ -109,6 +111,13 @@ def test_star_import(torch_is_there):
             f"assert ('CLALibQ8' in globals()) == {torch_is_there}\n"
             "try:\n    from systemds_b200 import CLALibDropout\n    there = True\nexcept ImportError:\n    there = False\n"
             f"assert there == {torch_is_there}\n")
-    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
-                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert r.returncode == 0, r.stderr
+
+
+def test_dense_launchers_share_no_plain_numbers():
+    """What threads share and write: atomics, marks of OncePerDevice, or each thread's own."""
+    for name in ("cla_dense.cu", "cla_dense.cuh", "cla_gemm.cu"):
+        with open(os.path.join(ROOT, "systemds_b200", "csrc", name)) as f:
+            found = re.findall(r"\bstatic\s+(?:bool|int|int32_t|int64_t|size_t|unsigned)\s+(\w+)\s*(?:;|=|\[)", f.read())
+        assert found == [], name

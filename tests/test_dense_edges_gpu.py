@@ -1,5 +1,8 @@
 """The dense operators on the GPU where a tail, another caller or an odd argument shows what the bounds of test_dense_gpu.py do not."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -178,3 +181,53 @@ def test_arguments_of_other_kinds_on_the_device():
             f()
     seed = torch.tensor(5)
     assert torch.equal(CLALibDropout.apply(x, torch.tensor(0.5), seed), CLALibDropout.apply(x, 0.5, 5))
+
+
+# ---- several host threads -----------------------------------------------------------------------------------------------
+THREADS = """
+import threading, torch
+from systemds_b200 import CLALibDropout, CLALibGated, CLALibQ8
+from systemds_b200.dense import status
+torch.cuda.init()
+inputs = []
+for i, (M, D, F) in enumerate([(1, 512, 900), (40, 300, 700), (700, 264, 333), (2000, 128, 512), (300, 64, 2500), (3000, 200, 64)]):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(i)
+    make = lambda *s: torch.randn(*s, device="cuda", generator=g).half()
+    inputs.append((make(M, D), make(D, F) / 16, make(D, F) / 16, make(M, F), torch.randint(-127, 128, (F, D), dtype=torch.int8, device="cuda", generator=g),
+                   torch.rand(F, device="cuda", generator=g)))
+torch.cuda.synchronize()
+
+def work(k):
+    x, wg, wu, dh, b, s = inputs[k % len(inputs)]
+    h, g, u = CLALibGated.forward(x, wg, wu, "gelu", p=0.1, seed=3, save=True)
+    return (h, CLALibQ8.linear(x, b, s), CLALibDropout.apply(x, 0.5, 7)) + CLALibQ8.quantizeCols(wg) + CLALibGated.backward(dh, x, wg, wu, g, u, "gelu", p=0.1, seed=3)
+
+got, start = {}, threading.Barrier(8)
+
+def run(t):
+    stream = torch.cuda.Stream()
+    start.wait()
+    with torch.cuda.stream(stream):
+        for turn in range(12):
+            got[t, turn] = work(t + turn)
+    stream.synchronize()
+
+threads = [threading.Thread(target=run, args=(t,)) for t in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+want = [work(k) for k in range(len(inputs))]
+assert len(got) == 96
+for (t, turn), r in got.items():
+    assert all(torch.equal(p, q) for p, q in zip(r, want[(t + turn) % len(inputs)])), (t, turn)
+status()
+print("ok")
+"""
+
+
+def test_first_calls_of_several_threads():
+    """Eight host threads whose first calls in the process meet, a stream each: the results of calls one after another."""
+    r = subprocess.run([sys.executable, "-c", THREADS], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
