@@ -172,17 +172,10 @@ __device__ __forceinline__ void q8_quotients(const Q8Row<typename WideOf<T>::typ
 }
 
 // ---- the activation, in FP32 ------------------------------------------------------------------------------------------
-// Nothing here subtracts from 1 what has come near it: sigmoid(g) and sigmoid(-g) are both quotients of e = exp(-|g|), whose denominator is between 1 and
-// 2, and the normal distribution's share below -|g| is exp(-g^2 / 2) times a smooth function. So the tails keep their relative error, in units of 2^-23
-// (the fast exponential of x: 2 + 1.2 |x|, the fast quotient 2, the roundings of an argument x: |x|): SiLU and sigmoid 6 + 1.2 |g|, GELU 10 + 1.2 g^2,
-// its tanh form 6 + 3.2 |y| for sigmoid(y). Slopes two to three times that, of their terms' magnitudes. A rounding to 16 bits of 2^-8 or 2^-11 follows.
-struct Sigmoids {
-  float s, r;  // of g and of -g
-};
-__device__ __forceinline__ Sigmoids sigmoids_of(float g) {
-  const float e = __expf(-fabsf(g)), q = __fdividef(1.f, 1.f + e), t = e * q;
-  return g < 0.f ? Sigmoids{t, q} : Sigmoids{q, t};
-}
+// No tail is what is left of a 1: sigmoid(g) is a quotient of 1 or e = exp(-|g|), whose denominator is between 1 and 2, and the normal distribution's
+// share below -|g| is exp(-g^2 / 2) times a smooth function. So the tails keep their relative error, in units of 2^-23 (the fast exponential of x:
+// 2 + 1.2 |x|, the fast quotient 2, the roundings of an argument x: |x|): SiLU and sigmoid 6 + 1.2 |g|, GELU 10 + 1.2 g^2, its tanh form 6 + 3.2 |y|
+// for sigmoid(y). Slopes two to three times that, of their terms' magnitudes. A rounding to 16 bits of 2^-8 or 2^-11 follows.
 __device__ __forceinline__ float sigmoid_of(float g) {
   const float e = __expf(-fabsf(g));
   return __fdividef(g < 0.f ? e : 1.f, 1.f + e);
@@ -221,14 +214,14 @@ __device__ __forceinline__ float act_value(int act, float g) {
 __device__ __forceinline__ float act_slope(int act, float g, float& value) {
   switch (act) {
     case CLA_ACT_SILU: {
-      const Sigmoids v = sigmoids_of(g);
-      value = g * v.s;
-      return v.s * (1.f + g * v.r);
+      const float s = sigmoid_of(g);
+      value = g * s;
+      return s * (1.f + g * (1.f - s));  // (where 1 - s cancels it is next to the 1: off by |g| / 2 units, and 0 from g = 17 on)
     }
     case CLA_ACT_SIGMOID: {
-      const Sigmoids v = sigmoids_of(g);
-      value = v.s;
-      return v.s * v.r;
+      const float e = __expf(-fabsf(g)), q = __fdividef(1.f, 1.f + e);
+      value = g < 0.f ? e * q : q;
+      return e * q * q;  // (of g and -g: the same)
     }
     case CLA_ACT_RELU: value = g < 0.f ? 0.f : g; return g > 0.f ? 1.f : 0.f;
     case CLA_ACT_GELU: {
@@ -237,9 +230,9 @@ __device__ __forceinline__ float act_slope(int act, float g, float& value) {
       return v.share + g * v.e * 0.39894228040143268f;
     }
     default: {
-      const Sigmoids v = sigmoids_of(gelu_arg(g));
-      value = g * v.s;
-      return v.s + g * v.s * v.r * 1.5957691216057308f * (1.f + 0.134145f * fminf(g * g, 1e4f));  // (beyond, s or r is 0, and the square may be infinite)
+      const float s = sigmoid_of(gelu_arg(g));
+      value = g * s;
+      return s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * fminf(g * g, 1e4f));  // (beyond, 1 - s or s is 0, and the square may be infinite)
     }
   }
 }
