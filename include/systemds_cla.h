@@ -338,7 +338,7 @@ int64_t cla_q8_mm_dev(const cla_q8* args, void* stream);
  * neither), as the backward call takes them.
  * Backward: from dh [M x F] and the saved g, u: with dh' = dropout(dh) of the same (seed, step), du = dh' act(g), dg = dh' u act'(g),
  * dx = dg t(wg) + du t(wu), dwg = t(x) dg, dwu = t(x) du. dx or both of dwg, dwu may be NULL (not wanted). dg and du are
- * rounded to the type before the products, which take operands of that type.
+ * rounded to the type before the products, which take operands of that type (F16: beyond 65504 they become infinite; scale dh to avoid it).
  * wTrans 1: wg and wu are stored transposed, as [F x D] rows of ldwg, ldwu elements. dwg and dwu are [D x F] in any case. */
 typedef struct cla_gated {
   int64_t M, D, F;

@@ -331,6 +331,9 @@ __global__ void __launch_bounds__(1024) k_quantize_cols(const T* __restrict__ x,
 }
 
 // ---- the gated block's elementwise gradients ----------------------------------------------------------------------------
+// dG and dU in FP32, rounded to the type once: the products that follow take operands of 16 bits, and FP32 ones would pass through the tensor
+// cores in three parts, three times the work. It costs the gradients 1.4 times the error of FP32 operands (relative, 64 bits compared: BF16 0.0023
+// against 0.0017, FP16 0.00029 against 0.00021).
 // (the next row's values are on their way while a row's are worked on)
 template <class T, bool VEC>
 __global__ void __launch_bounds__(DN_T, 3) k_gate_grad(const T* __restrict__ dh, int64_t lddh, const T* __restrict__ g, int64_t ldg,

@@ -221,7 +221,8 @@ class CLALibQ8:
 
 class CLALibGated:
     """``H = dropout(act(X Wg) * (X Wu))`` in bfloat16 or float16 with sums in FP32, and its gradients. ``act``: "silu", "gelu" (erf),
-    "gelu_tanh", "relu" or "sigmoid". Weights [D x F], or transposed views of [F x D] tensors (both alike)."""
+    "gelu_tanh", "relu" or "sigmoid". Weights [D x F], or transposed views of [F x D] tensors (both alike). Nothing is recorded for autograd, also
+    where operands require gradients: they are what ``backward`` returns."""
 
     @staticmethod
     def _args(x, wGate, wUp, act, p, seed, step, row0):
